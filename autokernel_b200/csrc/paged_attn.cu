@@ -1,0 +1,174 @@
+// Attention of packed new tokens over a paged key/value cache: entry point and the SIMT kernel
+// that takes every type, head dimension, stride and page size.
+//
+//   o[t, h] = sum_{j < vis(t)} softmax_j(scale q[t, h] . K[j, h / G]) V[j, h / G],  G = H / Hkv,
+//   vis(t) = position(t) + 1 (causal) or kv_lens[b].
+// A row that sees no key is 0.  A row that would see a key without a page (paged.cuh) is NaN.
+#include "paged_attn.cuh"
+
+namespace ak {
+namespace paged {
+
+// One CTA per (token, head): 32 groups of eight lanes each take every 32nd key with a running
+// maximum and sum of their own, and are joined through shared memory at the end, so nothing is
+// exchanged while keys are read.  The eight lanes split the head dimension (element
+// lane + 8 i), which coalesces to whole 32-byte sectors in fp32 at any alignment.
+template <int DT, int NI>
+__global__ void __launch_bounds__(256) simt_kernel(const AttnArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  const int t = blockIdx.x, h = blockIdx.y, hk = h / a.G;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane & 7, grp = threadIdx.x >> 3;
+  __shared__ int s_seq;
+  if (warp == 0) {
+    const int b = seq_of_token_warp(a.l, t);
+    if (lane == 0) s_seq = b;
+  }
+  __syncthreads();
+  const int b = s_seq;
+  if (b < 0 || b >= a.l.B) return;
+  const SeqRange r = seq_range(a.l, b);
+  if (t < r.begin || t >= r.begin + r.n) return;
+  const int vis = visible_keys(r, t - r.begin, a.causal);
+
+  float q[NI], o[NI];
+  const T* qp = reinterpret_cast<const T*>(a.q) + t * a.qs[0] + h * a.qs[1];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int d = sub + 8 * i;
+    q[i] = d < a.D ? E::to_f(qp[d]) : 0.f;
+    o[i] = 0.f;
+  }
+  float m = -INFINITY, sum = 0.f;
+  bool missing = false;
+  for (int j = grp; j < vis; j += 32) {
+    const int pi = j / a.l.page_size, slot = j - pi * a.l.page_size;
+    const int page = page_of(a.l, b, pi);
+    if (page < 0) {
+      missing = true;
+      break;
+    }
+    const T* kp = reinterpret_cast<const T*>(a.k) + page * a.kcs[0] + hk * a.kcs[1] + slot * a.kcs[2];
+    const T* vp = reinterpret_cast<const T*>(a.v) + page * a.vcs[0] + hk * a.vcs[1] + slot * a.vcs[2];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int d = sub + 8 * i;
+      if (d < a.D) s = fmaf(q[i], E::to_f(kp[d]), s);
+    }
+    const unsigned mask = 0xffu << (lane & 24);
+#pragma unroll
+    for (int x = 4; x > 0; x >>= 1) s += __shfl_xor_sync(mask, s, x);
+    const float mn = fmaxf(m, s);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    const float alpha = exp2f((m - ref) * a.scale_log2), p = exp2f((s - ref) * a.scale_log2);
+    m = mn;
+    sum = sum * alpha + p;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int d = sub + 8 * i;
+      if (d < a.D) o[i] = fmaf(p, E::to_f(vp[d]), o[i] * alpha);
+    }
+  }
+  missing = __syncthreads_or(missing);
+
+  // join the 32 groups
+  __shared__ float s_m[32], s_l[32];
+  __shared__ float s_o[8][8 * NI];
+  if (sub == 0) {
+    s_m[grp] = m;
+    s_l[grp] = sum;
+  }
+  __syncthreads();
+  const float top = warp_max(s_m[lane]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  const float total = warp_sum(s_l[lane] * exp2f((s_m[lane] - ref) * a.scale_log2));
+  const float w = exp2f((m - ref) * a.scale_log2);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    float x = o[i] * w;
+    x += __shfl_xor_sync(0xffffffffu, x, 8);
+    x += __shfl_xor_sync(0xffffffffu, x, 16);
+    if (lane < 8) s_o[warp][sub + 8 * i] = x;
+  }
+  __syncthreads();
+  T* op = reinterpret_cast<T*>(a.o) + t * a.os[0] + h * a.os[1];
+  for (int d = threadIdx.x; d < a.D; d += blockDim.x) {
+    float x = 0.f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) x += s_o[y][d];
+    op[d] = E::from_f(missing ? __int_as_float(0x7fffffff) : total == 0.f ? 0.f : x / total);
+  }
+}
+
+template <int DT>
+static int run_simt(const AttnArgs& a, cudaStream_t st) {
+  const dim3 grid((unsigned)a.l.N, (unsigned)a.H);
+  if (a.D <= 64)
+    simt_kernel<DT, 8><<<grid, 256, 0, st>>>(a);
+  else if (a.D <= 128)
+    simt_kernel<DT, 16><<<grid, 256, 0, st>>>(a);
+  else
+    simt_kernel<DT, 32><<<grid, 256, 0, st>>>(a);
+  return launch_status("paged_attention");
+}
+
+}  // namespace paged
+}  // namespace ak
+
+using namespace ak;
+
+extern "C" size_t ak_paged_attention_workspace_size(int64_t H, int64_t Hkv, int64_t D, int dtype) {
+  return 16;
+}
+
+extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void* v_cache,
+                                  void* out, const int32_t* page_table, const int32_t* cu_q,
+                                  const int32_t* kv_lens, int64_t N, int64_t B, int64_t H,
+                                  int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size,
+                                  int64_t max_pages, int64_t table_ld, const int64_t* q_strides,
+                                  const int64_t* out_strides, const int64_t* k_cache_strides,
+                                  const int64_t* v_cache_strides, int causal, float sm_scale,
+                                  int dtype, void* workspace, size_t ws_bytes, void* stream) {
+  AK_REQUIRE(dtype_ok(dtype), AK_ERR_DTYPE, "unsupported dtype %d", dtype);
+  AK_REQUIRE(N >= 0 && B >= 0 && H > 0 && Hkv > 0 && D > 0 && num_pages >= 0 && page_size > 0 &&
+                 max_pages >= 0 && table_ld >= 0,
+             AK_ERR_SHAPE, "bad shape");
+  AK_REQUIRE(H % Hkv == 0, AK_ERR_SHAPE, "query heads %lld not a multiple of kv heads %lld",
+             (long long)H, (long long)Hkv);
+  AK_REQUIRE(D <= 256, AK_ERR_SHAPE, "head_dim %lld exceeds 256", (long long)D);
+  AK_REQUIRE(N < (1LL << 31) && B < (1LL << 31) - 64 && H <= 65535 && num_pages < (1LL << 31) &&
+                 page_size < (1LL << 31) && max_pages < (1LL << 31),
+             AK_ERR_SHAPE, "dimension too large");
+  AK_REQUIRE(sm_scale > 0.f && sm_scale <= 3.0e38f, AK_ERR_ARG,
+             "sm_scale must be positive and finite");
+  if (N == 0 || B == 0) return AK_OK;
+  AK_REQUIRE(q && k_cache && v_cache && out && page_table && cu_q && kv_lens && q_strides &&
+                 out_strides && k_cache_strides && v_cache_strides,
+             AK_ERR_ARG, "null pointer");
+  AK_REQUIRE(workspace && ws_bytes >= ak_paged_attention_workspace_size(H, Hkv, D, dtype),
+             AK_ERR_ARG, "workspace too small");
+  paged::AttnArgs a{};
+  a.l = PagedLists{page_table, cu_q,           kv_lens,        table_ld,      (int)N,
+                   (int)B,     (int)max_pages, (int)num_pages, (int)page_size};
+  a.q = q; a.k = k_cache; a.v = v_cache; a.o = out;
+  a.H = (int)H; a.Hkv = (int)Hkv; a.G = (int)(H / Hkv); a.D = (int)D;
+  a.causal = causal;
+  a.dtype = dtype;
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  for (int i = 0; i < 2; ++i) {
+    a.qs[i] = q_strides[i];
+    a.os[i] = out_strides[i];
+  }
+  for (int i = 0; i < 3; ++i) {
+    a.kcs[i] = k_cache_strides[i];
+    a.vcs[i] = v_cache_strides[i];
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (dtype) {
+    case AK_F32: return paged::run_simt<AK_F32>(a, st);
+    case AK_F16: return paged::run_simt<AK_F16>(a, st);
+    default: return paged::run_simt<AK_BF16>(a, st);
+  }
+}

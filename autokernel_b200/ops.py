@@ -1,6 +1,7 @@
-"""The nine operators of AutoKernel's kernel_fn contract, on libak_b200.so.
+"""The nine operators of AutoKernel's kernel_fn contract, on libak_b200.so, their fused
+neighbours, and what serving a model adds (paged_append, paged_attention, sample).
 
-Each function keeps the signature, argument meaning, output shape and output
+Each of the nine keeps the signature, argument meaning, output shape and output
 dtype of the reference oracle (reference.py) and of the reference starters'
 ``kernel_fn`` (kernels/<op>.py), so AutoKernel's bench.py / verify.py and
 model code can call them unchanged:
@@ -591,6 +592,193 @@ def flash_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, causal: b
     call("ak_flash_attention", Qc.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), O.data_ptr(), bh, Sq,
          Sk, D, 1 if causal else 0, float(sm_scale), dtype_code(Q.dtype), stream_ptr(Q.device))
     return O
+
+
+# ---------------------------------------------------------------- serving
+
+def _i64s(*v: int):
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+def _paged_lists(name: str, k_cache, v_cache, page_table, cu_q, kv_lens) -> tuple:
+    """Check the cache and the lists of a paged call; (B, Hkv, D)."""
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise ValueError(f"{name}: k_cache and v_cache must be [pages, kv_heads, page_size, head_dim] alike")
+    if k_cache.shape[2] == 0 or k_cache.shape[1] == 0 or k_cache.shape[3] == 0:
+        raise ValueError(f"{name}: empty page")
+    for c in (k_cache, v_cache):
+        if c.stride(3) != 1 and c.shape[3] > 1:
+            raise ValueError(f"{name}: the caches' last dim must be contiguous")
+    for what, t in (("page_table", page_table), ("cu_q", cu_q), ("kv_lens", kv_lens)):
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name}: {what} must be int32, got {t.dtype}")
+    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+    if B < 0 or cu_q.shape != (B + 1,) or page_table.dim() != 2 or page_table.shape[0] != B:
+        raise ValueError(f"{name}: need kv_lens [B], cu_q [B + 1] and page_table [B, pages per sequence]")
+    if not (cu_q.is_contiguous() and kv_lens.is_contiguous()) or (
+            page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"{name}: the lists (and the rows of page_table) must be contiguous")
+    return B, k_cache.shape[1], k_cache.shape[3]
+
+
+def _tokens(name: str, what: str, x: torch.Tensor, heads, like: torch.Tensor, n=None) -> None:
+    """x must be [N, heads, D] of the cache's dtype and head_dim with a contiguous last dim."""
+    if (x.dim() != 3 or x.shape[2] != like.shape[3] or (heads is not None and x.shape[1] != heads)
+            or (n is not None and x.shape[0] != n) or x.shape[1] == 0):
+        raise ValueError(f"{name}: {what} must be [N, heads, head_dim] to go with the cache "
+                         f"{tuple(like.shape)}, got {tuple(x.shape)}")
+    if x.dtype != like.dtype:
+        raise ValueError(f"{name}: {what} is {x.dtype}, the cache {like.dtype}")
+    if x.stride(2) != 1 and x.shape[2] > 1:
+        raise ValueError(f"{name}: the last dim of {what} must be contiguous")
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 page_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor,
+                 q: torch.Tensor | None = None, cos: torch.Tensor | None = None,
+                 sin: torch.Tensor | None = None,
+                 q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Write the new tokens' keys and values to their slots of a paged cache, rotating the keys
+    (and q) by their positions on the way, in one launch.
+
+    k, v: [N, Hkv, D] and q: [N, H, D], packed: tokens cu_q[b]..cu_q[b+1] are sequence b's;
+    k_cache, v_cache: [pages, Hkv, page_size, D]; page_table: int32 [B, M]; cu_q: int32 [B + 1];
+    kv_lens: int32 [B], each sequence's keys with the new ones.  Any strides with a contiguous last
+    dim.  cos, sin: fp32 [positions, D / 2] (a dim of 1 between, as llama.rope_tables gives them,
+    is fine) for the interleaved RoPE of rope_apply, or None to append as is.
+
+    Returns the rotated q (in q_out if given, which may be q itself), or None without q.  Tokens
+    behind cu_q[B] are left alone (a fresh result is not initialised there).  A key whose position
+    is negative or has no page in the table is not stored; positions outside cos / sin give NaN.
+    Two tokens of a call must not share a slot: what such a slot holds is undefined."""
+    name = "paged_append"
+    B, Hkv, D = _paged_lists(name, k_cache, v_cache, page_table, cu_q, kv_lens)
+    N = k.shape[0] if k.dim() == 3 else None
+    _tokens(name, "k", k, Hkv, k_cache)
+    _tokens(name, "v", v, Hkv, k_cache, N)
+    if D % 2:
+        raise ValueError(f"{name}: head_dim must be even, got {D}")
+    if q is not None:
+        _tokens(name, "q", q, None, k_cache, N)
+    elif q_out is not None:
+        raise ValueError(f"{name}: q_out without q")
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{name}: cos and sin go together")
+    if q is not None and cos is None:
+        raise ValueError(f"{name}: q is only rotated, so it needs cos and sin")
+    positions = 0
+    if cos is not None:
+        if (cos.shape != sin.shape or cos.dim() < 2 or cos.shape[-1] != D // 2
+                or cos.numel() != cos.shape[0] * (D // 2) or cos.shape[0] == 0):
+            raise ValueError(f"{name}: cos and sin must be [positions, {D // 2}]")
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            raise ValueError(f"{name}: cos and sin must be float32")
+        if not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError(f"{name}: cos and sin must be contiguous")
+        positions = cos.shape[0]
+    if q_out is not None:
+        _tokens(name, "q_out", q_out, q.shape[1], k_cache, N)
+    code = dtype_code(k_cache.dtype)
+    require_cuda(k_cache, *(t for t in (k, v, v_cache, page_table, cu_q, kv_lens, q, cos, sin, q_out)
+                            if t is not None))
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    st = [_i64s(*t.stride()[:2]) if t is not None else None for t in (k, v, q, q_out)]
+    st += [_i64s(*t.stride()[:3]) for t in (k_cache, v_cache)]
+
+    def ptr(t):
+        return t.data_ptr() if t is not None else None
+
+    call("ak_paged_append", k.data_ptr(), v.data_ptr(), ptr(q), ptr(q_out), k_cache.data_ptr(),
+         v_cache.data_ptr(), page_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), ptr(cos),
+         ptr(sin), N, B, q.shape[1] if q is not None else 0, Hkv, D, k_cache.shape[0],
+         k_cache.shape[2], page_table.shape[1], page_table.stride(0), positions,
+         *st, code, stream_ptr(k.device))
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    page_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor,
+                    causal: bool = True, sm_scale: float | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of packed new tokens q [N, H, D] over a paged cache that already holds their keys
+    and values (paged_append; its arguments and layouts).  Token i of sequence b's n_b new ones
+    sees the keys up to its position kv_lens[b] - n_b + i, or all kv_lens[b] when not causal; one new
+    token per sequence is decoding.  H is a multiple of the cache's heads: query head h reads
+    key/value head h // (H // Hkv).  head_dim up to 256; sm_scale (D ** -0.5 by default) positive.
+
+    Returns [N, H, D] (written to out if given: any strides with a contiguous last dim).  A row that
+    sees no key is 0; one that sees a key without a page is NaN.  Rows behind cu_q[B] are left alone
+    (a fresh result is not initialised there).  Nothing behind a sequence's last key matters,
+    whatever the cache holds there."""
+    name = "paged_attention"
+    B, Hkv, D = _paged_lists(name, k_cache, v_cache, page_table, cu_q, kv_lens)
+    _tokens(name, "q", q, None, k_cache)
+    N, H, _ = q.shape
+    if H % Hkv:
+        raise ValueError(f"{name}: {H} query heads are not a multiple of {Hkv} key/value heads")
+    if D > 256:
+        raise ValueError(f"{name}: head_dim {D} exceeds 256")
+    if sm_scale is None:
+        sm_scale = D ** -0.5
+    if not 0 < sm_scale <= 3e38:
+        raise ValueError(f"{name}: sm_scale must be positive and finite, got {sm_scale}")
+    if out is not None:
+        _tokens(name, "out", out, H, k_cache, N)
+    code = dtype_code(k_cache.dtype)
+    require_cuda(q, k_cache, v_cache, page_table, cu_q, kv_lens, *([out] if out is not None else []))
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    ws = torch.empty(_lib.load().ak_paged_attention_workspace_size(H, Hkv, D, code),
+                     dtype=torch.uint8, device=q.device)
+    st = [_i64s(*t.stride()[:2]) for t in (q, o)] + [_i64s(*t.stride()[:3]) for t in (k_cache, v_cache)]
+    call("ak_paged_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
+         page_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), N, B, H, Hkv, D,
+         k_cache.shape[0], k_cache.shape[2], page_table.shape[1], page_table.stride(0), *st,
+         1 if causal else 0, float(sm_scale), code, ws.data_ptr(), ws.numel(), stream_ptr(q.device))
+    return o
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: float | torch.Tensor = 1.0,
+           top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
+           min_p: float | torch.Tensor = 0.0) -> torch.Tensor:
+    """One token (int64) per row of logits [rows, vocab], drawn with the uniform numbers u (fp32
+    [rows], cut to [0, 1)); every sum is taken in 64 bits.
+
+    Entries are ordered by logit, largest first, equal ones by index; with the weights
+    exp((x - max) / temperature) the entries kept are the first top_k (0: all), of those the ones
+    whose predecessors weigh less than top_p of the first top_k (1: all; the first always), and of
+    those the ones that weigh at least min_p times the largest (0: all).  The token is the lowest
+    index whose kept weights up to it exceed u times all kept weights.  temperature 0 takes the
+    largest logit, lowest index.  Each setting is a number (taken as fp32) or a tensor [rows]
+    (fp32; top_k int32).  NaN and -inf logits are never drawn (a row of nothing else gives -1);
+    entries of +inf share all weight."""
+    name = "sample"
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"{name}: logits must be [rows, vocab], got {tuple(logits.shape)}")
+    rows = logits.shape[0]
+    if u.shape != (rows,) or u.dtype != torch.float32:
+        raise ValueError(f"{name}: u must be float32 [{rows}]")
+    code = dtype_code(logits.dtype)
+    settings = []
+    for what, v, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(v, torch.Tensor):
+            if v.shape != (rows,) or v.dtype != dt:
+                raise ValueError(f"{name}: a tensor of {what} must be {dt} [{rows}]")
+            settings.append(v.contiguous())
+        else:
+            settings.append(min(int(v), 2 ** 31 - 1) if dt == torch.int32 else float(v))
+            if settings[-1] < 0 or settings[-1] != settings[-1]:
+                raise ValueError(f"{name}: {what} must not be negative, got {v}")
+    require_cuda(logits, u, *(v for v in settings if isinstance(v, torch.Tensor)))
+    x = logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
+    u = u.contiguous()
+    out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    arrays = [v.data_ptr() if isinstance(v, torch.Tensor) else None for v in settings]
+    numbers = [0 if isinstance(v, torch.Tensor) else v for v in settings]
+    call("ak_sample", x.data_ptr(), u.data_ptr(), rows, x.shape[1], x.stride(0), code, *arrays,
+         *numbers, out.data_ptr(), stream_ptr(logits.device))
+    return out
 
 
 OPS = {

@@ -260,6 +260,62 @@ AK_API int ak_flash_attention_strided(const void* Q, const void* K, const void* 
                                       const int64_t* o_strides, int causal, float sm_scale,
                                       int dtype, void* stream);
 
+/* ----------------------------------------------------------------- serving */
+
+/* Shared by the two cache operators.  N packed tokens of B sequences: tokens cu_q[b] ..
+ * cu_q[b+1]-1 are sequence b's n_b new tokens (cu_q [B+1], ascending), kv_lens[b] its keys with
+ * the new ones, so its i-th token sits at position kv_lens[b] - n_b + i.  Position p lies in slot
+ * p % page_size of page page_table[b * table_ld + p / page_size] (rows of max_pages entries).
+ * k_cache / v_cache are [num_pages, Hkv, page_size, D] by element strides {page, head, slot};
+ * k, v, q and out are [N, heads, D] by element strides {token, head}; D is contiguous.  The
+ * lists are device memory and are not checked by the host: token ranges are cut to [0, N), and a
+ * key whose page index is not below max_pages or whose page is not in [0, num_pages) has no page.
+ * Tokens before cu_q[0] or behind cu_q[B] are neither read into a cache nor written to an output.
+ * Fused neighbours of models/llama_7b.py:67-88 (RoPE, then attention) for cached decoding, which
+ * the reference does not have. */
+
+/* k_cache / v_cache at each token's position = rot(k), v; q_out (with q) = rot(q).  rot is the
+ * interleaved RoPE of ak_rotary_embedding with fp32 cos / sin [positions, D / 2] (one rounding);
+ * without tables it copies.  Positions outside the tables give NaN; keys without a page (or at
+ * a negative position) are not stored.  q may be NULL; q_out may be q.  Two tokens of one call
+ * must not name the same slot. */
+AK_API int ak_paged_append(const void* k, const void* v, const void* q, void* q_out, void* k_cache,
+                    void* v_cache, const int32_t* page_table, const int32_t* cu_q,
+                    const int32_t* kv_lens, const float* cos, const float* sin, int64_t N,
+                    int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t num_pages,
+                    int64_t page_size, int64_t max_pages, int64_t table_ld, int64_t positions,
+                    const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
+                    const int64_t* q_out_strides, const int64_t* k_cache_strides,
+                    const int64_t* v_cache_strides, int dtype, void* stream);
+
+/* out[t, h] = softmax(q[t, h] . K^T * sm_scale) V over the keys that token t sees: all up to its
+ * position (causal) or all kv_lens[b].  Query head h reads key/value head h / (H / Hkv).  A row
+ * that sees no key (or only scores of -inf) is 0; a row that sees a key without a page is NaN.
+ * What the cache holds behind a sequence's last key never matters.  D <= 256, sm_scale > 0.
+ * workspace: ak_paged_attention_workspace_size bytes, used by this call alone until it is done. */
+AK_API size_t ak_paged_attention_workspace_size(int64_t H, int64_t Hkv, int64_t D, int dtype);
+AK_API int ak_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* out,
+                       const int32_t* page_table, const int32_t* cu_q, const int32_t* kv_lens,
+                       int64_t N, int64_t B, int64_t H, int64_t Hkv, int64_t D,
+                       int64_t num_pages, int64_t page_size, int64_t max_pages, int64_t table_ld,
+                       const int64_t* q_strides, const int64_t* out_strides,
+                       const int64_t* k_cache_strides, const int64_t* v_cache_strides, int causal,
+                       float sm_scale, int dtype, void* workspace, size_t ws_bytes, void* stream);
+
+/* out[r] = one token of row r of logits [rows, vocab], drawn with the uniform number u[r]; all
+ * sums in 64 bits.  Weights exp((x - max) / T); in the order (logit descending, index ascending)
+ * the first min(top_k, n_p, n_m) entries are kept, n_p = those whose predecessors weigh less than
+ * top_p times the first top_k entries, n_m = those with a weight of at least min_p; the token is
+ * the lowest index whose kept weights up to it exceed u times the kept weight.  Settings per
+ * row (arrays, may be NULL) or one for all rows.  T <= 0 or NaN: the largest logit (lowest index);
+ * top_k <= 0: all; top_p >= 1: all, <= 0 or NaN: the first; min_p <= 0 or NaN: all, above 1 as 1.
+ * u is cut to [0, 1).  NaN and -inf logits are never drawn; a row with no other gives -1; entries of
+ * +inf share all weight. */
+AK_API int ak_sample(const void* logits, const float* u, int64_t rows, int64_t vocab, int64_t ld,
+              int dtype, const float* temperatures, const int32_t* top_ks, const float* top_ps,
+              const float* min_ps, float temperature, int32_t top_k, float top_p, float min_p,
+              int64_t* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
