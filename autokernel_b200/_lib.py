@@ -58,7 +58,7 @@ SIGNATURES = {
     "ak_flash_attention_strided": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
                                           _vp, _vp, _vp, _vp, _i32, _f32, _i32, _vp]),
     "ak_paged_append": (_i32, [_vp] * 11 + [_i64] * 10 + [_vp] * 6 + [_i32, _vp]),
-    "ak_paged_attention_workspace_size": (_sz, [_i64, _i64, _i64, _i32]),
+    "ak_paged_attention_workspace_size": (_sz, [_i64] * 5 + [_i32]),
     "ak_paged_attention": (_i32, [_vp] * 7 + [_i64] * 9 + [_vp] * 4 + [_i32, _f32, _i32, _vp, _sz, _vp]),
     "ak_sample": (_i32, [_vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _f32, _i32, _f32, _f32,
                          _vp, _vp]),

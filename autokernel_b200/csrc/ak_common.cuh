@@ -180,6 +180,8 @@ struct FastDiv {
   AK_D uint32_t mod(uint32_t n) const { return n - div(n) * d; }
 };
 
+bool force_simt();  // contract.cu: the SIMT kernels are asked for
+
 struct DeviceInfo {
   int sm_count;
   int max_smem_optin;

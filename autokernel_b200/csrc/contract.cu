@@ -23,6 +23,7 @@ static int g_force_simt = [] {
   const char* e = getenv("AK_FORCE_SIMT");
   return (e && e[0] == '1') ? 1 : 0;
 }();
+bool force_simt() { return g_force_simt != 0; }
 }  // namespace ak
 
 using namespace ak;

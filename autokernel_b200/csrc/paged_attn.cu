@@ -114,13 +114,36 @@ static int run_simt(const AttnArgs& a, cudaStream_t st) {
   return launch_status("paged_attention");
 }
 
+// The tensor-core kernels read pages by TMA (16-byte multiples, boxes of at least the eight slots of a
+// swizzle atom) and lay all tiles on one 64-bit line.
+static bool tc_ok(const AttnArgs& a) {
+  if (force_simt() || a.dtype == AK_F32 || (a.D != 64 && a.D != 128) || a.l.page_size % 8 || a.G > 128)
+    return false;
+  if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.o)) return false;
+  if (a.l.num_pages == 0) return false;
+  auto ok = [](int64_t size, int64_t stride) {
+    return size <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1LL << 38));
+  };
+  const int64_t cache[3] = {a.l.num_pages, a.Hkv, a.l.page_size}, tokens[2] = {a.l.N, a.H};
+  for (int i = 0; i < 3; ++i)
+    if (!ok(cache[i], a.kcs[i]) || !ok(cache[i], a.vcs[i])) return false;
+  for (int i = 0; i < 2; ++i)
+    if (!ok(tokens[i], a.qs[i]) || !ok(tokens[i], a.os[i])) return false;
+  const double keys = (double)a.l.max_pages * a.l.page_size;
+  if (((double)a.l.N * a.G + a.l.B) * a.Hkv * ((keys < 2147483647.0 ? keys : 2147483647.0) + 1024) > 4e18)
+    return false;
+  return device_info().cc_major == 10;
+}
+
 }  // namespace paged
 }  // namespace ak
 
 using namespace ak;
 
-extern "C" size_t ak_paged_attention_workspace_size(int64_t H, int64_t Hkv, int64_t D, int dtype) {
-  return 16;
+extern "C" size_t ak_paged_attention_workspace_size(int64_t N, int64_t B, int64_t H, int64_t Hkv,
+                                                    int64_t D, int dtype) {
+  if (dtype == AK_F32 || (D != 64 && D != 128)) return 0;
+  return paged::decode_workspace((int)D);
 }
 
 extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void* v_cache,
@@ -147,8 +170,9 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
   AK_REQUIRE(q && k_cache && v_cache && out && page_table && cu_q && kv_lens && q_strides &&
                  out_strides && k_cache_strides && v_cache_strides,
              AK_ERR_ARG, "null pointer");
-  AK_REQUIRE(workspace && ws_bytes >= ak_paged_attention_workspace_size(H, Hkv, D, dtype),
-             AK_ERR_ARG, "workspace too small");
+  const size_t need = ak_paged_attention_workspace_size(N, B, H, Hkv, D, dtype);
+  AK_REQUIRE(need == 0 || (workspace && aligned16(workspace) && ws_bytes >= need), AK_ERR_ARG,
+             "workspace of %zu bytes (16-byte aligned) needed, %zu given", need, ws_bytes);
   paged::AttnArgs a{};
   a.l = PagedLists{page_table, cu_q,           kv_lens,        table_ld,      (int)N,
                    (int)B,     (int)max_pages, (int)num_pages, (int)page_size};
@@ -166,6 +190,7 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
     a.vcs[i] = v_cache_strides[i];
   }
   cudaStream_t st = (cudaStream_t)stream;
+  if (paged::tc_ok(a)) return paged::run_decode(a, workspace, st);
   switch (dtype) {
     case AK_F32: return paged::run_simt<AK_F32>(a, st);
     case AK_F16: return paged::run_simt<AK_F16>(a, st);

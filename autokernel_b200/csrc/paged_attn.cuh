@@ -1,6 +1,7 @@
 // Arguments of one paged attention call, shared by the C ABI and the kernels.
 #pragma once
 #include "paged.cuh"
+#include "sm100.cuh"
 
 namespace ak {
 namespace paged {
@@ -19,6 +20,52 @@ struct AttnArgs {
 // Keys that the i-th new token of a sequence sees.
 AK_D int visible_keys(const SeqRange& r, int i, int causal) {
   return causal ? max(r.kv_len - r.n + i + 1, 0) : r.kv_len;
+}
+
+// paged_decode.cu: 16 query rows per tile, all keys read once; paged_chunk.cu: 128-row tensor-core tiles.
+int run_decode(const AttnArgs& a, void* ws, cudaStream_t st);
+size_t decode_workspace(int D);
+
+inline int gcd_int(int x, int y) {
+  while (y) {
+    const int r = x % y;
+    x = y;
+    y = r;
+  }
+  return x;
+}
+
+// 4-D map over a cache [pages, heads, slots, D]: boxes of `box` slots x 64 elements of one page.
+inline bool cache_tmap(CUtensorMap* m, const AttnArgs& a, const void* base, const int64_t* st,
+                       int box) {
+  const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)a.l.page_size, (uint64_t)a.Hkv,
+                            (uint64_t)a.l.num_pages};
+  uint64_t strides[3];
+  for (int i = 0; i < 3; ++i)  // a dim of one element may carry any stride
+    strides[i] = (uint64_t)(dims[i + 1] > 1 ? st[2 - i] : a.D) * 2;
+  const uint32_t b[4] = {64, (uint32_t)box, 1, 1};
+  return make_tmap(m, a.dtype, 4, base, dims, strides, b);
+}
+
+// Launch a kernel that may begin while its predecessor on the stream finishes (it waits for it
+// with griddepcontrol.wait before it reads what that one wrote).
+template <class... P, class... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    set_error("paged_attention: launch failed: %s", cudaGetErrorString(e));
+    return AK_ERR_LAUNCH;
+  }
+  return AK_OK;
 }
 
 }  // namespace paged

@@ -1,0 +1,462 @@
+// Paged attention of few query rows per sequence (decoding) for sm_100a: 16-bit types, D 64 or 128.
+//
+// Bound by reading the live keys and values once (4 D bytes per key and key/value head in 16-bit
+// types); the matrix work is small, so it runs on warp-level MMAs whose operands come from shared
+// memory, and everything else serves keeping loads in flight.  A tile is 16 query rows: the
+// heads of one key/value head's group (and the next tokens) share every key that is read.
+//   warp 0      TMA producer: a ring of {K, V} blocks of 64 keys, gathered page by page
+//               (a box is gcd(page_size, 64) slots of one page; 128-byte swizzle)
+//   warps 1..8  two groups of four take alternate blocks, a warp 16 keys of its block, each with
+//               its own running maximum, sum and output, joined through shared memory per segment
+// One CTA per SM; the line of paged_sched.cuh gives each the same number of keys.
+//
+// P = exp2(S scale log2e - m) is split into two 16-bit terms for P V (P = hi + lo, 16 bits of P kept):
+// the matrix units have time to spare here, and it leaves one rounding, that of the result.
+#include "paged_sched.cuh"
+#include "sm100.cuh"
+
+namespace ak {
+namespace paged {
+
+using namespace sm100;
+
+constexpr int kRows = 16, kBlk = 64, kWarps = 8, kThreads = 32 * (kWarps + 1);
+constexpr int kChunk = kBlk * 128;  // 64 keys x 64 16-bit elements
+
+template <int D>
+struct DecodeCfg {
+  static constexpr int NC = D / 64;
+  static constexpr int HALF = NC * kChunk;       // K or V of one block
+  static constexpr int STAGE = 2 * HALF;
+  static constexpr int STAGES = 160 * 1024 / STAGE;
+  static constexpr int O_OFF = STAGES * STAGE;   // float [8][16][D]
+  static constexpr int SMEM = O_OFF + kWarps * kRows * D * 4 + 1024;
+};
+
+static TileRule decode_rule() { return TileRule{kRows, 0, kBlk, 64, 256}; }
+
+static size_t decode_part_floats(int D) { return (size_t)kRows * (D + 2); }
+
+template <int DT>
+AK_D void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (DT == AK_BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+AK_D void ldmatrix4(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+AK_D void ldmatrix4t(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// (a, b) as 16-bit pairs hi + lo
+template <int DT>
+AK_D void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  if constexpr (DT == AK_BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  }
+}
+
+AK_D void group_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                  const __grid_constant__ AttnArgs a, const TileRule rule, int box,
+                  float* ws) {
+  using C = DecodeCfg<D>;
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int NF = D / 8;  // n8 tiles of the output
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~(uintptr_t)1023);
+  float* s_o = reinterpret_cast<float*>(smem + C::O_OFF);
+  __shared__ uint64_t full[C::STAGES], empty[C::STAGES];
+  __shared__ int s_bad[C::STAGES];  // first key of the block without a page
+  __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+  __shared__ int s_badw[kWarps];
+  __shared__ int s_again;           // rows to look at again (bits)
+  __shared__ int abort_flag, s_stop;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    abort_flag = 0;
+    s_again = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  const Line line = find_piece(a, rule, gridDim.x, blockIdx.x);
+  __syncthreads();
+  volatile int* abort_p = &abort_flag;
+  Walker walk(a, rule, line);
+  Segment s;
+  int g = 0;  // ring slots used so far
+
+  if (warp == 0) {  // ---------------------------------------------------- TMA producer
+    const int boxes = kBlk / box;
+    while (walk.next(s)) {
+      // this lane's page of block blk
+      auto page_at = [&](int blk) {
+        const int key = blk * kBlk + lane * box;
+        return lane < boxes && key < s.kv_hi ? page_of(a.l, s.b, key / a.l.page_size) : -2;
+      };
+      int ahead = s.blk0 < s.blk1 ? page_at(s.blk0) : -2;
+      for (int blk = s.blk0; blk < s.blk1; ++blk, ++g) {
+        const int st = g % C::STAGES, page = ahead;
+        if (blk + 1 < s.blk1) ahead = page_at(blk + 1);
+        const bool ok = mbar_wait(&empty[st], ((g / C::STAGES) & 1) ^ 1, abort_p);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const int key = blk * kBlk + lane * box;
+        const int bad = __reduce_min_sync(0xffffffffu, page == -1 ? key : 0x7fffffff);
+        if (lane == 0) {
+          s_bad[st] = bad;
+          mbar_expect_tx(&full[st], C::STAGE);
+        }
+        __syncwarp();
+        if (lane < boxes) {
+          // no page: the coordinate behind the last page, which reads as zeros
+          const int p = page < 0 ? a.l.num_pages : page;
+          const int slot = page < 0 ? 0 : key % a.l.page_size;
+          uint8_t* dst = smem + st * C::STAGE + lane * box * 128;
+#pragma unroll
+          for (int c = 0; c < C::NC; ++c) {
+            tma_load_4d(dst + c * kChunk, &tk, &full[st], c * 64, slot, s.h, p);
+            tma_load_4d(dst + C::HALF + c * kChunk, &tv, &full[st], c * 64, slot, s.h, p);
+          }
+        }
+      }
+      if (*abort_p) break;
+    }
+    // giving up: the copies in flight still land in this CTA's shared memory
+    if (*abort_p && lane == 0) drain_ring(full, C::STAGES, g);
+  } else {  // ---------------------------------------------------------------- consumers
+    const int cw = warp - 1, grp = cw >> 2, k16 = (cw & 3) * 16;  // the warp's keys of its blocks
+    const int r0 = lane >> 2, cq = 2 * (lane & 3);
+    const uint32_t ring = smem_u32(smem);
+    const int cap = capacity(a.l);
+    bool ok = true;
+    while (ok && walk.next(s)) {
+      const int64_t row0 = (int64_t)s.tile * kRows;
+      const int nr = (int)min((int64_t)kRows, (int64_t)s.r.n * a.G - row0);
+      const T* qrow[2];
+      int vis[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int rr = min(r0 + 8 * i, nr - 1);
+        const int t = (int)((row0 + rr) / a.G), hg = (int)((row0 + rr) % a.G);
+        qrow[i] = reinterpret_cast<const T*>(a.q) + (int64_t)(s.r.begin + t) * a.qs[0] +
+                  (int64_t)(s.h * a.G + hg) * a.qs[1];
+        vis[i] = visible_keys(s.r, t, a.causal);
+      }
+      uint32_t q[D / 16][4];
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          q[kk][i] = __ldg(reinterpret_cast<const unsigned int*>(qrow[i & 1] + kk * 16 + cq + (i >> 1) * 8));
+      float o[NF][4];
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      int bad = cap;
+      // every row of the tile sees keys below this
+      const int vis_all = visible_keys(s.r, s.t_lo, a.causal);
+      for (int blk = s.blk0; blk < s.blk1; ++blk, ++g) {
+        if ((g & 1) != grp) continue;
+        const int st = g % C::STAGES;
+        const bool got = mbar_wait(&full[st], (g / C::STAGES) & 1, abort_p);
+        if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
+        bad = min(bad, s_bad[st]);
+        const uint32_t kbase = ring + st * C::STAGE, vbase = kbase + C::HALF;
+        const int key0 = blk * kBlk + k16;
+        // S = Q K^T for 16 keys
+        float sc[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+          const int row = k16 + n * 8 + (lane & 7);
+#pragma unroll
+          for (int kk = 0; kk < D / 32; ++kk) {  // 32 dims a load
+            const int unit = (kk & 1) * 4 + (lane >> 3);
+            uint32_t kf[4];
+            ldmatrix4(kf, kbase + (kk >> 1) * kChunk + row * 128 + ((unit ^ (row & 7)) << 4));
+            mma16816<DT>(sc[n], q[2 * kk], kf[0], kf[1]);
+            mma16816<DT>(sc[n], q[2 * kk + 1], kf[2], kf[3]);
+          }
+        }
+        if (key0 + 16 > vis_all) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (key0 + n * 8 + cq + (j & 1) >= vis[j >> 1]) sc[n][j] = -INFINITY;
+        }
+        // running maximum, moved only when a block raises it by more than 8 (log2)
+        float alpha[2];
+        bool move = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          x *= a.scale_log2;
+          alpha[i] = 1.f;
+          if (x > m[i] + 8.f) {
+            alpha[i] = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - x);
+            m[i] = x;
+            move = true;
+          }
+        }
+        if (__any_sync(0xffffffffu, move)) {
+          l[0] *= alpha[0];
+          l[1] *= alpha[1];
+#pragma unroll
+          for (int i = 0; i < NF; ++i) {
+            o[i][0] *= alpha[0];
+            o[i][1] *= alpha[0];
+            o[i][2] *= alpha[1];
+            o[i][3] *= alpha[1];
+          }
+        }
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float ref = m[i] == -INFINITY ? 0.f : m[i];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const float x = ex2_approx(fmaf(sc[n][2 * i], a.scale_log2, -ref));
+            const float y = ex2_approx(fmaf(sc[n][2 * i + 1], a.scale_log2, -ref));
+            l[i] += x + y;
+            split2<DT>(x, y, ph[2 * n + i], pl[2 * n + i]);
+          }
+        }
+        // O += P V; keys behind the last visible one count as 0 whatever their slots hold
+        uint32_t mask[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int k = key0 + 8 * i + cq;
+          mask[i] = k + 1 < s.kv_hi ? 0xffffffffu : k < s.kv_hi ? 0x0000ffffu : 0u;
+        }
+        const int vrow = k16 + (lane & 15);
+#pragma unroll
+        for (int n = 0; n < NF / 2; ++n) {  // 16 dims a load
+          const int unit = (n & 3) * 2 + (lane >> 4);
+          uint32_t vf[4];
+          ldmatrix4t(vf, vbase + (n >> 2) * kChunk + vrow * 128 + ((unit ^ (vrow & 7)) << 4));
+          vf[0] &= mask[0];
+          vf[1] &= mask[1];
+          vf[2] &= mask[0];
+          vf[3] &= mask[1];
+          mma16816<DT>(o[2 * n], ph, vf[0], vf[1]);
+          mma16816<DT>(o[2 * n + 1], ph, vf[2], vf[3]);
+          mma16816<DT>(o[2 * n], pl, vf[0], vf[1]);
+          mma16816<DT>(o[2 * n + 1], pl, vf[2], vf[3]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+      }
+      // join the eight warps
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        const int row = r0 + 8 * i;
+        if (row < nr) {
+          if ((lane & 3) == 0) {
+            s_m[cw][row] = m[i];
+            s_l[cw][row] = l[i];
+          }
+#pragma unroll
+          for (int n = 0; n < NF; ++n)
+            *reinterpret_cast<float2*>(s_o + (cw * kRows + row) * D + ((n * 8 + cq) ^ ((row & 7) * 8))) =
+                make_float2(o[n][2 * i], o[n][2 * i + 1]);
+        }
+      }
+      if (lane == 0) s_badw[cw] = bad;
+      // a warp that gave up still meets the others here; the results no longer count then
+      group_sync();
+      int first_bad = cap;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) first_bad = min(first_bad, s_badw[w]);
+      const bool again = a.causal && s.t_hi - s.t_lo > 1;  // rows of the tile hide keys from one another
+      float* part = ws + ((int64_t)blockIdx.x * 2 + s.slot) * (kRows * (D + 2));
+      for (int e = threadIdx.x - 32; e < nr * D; e += 32 * kWarps) {
+        const int row = e / D, d = e % D;
+        float top = s_m[0][row];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][row]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = ex2_approx(s_m[w][row] - ref);
+          sum = fmaf(s_l[w][row], f, sum);
+          x = fmaf(s_o[(w * kRows + row) * D + (d ^ ((row & 7) * 8))], f, x);
+        }
+        const int t = (int)((row0 + row) / a.G), hg = (int)((row0 + row) % a.G);
+        const int v = visible_keys(s.r, t, a.causal);
+        if (v > first_bad) sum = __int_as_float(0x7fffffff);
+        if (s.whole) {
+          const float y = sum == 0.f ? 0.f : x / sum;
+          if (again && !(fabsf(y) <= 3.4028235e38f) && fabsf(sum) <= 3.4028235e38f && v < s.kv_hi)
+            atomicOr(&s_again, 1 << row);
+          reinterpret_cast<T*>(a.o)[(int64_t)(s.r.begin + t) * a.os[0] +
+                                    (int64_t)(s.h * a.G + hg) * a.os[1] + d] = E::from_f(y);
+        } else {
+          part[row * D + d] = x;
+          if (d == 0) {
+            part[kRows * D + row] = top;
+            part[kRows * D + kRows + row] = sum;
+          }
+        }
+      }
+      if (threadIdx.x == 32) s_stop = *abort_p;  // one reading, so that all warps leave together
+      group_sync();
+      ok = !s_stop;
+      if (s.whole && again) {
+        const int rows = s_again;
+        group_sync();
+        if (threadIdx.x == 32) s_again = 0;
+        for (int row = cw; row < nr; row += kWarps) {
+          if (!(rows >> row & 1)) continue;
+          const int t = (int)((row0 + row) / a.G), h = s.h * a.G + (int)((row0 + row) % a.G);
+          if (hidden_not_finite<DT>(a, s.b, s.h, visible_keys(s.r, t, a.causal), s.kv_hi))
+            row_by_key<DT>(a, s.b, s.r, t, h);
+        }
+        group_sync();
+      }
+    }
+  }
+}
+
+// Joins the parts of the tile that boundary blockIdx.x + 1 cuts first.
+template <int DT, int D>
+__global__ void __launch_bounds__(128)
+    decode_join_kernel(const __grid_constant__ AttnArgs a, const TileRule rule, int pieces,
+                       const float* ws) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  const int c = blockIdx.x + 1;
+  const Line line = find_piece(a, rule, pieces, c);
+  if (line.x < 0) return;
+  Segment s;
+  s.b = line.b;
+  s.r = seq_range(a.l, s.b);
+  const SeqCost sc = seq_cost(a, rule, s.r);
+  const int64_t head = sc.total();
+  int64_t y = line.x - line.b_at;
+  s.h = (int)(y / head);
+  y -= s.h * head;
+  s.tile = sc.find(y);
+  const int64_t at = line.x - (y - sc.prefix(s.tile)), cost = sc.cost(s.tile);
+  if (at == line.x || at < (int64_t)(c - 1) * line.q) return;  // not the tile's first boundary
+  const int last = (int)((at + cost - 1) / line.q);
+  const int64_t row0 = (int64_t)s.tile * kRows;
+  const int nr = (int)min((int64_t)kRows, (int64_t)s.r.n * a.G - row0);
+  __shared__ int s_again;
+  if (threadIdx.x == 0) s_again = 0;
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  bool final = false;
+  for (int e = threadIdx.x; e < nr * D; e += blockDim.x) {
+    const int row = e / D, d = e % D;
+    float top = -INFINITY, sum = 0.f, x = 0.f;
+    for (int p = c - 1; p <= last; ++p) {
+      const int64_t from = (int64_t)p * line.q;
+      set_blocks(a, rule, cost, max(from - at, (int64_t)0), min(cost, from + line.q - at), s);
+      if (s.whole || s.nb == 0) final = true;
+      if (final) break;
+      if (s.blk0 >= s.blk1) continue;
+      const float* part = ws + ((int64_t)p * 2 + (from >= at ? 0 : 1)) * (kRows * (D + 2));
+      const float m = __ldcg(part + kRows * D + row), l = __ldcg(part + kRows * D + kRows + row);
+      const float mn = fmaxf(top, m);
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float f0 = ex2_approx(top - ref), f1 = ex2_approx(m - ref);
+      top = mn;
+      sum = sum * f0 + l * f1;
+      x = x * f0 + __ldcg(part + row * D + d) * f1;
+    }
+    if (final) break;
+    const float out = sum == 0.f ? 0.f : x / sum;
+    const int t = (int)((row0 + row) / a.G), hg = (int)((row0 + row) % a.G);
+    if (!(fabsf(out) <= 3.4028235e38f) && fabsf(sum) <= 3.4028235e38f &&
+        visible_keys(s.r, t, a.causal) < s.kv_hi)
+      atomicOr(&s_again, 1 << row);
+    reinterpret_cast<T*>(a.o)[(int64_t)(s.r.begin + t) * a.os[0] +
+                              (int64_t)(s.h * a.G + hg) * a.os[1] + d] = E::from_f(out);
+  }
+  __syncthreads();
+  const int rows = s_again;
+  for (int row = threadIdx.x >> 5; row < nr && rows; row += 4) {
+    if (!(rows >> row & 1)) continue;
+    const int t = (int)((row0 + row) / a.G), h = s.h * a.G + (int)((row0 + row) % a.G);
+    if (hidden_not_finite<DT>(a, s.b, s.h, visible_keys(s.r, t, a.causal), s.kv_hi))
+      row_by_key<DT>(a, s.b, s.r, t, h);
+  }
+}
+
+template <int DT, int D>
+static int launch_decode(const AttnArgs& a, float* ws, cudaStream_t st) {
+  const int box = gcd_int(a.l.page_size, kBlk);
+  CUtensorMap tk, tv;
+  if (!cache_tmap(&tk, a, a.k, a.kcs, box) || !cache_tmap(&tv, a, a.v, a.vcs, box))
+    return AK_ERR_LAUNCH;
+  const cudaError_t attr = smem_optin<decode_kernel<DT, D>>(DecodeCfg<D>::SMEM);
+  AK_REQUIRE(attr == cudaSuccess, AK_ERR_LAUNCH, "paged_attention smem attribute: %s",
+             cudaGetErrorString(attr));
+  const int pieces = device_info().sm_count;
+  const TileRule rule = decode_rule();
+  decode_kernel<DT, D><<<pieces, kThreads, DecodeCfg<D>::SMEM, st>>>(tk, tv, a, rule, box, ws);
+  const int rc = launch_status("paged_attention");
+  if (rc || pieces < 2) return rc;
+  return launch_after(decode_join_kernel<DT, D>, dim3(pieces - 1), 128, st, a, rule, pieces,
+                      (const float*)ws);
+}
+
+size_t decode_workspace(int D) {
+  return 2 * (size_t)device_info().sm_count * decode_part_floats(D) * sizeof(float);
+}
+
+int run_decode(const AttnArgs& a, void* ws, cudaStream_t st) {
+  float* f = reinterpret_cast<float*>(ws);
+  if (a.dtype == AK_BF16)
+    return a.D == 128 ? launch_decode<AK_BF16, 128>(a, f, st) : launch_decode<AK_BF16, 64>(a, f, st);
+  return a.D == 128 ? launch_decode<AK_F16, 128>(a, f, st) : launch_decode<AK_F16, 64>(a, f, st);
+}
+
+}  // namespace paged
+}  // namespace ak

@@ -1,0 +1,275 @@
+// How the paged attention kernels share their work out.
+//
+// A tile is a run of one sequence's query rows for one key/value head; its work is its keys.  All
+// tiles are laid end to end on one line (sequence, head, tile), each as long as its keys plus a
+// constant for its prologue and epilogue, and the line is cut into one equal piece per CTA: every
+// SM gets the same number of keys whatever the lengths are, and no host code has to know them.  A
+// piece may end inside a tile.  Such a tile's parts go to the workspace, at most two per CTA (its
+// first and its last segment), and a second kernel joins them in the line's order, so results do
+// not depend on timing.
+#pragma once
+#include "paged_attn.cuh"
+
+namespace ak {
+namespace paged {
+
+// Rule by which a kernel cuts a sequence's tokens into tiles.
+struct TileRule {
+  int rows;    // query rows (token, head of the group) per tile, when tiles are cut by rows; or 0
+  int tokens;  // tokens per tile otherwise
+  int blk;     // keys per block
+  int over;    // cost of a tile beside its keys, in keys
+  int64_t min_piece;  // shortest piece of the line that a CTA gets
+};
+
+// A sequence on the line: tile i of a head is base + slope * (i + 1) long, the last one `last`.
+struct SeqCost {
+  int tiles;
+  int64_t base, slope, last;
+  AK_D int64_t prefix(int64_t i) const { return i * base + slope * (i * (i + 1) / 2); }
+  AK_D int64_t total() const { return tiles ? prefix(tiles - 1) + last : 0; }
+  AK_D int64_t cost(int i) const { return i == tiles - 1 ? last : base + slope * (i + 1); }
+  AK_D int find(int64_t y) const {  // tile that holds point y
+    int lo = 0, hi = tiles;         // prefix(lo) <= y < prefix(hi) or the end
+    while (hi - lo > 1) {
+      const int mid = lo + (hi - lo) / 2;
+      if (prefix(mid) <= y) lo = mid; else hi = mid;
+    }
+    return lo;
+  }
+};
+
+AK_D int capacity(const PagedLists& l) {  // keys that a table row can name
+  const int64_t c = (int64_t)l.max_pages * l.page_size;
+  return c < 0x7fffffff ? (int)c : 0x7fffffff;
+}
+
+AK_D SeqCost seq_cost(const AttnArgs& a, const TileRule& t, const SeqRange& r) {
+  SeqCost c{0, 0, 0, 0};
+  if (r.n == 0) return c;
+  const int kv = min(r.kv_len, capacity(a.l));
+  if (t.rows) {
+    c.tiles = (int)(((int64_t)r.n * a.G + t.rows - 1) / t.rows);
+    c.base = c.last = (int64_t)kv + t.over;
+  } else {
+    c.tiles = (r.n + t.tokens - 1) / t.tokens;
+    if (a.causal) {
+      c.base = (int64_t)max(kv - r.n, 0) + t.over;
+      c.slope = t.tokens;
+      c.last = c.base + r.n;
+    } else {
+      c.base = c.last = (int64_t)kv + t.over;
+    }
+  }
+  return c;
+}
+
+// A CTA's part of one tile: key blocks [blk0, blk1) of the tile's nb.
+struct Segment {
+  SeqRange r;
+  int b, h, tile;
+  int t_lo, t_hi;  // the tile's tokens within the sequence
+  int kv_hi;       // keys that its last token sees (and the table can name)
+  int blk0, blk1, nb;
+  bool whole;      // the whole tile: its result is final
+  int slot;        // workspace slot of a part: 0 for the CTA's first segment, 1 for its last
+};
+
+// The tile's tokens, keys and blocks; z0, z1 on the tile's own stretch of the line.
+AK_D void set_blocks(const AttnArgs& a, const TileRule& t, int64_t cost, int64_t z0, int64_t z1,
+                     Segment& s) {
+  if (t.rows) {
+    const int64_t r0 = (int64_t)s.tile * t.rows, r1 = min(r0 + t.rows, (int64_t)s.r.n * a.G);
+    s.t_lo = (int)(r0 / a.G);
+    s.t_hi = (int)((r1 - 1) / a.G) + 1;
+  } else {
+    s.t_lo = s.tile * t.tokens;
+    s.t_hi = min(s.t_lo + t.tokens, s.r.n);
+  }
+  s.kv_hi = min(visible_keys(s.r, s.t_hi - 1, a.causal), capacity(a.l));
+  s.nb = (int)(((int64_t)s.kv_hi + t.blk - 1) / t.blk);
+  auto block = [&](int64_t z) {
+    return z >= cost ? s.nb : (int)min((int64_t)s.nb, (z + t.blk / 2) / t.blk);
+  };
+  s.blk0 = block(z0);
+  s.blk1 = block(z1);
+  s.whole = s.blk0 == 0 && s.blk1 == s.nb;
+}
+
+// The line and the piece of it that starts at `piece` (in units of q).
+struct Line {
+  int64_t q;      // length of a piece
+  int64_t x;      // the piece's start, or -1: there is no such piece
+  int b;          // sequence that holds x
+  int64_t b_at;   // where that sequence starts
+  int64_t total;
+};
+
+// Run by the whole CTA.
+AK_D Line find_piece(const AttnArgs& a, const TileRule& t, int pieces, int piece) {
+  __shared__ int64_t s_warp[32];
+  __shared__ int64_t s_at;
+  __shared__ int s_b;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = (blockDim.x + 31) >> 5;
+  auto cost_of = [&](int b) {
+    return b < a.l.B ? a.Hkv * seq_cost(a, t, seq_range(a.l, b)).total() : (int64_t)0;
+  };
+  Line line;
+  int64_t mine = 0;
+  const int64_t first = cost_of(threadIdx.x);
+  mine = first;
+  for (int64_t b = (int64_t)threadIdx.x + blockDim.x; b < a.l.B; b += blockDim.x) mine += cost_of((int)b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) s_warp[warp] = mine;
+  if (threadIdx.x == 0) s_b = -1;
+  __syncthreads();
+  line.total = 0;
+  for (int i = 0; i < nw; ++i) line.total += s_warp[i];
+  line.q = max((line.total + pieces - 1) / pieces, t.min_piece);
+  line.x = (int64_t)piece * line.q;
+  if (line.x >= line.total) {
+    line.x = -1;
+    return line;
+  }
+  int64_t run = 0;
+  for (int64_t base = 0; base < a.l.B; base += blockDim.x) {
+    const int64_t v = base == 0 ? first : cost_of((int)min(base + threadIdx.x, (int64_t)a.l.B));
+    int64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    __syncthreads();
+    if (lane == 31) s_warp[warp] = inc;
+    __syncthreads();
+    int64_t at = run + inc - v;
+    for (int i = 0; i < nw; ++i) {
+      if (i < warp) at += s_warp[i];
+      run += s_warp[i];
+    }
+    if (line.x >= at && line.x < at + v) {
+      s_b = (int)(base + threadIdx.x);
+      s_at = at;
+    }
+    __syncthreads();
+    if (s_b >= 0) break;
+  }
+  line.b = s_b;
+  line.b_at = s_at;
+  return line;
+}
+
+// Walks the segments of one piece, in order; every role of a CTA walks for itself.
+struct Walker {
+  const AttnArgs& a;
+  const TileRule& t;
+  int64_t x, start, end, b_at;
+  int b, loaded;
+  SeqRange r;
+  SeqCost c;
+  int64_t head;  // length of one head of sequence b
+
+  AK_D Walker(const AttnArgs& a_, const TileRule& t_, const Line& line)
+      : a(a_), t(t_), x(line.x), start(line.x), end(min(line.x + line.q, line.total)),
+        b_at(line.b_at), b(line.b), loaded(-1), head(0) {
+    if (line.x < 0) end = x;
+  }
+  AK_D bool next(Segment& s) {
+    while (x < end) {
+      if (loaded != b) {
+        r = seq_range(a.l, b);
+        c = seq_cost(a, t, r);
+        head = c.total();
+        loaded = b;
+      }
+      if (x >= b_at + head * a.Hkv) {
+        b_at += head * a.Hkv;
+        if (++b >= a.l.B) return false;
+        continue;
+      }
+      int64_t y = x - b_at;
+      s.h = (int)(y / head);
+      y -= s.h * head;
+      s.r = r;
+      s.b = b;
+      s.tile = c.find(y);
+      const int64_t cost = c.cost(s.tile), z0 = y - c.prefix(s.tile);
+      const int64_t z1 = min(cost, z0 + (end - x));
+      s.slot = x == start ? 0 : 1;
+      x += z1 - z0;
+      set_blocks(a, t, cost, z0, z1, s);
+      if (s.nb == 0) {
+        if (z0 == 0) return true;  // no keys at all: its first part writes the zeros
+      } else if (s.blk0 < s.blk1) {
+        return true;
+      }
+    }
+    return false;
+  }
+};
+
+// ------------------------------------------------------------------ rows read key by key
+// The matrix instructions multiply a hidden key's value by a weight of 0, which is NaN when the
+// value is not finite.  A row whose result is not finite although its sum of weights is, and
+// that shares its tile with keys hidden from it, is looked at again: if a hidden value is the
+// cause, the row is computed from its visible keys alone.  One warp does a row.
+
+// Whether V holds a value that is not finite at keys [lo, hi).
+template <int DT>
+AK_D bool hidden_not_finite(const AttnArgs& a, int b, int hk, int lo, int hi) {
+  using E = Elem<DT>;
+  const int lane = threadIdx.x & 31;
+  bool found = false;
+  for (int j = lo; j < hi; ++j) {
+    const int page = page_of(a.l, b, j / a.l.page_size);
+    if (page < 0) continue;
+    const typename E::T* v = reinterpret_cast<const typename E::T*>(a.v) + page * a.vcs[0] +
+                             hk * a.vcs[1] + (j % a.l.page_size) * a.vcs[2];
+    for (int d = lane; d < a.D; d += 32) found |= !(fabsf(E::to_f(v[d])) <= 3.4028235e38f);
+  }
+  return __any_sync(0xffffffffu, found);
+}
+
+// Row (token t of the sequence, query head h) from its visible keys; D <= 128.
+template <int DT>
+__device__ __noinline__ void row_by_key(const AttnArgs& a, int b, const SeqRange& r, int t, int h) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  const int lane = threadIdx.x & 31, hk = h / a.G;
+  const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(r.begin + t) * a.qs[0] + h * a.qs[1];
+  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = lane + 32 * i < a.D ? E::to_f(qp[lane + 32 * i]) : 0.f;
+  float m = -INFINITY, sum = 0.f;
+  const int vis = visible_keys(r, t, a.causal);
+  for (int j = 0; j < vis; ++j) {
+    const int slot = j % a.l.page_size, page = page_of(a.l, b, j / a.l.page_size);
+    if (page < 0) {
+      sum = __int_as_float(0x7fffffff);
+      break;
+    }
+    const T* kp = reinterpret_cast<const T*>(a.k) + page * a.kcs[0] + hk * a.kcs[1] + slot * a.kcs[2];
+    const T* vp = reinterpret_cast<const T*>(a.v) + page * a.vcs[0] + hk * a.vcs[1] + slot * a.vcs[2];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < a.D) s = fmaf(q[i], E::to_f(kp[lane + 32 * i]), s);
+    s = warp_sum(s);
+    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
+    const float alpha = exp2f((m - ref) * a.scale_log2), p = exp2f((s - ref) * a.scale_log2);
+    m = mn;
+    sum = sum * alpha + p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < a.D) o[i] = fmaf(p, E::to_f(vp[lane + 32 * i]), o[i] * alpha);
+  }
+  T* op = reinterpret_cast<T*>(a.o) + (int64_t)(r.begin + t) * a.os[0] + h * a.os[1];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 32 * i < a.D) op[lane + 32 * i] = E::from_f(sum == 0.f ? 0.f : o[i] / sum);
+}
+
+}  // namespace paged
+}  // namespace ak

@@ -72,6 +72,16 @@ AK_D bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   }
 }
 
+// For a producer that gives up: wait (half a second at most) until its copies into a ring of
+// full-barriers have landed.  `used` ring slots were filled, one phase each, the last one possibly
+// not issued.
+AK_D void drain_ring(uint64_t* full, int stages, int used) {
+  const unsigned long long t0 = globaltimer();
+  for (int g = used > stages ? used - stages : 0; g < used; ++g)
+    while (!mbar_try_wait(&full[g % stages], (g / stages) & 1))
+      if (globaltimer() - t0 > kWaitTimeoutNs / 4) return;
+}
+
 // ------------------------------------------------------------------ TMA
 AK_D void tma_prefetch_desc(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");

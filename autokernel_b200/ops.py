@@ -728,7 +728,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     code = dtype_code(k_cache.dtype)
     require_cuda(q, k_cache, v_cache, page_table, cu_q, kv_lens, *([out] if out is not None else []))
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    ws = torch.empty(_lib.load().ak_paged_attention_workspace_size(H, Hkv, D, code),
+    ws = torch.empty(_lib.load().ak_paged_attention_workspace_size(N, B, H, Hkv, D, code),
                      dtype=torch.uint8, device=q.device)
     st = [_i64s(*t.stride()[:2]) for t in (q, o)] + [_i64s(*t.stride()[:3]) for t in (k_cache, v_cache)]
     call("ak_paged_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),

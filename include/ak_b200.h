@@ -293,7 +293,8 @@ AK_API int ak_paged_append(const void* k, const void* v, const void* q, void* q_
  * that sees no key (or only scores of -inf) is 0; a row that sees a key without a page is NaN.
  * What the cache holds behind a sequence's last key never matters.  D <= 256, sm_scale > 0.
  * workspace: ak_paged_attention_workspace_size bytes, used by this call alone until it is done. */
-AK_API size_t ak_paged_attention_workspace_size(int64_t H, int64_t Hkv, int64_t D, int dtype);
+AK_API size_t ak_paged_attention_workspace_size(int64_t N, int64_t B, int64_t H, int64_t Hkv,
+                                         int64_t D, int dtype);
 AK_API int ak_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* out,
                        const int32_t* page_table, const int32_t* cu_q, const int32_t* kv_lens,
                        int64_t N, int64_t B, int64_t H, int64_t Hkv, int64_t D,
