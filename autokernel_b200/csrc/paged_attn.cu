@@ -143,7 +143,7 @@ using namespace ak;
 extern "C" size_t ak_paged_attention_workspace_size(int64_t N, int64_t B, int64_t H, int64_t Hkv,
                                                     int64_t D, int dtype) {
   if (dtype == AK_F32 || (D != 64 && D != 128)) return 0;
-  return paged::decode_workspace((int)D);
+  return N <= B ? paged::decode_workspace((int)D) : paged::chunk_workspace((int)D);
 }
 
 extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void* v_cache,
@@ -190,7 +190,9 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
     a.vcs[i] = v_cache_strides[i];
   }
   cudaStream_t st = (cudaStream_t)stream;
-  if (paged::tc_ok(a)) return paged::run_decode(a, workspace, st);
+  // No more tokens than sequences is a decoding step (any sequence may still hold several).
+  if (paged::tc_ok(a))
+    return N <= B ? paged::run_decode(a, workspace, st) : paged::run_chunk(a, workspace, st);
   switch (dtype) {
     case AK_F32: return paged::run_simt<AK_F32>(a, st);
     case AK_F16: return paged::run_simt<AK_F16>(a, st);

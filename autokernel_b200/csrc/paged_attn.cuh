@@ -25,6 +25,8 @@ AK_D int visible_keys(const SeqRange& r, int i, int causal) {
 // paged_decode.cu: 16 query rows per tile, all keys read once; paged_chunk.cu: 128-row tensor-core tiles.
 int run_decode(const AttnArgs& a, void* ws, cudaStream_t st);
 size_t decode_workspace(int D);
+int run_chunk(const AttnArgs& a, void* ws, cudaStream_t st);
+size_t chunk_workspace(int D);
 
 inline int gcd_int(int x, int y) {
   while (y) {

@@ -372,6 +372,7 @@ __global__ void __launch_bounds__(128)
   using T = typename E::T;
   const int c = blockIdx.x + 1;
   const Line line = find_piece(a, rule, pieces, c);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // in every block, also one without a part
   if (line.x < 0) return;
   Segment s;
   s.b = line.b;
@@ -390,7 +391,6 @@ __global__ void __launch_bounds__(128)
   __shared__ int s_again;
   if (threadIdx.x == 0) s_again = 0;
   __syncthreads();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   bool final = false;
   for (int e = threadIdx.x; e < nr * D; e += blockDim.x) {
     const int row = e / D, d = e % D;
