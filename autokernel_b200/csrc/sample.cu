@@ -4,11 +4,11 @@
 //   kept = the first min(k, n_p, n_m) of that order, where n_p counts the entries whose
 //   predecessors' weights sum to less than p * (the weight of the first k), and n_m the w_i >= min_p;
 //   token = the lowest index whose kept weights up to it sum to more than u * (the kept weight).
-// T <= 0: the largest logit, lowest index.  No alive entry: -1.
+// T <= 0: the largest logit, lowest index.  No alive entry: -1.  With a largest logit of +inf only
+// the entries equal to it are alive.
 //
-// The kept set is always the front of the order, so it is given by a key tau and the number of
-// entries equal to tau that belong to it (those of lowest index): keys are the logits' bits made
-// monotone, and tau is found by bisection over counts (top-k) and weights (top-p).
+// The kept set is the front of the order, so it is given by the rank of its last entry: a 64-bit
+// number, the logit's bits made monotone above the inverted index.
 #include "ak_common.cuh"
 
 #include <cooperative_groups.h>
@@ -17,6 +17,8 @@ namespace cg = cooperative_groups;
 
 namespace ak {
 namespace {
+
+using u64 = unsigned long long;
 
 struct SampleArgs {
   const void* x;
@@ -30,163 +32,113 @@ struct SampleArgs {
   int vocab;
 };
 
-// Monotone key of a logit: larger logit, larger key; -0 and +0 share one; NaN and -inf are 0.
-template <int DT>
-struct Key;
-template <>
-struct Key<AK_F32> {
-  using Bits = uint32_t;
-  static constexpr uint32_t kLowest = 0x00800000u;  // of the lowest finite value
-  static AK_D uint32_t of(uint32_t u) {
-    if ((u << 1) == 0) u = 0;
-    if ((u & 0x7fffffffu) > 0x7f800000u || u == 0xff800000u) return 0;
-    return (u >> 31) ? ~u : u | 0x80000000u;
-  }
-  static AK_D float value(uint32_t k) {
-    return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
-  }
+struct Settings {
+  float t, p;
+  double m;  // smallest weight that is kept
+  int k;
+  double u;
+  bool first_only;
 };
-template <int DT>
-struct Key16 {
-  using Bits = uint16_t;
-  static constexpr uint32_t kInf = DT == AK_F16 ? 0x7c00u : 0x7f80u;
-  static constexpr uint32_t kLowest = DT == AK_F16 ? 0x0400u : 0x0080u;
-  static AK_D uint32_t of(uint32_t u) {
-    if ((u & 0x7fffu) == 0) u = 0;
-    if ((u & 0x7fffu) > kInf || u == (kInf | 0x8000u)) return 0;
-    return (u & 0x8000u) ? ~u & 0xffffu : u | 0x8000u;
-  }
-  static AK_D float value(uint32_t k) {
-    const uint16_t b = (uint16_t)((k & 0x8000u) ? k & 0x7fffu : ~k);
-    return Elem<DT>::to_f(*reinterpret_cast<const typename Elem<DT>::T*>(&b));
-  }
-};
-template <>
-struct Key<AK_F16> : Key16<AK_F16> {};
-template <>
-struct Key<AK_BF16> : Key16<AK_BF16> {};
-
-template <int DT>
-struct Weight {
-  uint32_t top;
-  double max, t;
-  AK_D double operator()(uint32_t key) const {
-    if (key == 0) return 0.0;
-    if (key == top) return 1.0;
-    const double d = ((double)Key<DT>::value(key) - max) / t;
-    return d == d ? exp(d) : 0.0;  // (largest logit and temperature both infinite)
-  }
-};
-
-// Cuts by bisection over keys: `count(key)` entries and `mass(key)` weight lie above a key.
-// top-k: the key of the k-th entry; `ties` of its entries belong to the first k.
-template <int DT, class Count>
-AK_D uint32_t cut_by_count(Count count, uint32_t top, int64_t k, int64_t& ties) {
-  uint32_t lo = Key<DT>::kLowest - 1, hi = top;  // count(lo) >= k > count(hi)
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (count(mid) >= k) lo = mid; else hi = mid;
-  }
-  ties = k - count(hi);
-  return hi;
-}
-// top-p of the entries above tau and the first `ties` equal to it.
-template <int DT, class Count, class Mass>
-AK_D uint32_t cut_by_weight(Count count, Mass mass, const Weight<DT>& w, uint32_t top, uint32_t tau,
-                            double p, int64_t n, int64_t& ties) {
-  const double wt = w(tau);
-  const double at = (double)(count(tau - 1) - count(tau));
-  const double target = p * (mass(tau) + wt * fmin((double)ties, at));
-  uint32_t lo = tau - 1, hi = top;  // mass(hi) < target <= mass(lo), or lo below tau
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (mass(mid) >= target) lo = mid; else hi = mid;
-  }
-  // the entries equal to hi whose predecessors weigh less than the target
-  const double above = mass(hi), wh = w(hi);
-  const int64_t limit = hi == tau ? ties : n;
-  int64_t c = wh > 0.0 ? (int64_t)fmin(ceil((target - above) / wh), (double)n) : n;
-  while (c > 1 && !(above + (double)(c - 1) * wh < target)) --c;
-  while (c < n && above + (double)c * wh < target) ++c;
-  ties = c < 1 ? 1 : (c < limit ? c : limit);
-  return hi;
+AK_D Settings settings_of(const SampleArgs& a, int64_t row) {
+  Settings s;
+  s.t = a.t_row ? a.t_row[row] : a.t;
+  s.p = a.p_row ? a.p_row[row] : a.p;
+  s.k = a.k_row ? a.k_row[row] : a.k;
+  const float m = a.m_row ? a.m_row[row] : a.m, u = a.u[row];
+  s.m = m > 0.f ? fmin((double)m, 1.0) : 0.0;
+  s.u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
+  s.first_only = !(s.t > 0.f) || !(s.p > 0.f) || s.k == 1;
+  if (s.k <= 0 || s.k >= a.vocab) s.k = 0;
+  return s;
 }
 
-// A row of any length, read again in every pass; for rows that a cluster cannot hold.
+// Alive entries are floats above -inf; a dead one is NaN or -inf.
+AK_D bool alive(float x) { return x > -INFINITY; }
+// Monotone bits of an alive logit, never 0; -0 and +0 are one.
+AK_D uint32_t key_of(float x) {
+  const uint32_t u = x == 0.f ? 0u : __float_as_uint(x);
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+AK_D float value_of(uint32_t k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
+AK_D u64 rank_of(float x, int i) { return (u64)key_of(x) << 32 | (uint32_t)~i; }
+constexpr u64 kAll = 1ull << 32;  // below the rank of every alive entry
+
+// Sums over a row of any length, one CTA, the row read again in every pass: for rows that a cluster
+// cannot hold.  The cuts are found by bisection over ranks.
 template <int DT>
 __global__ void __launch_bounds__(512) sample_kernel(const SampleArgs a) {
-  using K = Key<DT>;
+  using E = Elem<DT>;
   const int64_t row = blockIdx.x;
-  const typename K::Bits* x = reinterpret_cast<const typename K::Bits*>(a.x) + row * a.ld;
+  const typename E::T* x = reinterpret_cast<const typename E::T*>(a.x) + row * a.ld;
   const int n = a.vocab, tid = threadIdx.x, nt = blockDim.x;
-  __shared__ double s_red[32];
-  __shared__ double s_scan[512];
-  __shared__ int s_ties[512];
-
-  auto count = [&](uint32_t above) {  // entries with key > above
-    int c = 0;
-    for (int i = tid; i < n; i += nt) c += K::of(x[i]) > above;
-    return (int64_t)block_sum_d((double)c, s_red);
-  };
-
-  uint32_t top = 0;
-  for (int i = tid; i < n; i += nt) top = max(top, K::of(x[i]));
-  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  __shared__ double s_red[32], s_scan[512];
+  __shared__ u64 s_top;
+  const Settings set = settings_of(a, row);
+  if (tid == 0) s_top = 0;
   __syncthreads();
-  if ((tid & 31) == 0) s_ties[tid >> 5] = (int)top;
+  u64 top = 0;  // the first entry's rank
+  for (int i = tid; i < n; i += nt) {
+    const float f = E::to_f(x[i]);
+    if (alive(f)) top = max(top, rank_of(f, i));
+  }
+  atomicMax(&s_top, top);
   __syncthreads();
-  for (int i = 0; i < nt / 32; ++i) top = max(top, (uint32_t)s_ties[i]);
-  __syncthreads();
-  if (top == 0) {
-    if (tid == 0) a.out[row] = -1;
+  top = s_top;
+  if (top == 0 || set.first_only) {
+    if (tid == 0) a.out[row] = top ? (int64_t)(uint32_t)~(uint32_t)top : -1;
     return;
   }
-
-  const float tf = a.t_row ? a.t_row[row] : a.t, pf = a.p_row ? a.p_row[row] : a.p;
-  const float mf = a.m_row ? a.m_row[row] : a.m;
-  const int kf = a.k_row ? a.k_row[row] : a.k;
-  const bool greedy = !(tf > 0.f);
-  const Weight<DT> w{top, (double)K::value(top), greedy ? 1.0 : (double)tf};
-  const double p = pf, m = mf > 0.f ? fmin((double)mf, 1.0) : 0.0;
-  const int64_t alive = count(0);
-
-  uint32_t tau = K::kLowest;
-  int64_t ties = n;
-  if (greedy || !(pf > 0.f)) {
-    tau = top;
-    ties = 1;
-  } else {
-    if (kf > 0 && kf < alive) tau = cut_by_count<DT>(count, top, kf, ties);
-    if (pf < 1.f) {
-      auto mass = [&](uint32_t above) {  // weight of the entries with key > above
-        double c = 0.0;
-        for (int i = tid; i < n; i += nt) {
-          const uint32_t key = K::of(x[i]);
-          if (key > above) c += w(key);
-        }
-        return block_sum_d(c, s_red);
-      };
-      tau = cut_by_weight<DT>(count, mass, w, top, tau, p, n, ties);
+  const float max_ = value_of((uint32_t)(top >> 32));
+  const double rate = 1.4426950408889634 / (double)set.t;
+  auto w = [&](float f) {
+    return f == max_ ? 1.0 : max_ == INFINITY ? 0.0 : exp2(((double)f - (double)max_) * rate);
+  };
+  auto count = [&](u64 from) {  // entries of rank `from` and above
+    int c = 0;
+    for (int i = tid; i < n; i += nt) {
+      const float f = E::to_f(x[i]);
+      c += alive(f) && rank_of(f, i) >= from;
     }
+    return block_sum_d((double)c, s_red);
+  };
+  auto mass = [&](u64 from) {
+    double c = 0.0;
+    for (int i = tid; i < n; i += nt) {
+      const float f = E::to_f(x[i]);
+      if (alive(f) && rank_of(f, i) >= from) c += w(f);
+    }
+    return block_sum_d(c, s_red);
+  };
+  u64 least = kAll;  // the smallest rank that is kept
+  if (set.k && count(least) > (double)set.k) {
+    u64 lo = kAll, hi = top;  // count(lo) > k >= count(hi)
+    while (hi - lo > 1) {
+      const u64 mid = lo + (hi - lo) / 2;
+      if (count(mid) > (double)set.k) lo = mid; else hi = mid;
+    }
+    least = hi;
   }
-
-  // token: prefix sums over runs of consecutive entries, one run per thread
+  if (set.p < 1.f) {
+    // the smallest rank above which less than the target lies
+    const double target = (double)set.p * mass(least);
+    u64 lo = least - 1, hi = top;  // mass above lo >= target (or nothing is left), above hi less
+    while (hi - lo > 1) {
+      const u64 mid = lo + (hi - lo) / 2;
+      if (mass(mid + 1) >= target) lo = mid; else hi = mid;
+    }
+    least = max(least, hi);
+  }
+  // token: sums over runs of consecutive entries, one run per thread
   const int run = (n + nt - 1) / nt;
   const int i0 = min(tid * run, n), i1 = min(i0 + run, n);
-  int eq = 0;
-  for (int i = i0; i < i1; ++i) eq += K::of(x[i]) == tau;
-  s_ties[tid] = eq;
-  __syncthreads();
-  int before = 0;
-  for (int i = 0; i < tid; ++i) before += s_ties[i];
+  auto kept = [&](int i) {
+    const float f = E::to_f(x[i]);
+    if (!alive(f) || rank_of(f, i) < least) return 0.0;
+    const double v = w(f);
+    return v >= set.m ? v : 0.0;
+  };
   double sum = 0.0;
-  int seen = before;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t key = K::of(x[i]);
-    if (key < tau || (key == tau && seen++ >= ties)) continue;
-    const double v = w(key);
-    if (v >= m) sum += v;
-  }
+  for (int i = i0; i < i1; ++i) sum += kept(i);
   s_scan[tid] = sum;
   __syncthreads();
   double start = 0.0, total = 0.0;
@@ -194,17 +146,11 @@ __global__ void __launch_bounds__(512) sample_kernel(const SampleArgs a) {
     if (i == tid) start = total;
     total += s_scan[i];
   }
-  float uf = a.u[row];
-  uf = uf > 0.f ? fminf(uf, 0.99999994f) : 0.f;
-  const double goal = (double)uf * total;
+  const double goal = set.u * total;
   if (start <= goal && goal < start + sum) {
     double c = 0.0;
-    seen = before;
     for (int i = i0; i < i1; ++i) {
-      const uint32_t key = K::of(x[i]);
-      if (key < tau || (key == tau && seen++ >= ties)) continue;
-      const double v = w(key);
-      if (v >= m) c += v;
+      c += kept(i);
       if (start + c > goal) {
         a.out[row] = i;
         break;
@@ -216,66 +162,74 @@ __global__ void __launch_bounds__(512) sample_kernel(const SampleArgs a) {
 // ------------------------------------------------------------------ the row in a cluster
 // One cluster of C CTAs per row (C up to 8), which keep it in shared memory, each thread reading only
 // the 16-byte vectors it fetched, so logits come from memory once:
-//   1  the largest key
-//   2  (top-k or top-p) a histogram over max - x, 1536 bins of T / 48: counts, and weights as 64-bit
-//      fixed point (2^-45, so sums do not depend on their order); the bin where the cut falls is
-//      found by a scan, its few entries are gathered, sorted and cut exactly
-//   3  kept weights per run of 32 vectors, then the run, the lane and the entry that u falls in
-// Rows whose cut lies outside the bins or in a crowded bin (equal logits) are cut by bisection
-// over keys instead.
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1536, kList = 1024;
-constexpr int kMaxSlice = 160 * 1024;                  // bytes of a row per CTA
+//   1  the largest logit
+//   2  top-k: a histogram of counts over max - x (1535 bins of T / 48 and one for what lies beyond)
+//      gives the bin that holds the k-th entry; its entries, when they are few, are gathered,
+//      sorted and cut, and what is not kept dies.  A crowded bin is divided again by the bits of the
+//      rank.
+//   3  top-p: what top-k left, when it is few, is gathered and sorted at once.  Otherwise
+//      the histogram of counts times a weight per bin tells a small stretch of logits that holds the
+//      cut; one pass sums every weight exactly (64-bit floating point above and below the stretch,
+//      fixed point, 2^-45, in 1536 bins of the stretch, where no order of additions matters), and
+//      the stretch is cut like top-k's bin.
+//   4  kept weights per run of 32 vectors, then the run, the lane and the entry that u falls in
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1536, kList = 128, kNear = 2048;
+constexpr int kMaxSlice = 160 * 1024;                   // bytes of a row per CTA
 constexpr int kMaxRuns = kMaxSlice / 16 / 32 + kWarps;  // runs of 32 vectors
-constexpr double kFixed = 35184372088832.0;            // 2^45: 2^18 weights of 1 fit 64 bits
+constexpr double kFixed = 35184372088832.0;             // 2^45: 2^18 weights of 1 fit 64 bits
 constexpr int kMaxVocab = 1 << 18;
 
-struct Hist {
-  unsigned long long mass[kBins];
-  uint32_t count[kBins];
-};
-struct List {
-  uint32_t key[kList], idx[kList], key_sorted[kList], idx_sorted[kList];
-  double weight[kList];
+// A 64-bit atomic addition in shared memory takes about 70 cycles a warp (measured, without
+// conflicts), a 32-bit one 0.75: fixed-point weights (up to 2^45) are added in three digits of 15
+// bits, whose sums over a slice (at most 2^17 entries) fit 32 bits.
+struct Bins {
+  uint32_t digit[3][kBins], count[kBins];
 };
 struct Shared {
-  union {
-    Hist h;   // this CTA's
-    List list;  // the leader's, once the histograms are added up
-  };
-  Hist all;   // the leader's: of all CTAs
-  unsigned long long rest, rest_all;  // weight outside the bins
+  Bins h;  // this CTA's; then, in the leader's, of all CTAs with the weight in digits 0 and 1
+  u64 list[kList], sorted[kList];
+  double weight[kList];
+  uint32_t near[kNear];  // this CTA's entries (numbers within the slice) in top-p's stretch
+  int n_near;
   double run[kMaxRuns];
-  double red[kWarps], total, above, target;
-  unsigned long long scan[kWarps];
-  uint32_t top, found, need;
-  int n_list, bin, regather, bisect_k, bisect_p;
-  uint32_t tau, last;  // cut: keys above tau, and those equal to it up to index `last`
+  double red[kWarps], total, above_w, below_w;
+  u64 scan[kWarps], scan2[kWarps];
+  u64 hi, lo;  // largest and smallest rank of this CTA's entries in the bin
+  uint32_t found;
+  float top[kWarps], max_;
+  // the leader's decisions
+  u64 above, goal, cut;  // what lies above the bin; where the place is; its rank
+  double real_goal;      // top-p's, before it is rounded up
+  uint32_t in_bin;
+  int bin, n_list, next;
+  float f_hi, f_lo;  // the stretch that holds top-p's cut
 };
+enum Step { kCount, kWeigh, kSums, kDivide, kGather };
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const SampleArgs a) {
-  using K = Key<DT>;
-  using Bits = typename K::Bits;
-  constexpr int VEC = Elem<DT>::kVec;
+__global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __grid_constant__ SampleArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int VEC = E::kVec;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
+  uint4* const slice = reinterpret_cast<uint4*>(smem_raw + (sizeof(Shared) + 15) / 16 * 16);
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
   const int64_t row = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Shared& lead = *cluster.map_shared_rank(&s, 0);
-
-  const float tf = a.t_row ? a.t_row[row] : a.t, pf = a.p_row ? a.p_row[row] : a.p;
-  const float mf = a.m_row ? a.m_row[row] : a.m;
-  const int kf = a.k_row ? a.k_row[row] : a.k;
+  auto peer = [&](int c) -> Shared& { return *cluster.map_shared_rank(&s, c); };
+  auto sync = [&] {
+    if (C > 1) cluster.sync(); else __syncthreads();
+  };
 
   // load: vectors start on 16-byte boundaries, so the first and the last may hold entries that are
-  // not the row's; those become NaN, which no pass counts
-  uint4* const slice = reinterpret_cast<uint4*>(smem_raw + (sizeof(Shared) + 15) / 16 * 16);
-  int nv = 0, first, per;  // vectors of this thread; index of entry 0 of its first one; vectors of the CTA
+  // not the row's; those become NaN, which is dead
+  int nv = 0, first, per;  // this thread's vectors; index of its first entry; the CTA's vectors
   {
-    const Bits* x = reinterpret_cast<const Bits*>(a.x) + row * a.ld;
-    const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(Bits));
+    const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld;
+    const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
     per = ((a.vocab + mis + VEC - 1) / VEC + C - 1) / C;
     first = (rank * per + tid) * VEC - mis;
     for (int j = tid; j < per; j += kThreads, ++nv) {
@@ -289,422 +243,549 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
         uint4 raw = make_uint4(~0u, ~0u, ~0u, ~0u);  // NaN
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
-          if (i + e >= 0 && i + e < a.vocab) reinterpret_cast<Bits*>(&raw)[e] = x[i + e];
+          if (i + e >= 0 && i + e < a.vocab) reinterpret_cast<T*>(&raw)[e] = x[i + e];
         slice[j] = raw;
       }
     }
+    if (tid == 0) s.found = 0xffffffffu;
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
+  const Settings set = settings_of(a, row);
   const int rounds = (per + kThreads - 1) / kThreads;
-  auto index = [&](int v, int e) { return first + v * kThreads * VEC + e; };
-  auto keys_of = [&](int v, uint32_t* key) {
-    const uint4 raw = slice[v * kThreads + tid];
-    const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+  auto unpack = [](const uint4& raw, float* f) {
+    const T* t = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      key[e] = VEC == 4 ? K::of(word[e]) : K::of((e & 1) ? word[e / 2] >> 16 : word[e / 2] & 0xffffu);
-  };
-  // f(key, index) for every entry of this thread
-  auto each = [&](auto f) {
-#pragma unroll 1
-    for (int v = 0; v < nv; ++v) {
-      uint32_t key[VEC];
-      keys_of(v, key);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) f(key[e], index(v, e));
-    }
+    for (int e = 0; e < VEC; ++e) f[e] = E::to_f(t[e]);
   };
 
-  // 1: the largest key of the row
-  uint32_t top = 0;
-  each([&](uint32_t key, int) { top = max(top, key); });
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (tid == 0) {
-    s.top = 0;
-    s.found = 0xffffffffu;
-    s.rest = 0;
-    s.n_list = s.bisect_k = s.bisect_p = s.regather = 0;
+  // 1: the largest logit (a maximum skips NaN)
+  float max_ = -INFINITY;
+#pragma unroll 2
+  for (int v = 0; v < nv; ++v) {
+    const uint4 raw = slice[v * kThreads + tid];
+    float f[VEC];
+    unpack(raw, f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) max_ = fmaxf(max_, f[e]);
   }
+  max_ = warp_max(max_);
+  if (lane == 0) s.top[warp] = max_;
   __syncthreads();
-  if (lane == 0) atomicMax(&s.top, top);
-  cluster.sync();
-  for (int i = 0; i < C; ++i) top = max(top, cluster.map_shared_rank(&s, i)->top);
-  if (top == 0) {
+  max_ = warp_max(s.top[lane & (kWarps - 1)]);
+  if (C > 1) {
+    if (tid == 0) s.max_ = max_;
+    cluster.sync();
+    for (int c = 0; c < C; ++c) max_ = fmaxf(max_, peer(c).max_);
+  }
+  if (!alive(max_)) {
     if (rank == 0 && tid == 0) a.out[row] = -1;
-    cluster.sync();  // no CTA leaves while another may read its memory
+    if (C > 1) cluster.sync();  // no CTA leaves while another may read its memory
     return;
   }
 
-  const bool first_only = !(tf > 0.f) || !(pf > 0.f) || kf == 1;
-  if (first_only) {
+  // The code below is kept small (each pass exists once, and what few entries need runs in a loop of
+  // its own): a row passes through it once, and waiting for instructions cost more than the work.
+  auto index = [&](int v, int e) { return first + v * kThreads * VEC + e; };
+  auto load = [&](int v, float* f) {
+    const uint4 raw = slice[v * kThreads + tid];
+    unpack(raw, f);
+  };
+  auto entry = [&](int j, int e) {  // entry e of the CTA's vector j
+    return E::to_f(reinterpret_cast<const T*>(slice)[j * VEC + e]);
+  };
+  // every entry becomes value(entry, index): -inf to die
+  auto kill = [&](auto value) {
+#pragma unroll 1
+    for (int v = 0; v < nv; ++v) {
+      float f[VEC];
+      load(v, f);
+      uint4 raw;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) reinterpret_cast<T*>(&raw)[e] = E::from_f(value(f[e], index(v, e)));
+      slice[v * kThreads + tid] = raw;
+    }
+  };
+  if (max_ == INFINITY) {  // only the infinite entries count, all alike
+    kill([](float f, int) { return f == INFINITY ? 0.f : -INFINITY; });
+    max_ = 0.f;
+  }
+
+  if (set.first_only) {
     uint32_t at = 0xffffffffu;
-    each([&](uint32_t key, int i) {
-      if (key == top) at = min(at, (uint32_t)i);
-    });
+#pragma unroll 1
+    for (int v = 0; v < nv; ++v) {
+      float f[VEC];
+      load(v, f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (f[e] == max_) at = min(at, (uint32_t)index(v, e));
+    }
     at = __reduce_min_sync(0xffffffffu, at);
     if (lane == 0 && at != 0xffffffffu) atomicMin(&lead.found, at);
-    cluster.sync();
+    sync();
     if (rank == 0 && tid == 0) a.out[row] = s.found;
     return;
   }
 
-  const Weight<DT> w{top, (double)K::value(top), (double)tf};
-  const double p = pf, m = mf > 0.f ? fmin((double)mf, 1.0) : 0.0;
-  const bool cut_p = pf < 1.f;
-  const bool cut_k = kf > 0 && kf < a.vocab;
-
-  // bin of an entry: monotone in x, kBins when outside
-  const float maxf_ = K::value(top), inv = kBins / fminf(fmaxf(32.f * tf, 16.f), 64.f);
-  auto bin_of = [&](uint32_t key) {
-    if (key == top) return 0;
-    const float b = (maxf_ - K::value(key)) * inv;
-    return b < (float)kBins ? (int)b : kBins;
+  const double rate = 1.4426950408889634 / (double)set.t, top_d = max_;
+  auto w = [&](float f) { return exp2(((double)f - top_d) * rate); };
+  // an entry of weight w to bin b; round(w 2^45) is in the low bits of a sum with 2^52
+  auto add = [&](int b, double w) {
+    const u64 x = __double_as_longlong(fma(w, kFixed, 4503599627370496.0)) - 0x4330000000000000ll;
+    atomicAdd(&s.h.count[b], 1u);
+    atomicAdd(&s.h.digit[0][b], (uint32_t)x & 0x7fffu);
+    atomicAdd(&s.h.digit[1][b], (uint32_t)(x >> 15) & 0x7fffu);
+    atomicAdd(&s.h.digit[2][b], (uint32_t)(x >> 30));
   };
-  // sum over the cluster, the same in every thread; a fixed order
-  auto cluster_sum = [&](double v) {
-    v = warp_sum_d(v);
-    __syncthreads();
-    if (lane == 0) s.red[warp] = v;
-    __syncthreads();
-    if (tid == 0) {
-      double t = 0.0;
-      for (int i = 0; i < kWarps; ++i) t += s.red[i];
-      s.total = t;
-    }
-    cluster.sync();
-    double t = 0.0;
-    for (int i = 0; i < C; ++i) t += cluster.map_shared_rank(&s, i)->total;
-    cluster.sync();
-    return t;
-  };
+  // place of an entry in units of a bin, monotone in x; entries beyond the bins share the last one
+  const float per_bin = (kBins - 1) / fminf(fmaxf(32.f * set.t, 16.f), 64.f);
+  auto units = [&](float f) { return fminf(__fmul_rn(__fsub_rn(max_, f), per_bin), (float)(kBins - 1)); };
+  // kept: entries above `cut_f`, and those equal to it up to index `cut_i`; at first all alive ones
+  float cut_f = -INFINITY;
+  int cut_i = -1;
+  auto keep = [&](float f, int i) { return f > cut_f || (f == cut_f && i <= cut_i); };
 
-  uint32_t tau = 0, last = 0xffffffffu;
-  if (cut_k || cut_p) {
-    for (int i = tid; i < kBins; i += kThreads) {
-      s.h.mass[i] = 0;
-      s.h.count[i] = 0;
-    }
-    __syncthreads();
-    double rest = 0.0;
-    each([&](uint32_t key, int) {
-      if (key == 0) return;
-      const int b = bin_of(key);
-      if (b < kBins) {
-        if (cut_k) atomicAdd(&s.h.count[b], 1u);
-        if (cut_p) atomicAdd(&s.h.mass[b], __double2ull_rn(w(key) * kFixed));
-      } else if (cut_p) {
-        rest += w(key);
-      }
-    });
-    if (cut_p) {
-      rest = warp_sum_d(rest);
-      if (lane == 0) atomicAdd(&s.rest, __double2ull_rn(rest * kFixed));
-    }
-    cluster.sync();
-    // each CTA adds up its share of the bins and hands it to the leader
-    const int share = kBins / C;
-    for (int i = rank * share + tid; i < (rank + 1) * share; i += kThreads) {
-      unsigned long long ms = 0;
-      uint32_t cs = 0;
-      for (int c = 0; c < C; ++c) {
-        const Shared& o = *cluster.map_shared_rank(&s, c);
-        if (cut_p) ms += o.h.mass[i];
-        if (cut_k) cs += o.h.count[i];
-      }
-      lead.all.mass[i] = ms;
-      lead.all.count[i] = cs;
-    }
-    if (rank == 0 && tid == 0) {
-      unsigned long long t = 0;
-      for (int c = 0; c < C; ++c) t += cluster.map_shared_rank(&s, c)->rest;
-      s.rest_all = t;
-    }
-    cluster.sync();
-
-    // sums before this thread's bins (leader)
-    constexpr int PER = kBins / kThreads;
-    auto scan = [&](unsigned long long v) {
-      unsigned long long inc = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
-      }
-      __syncthreads();
-      if (lane == 31) s.scan[warp] = inc;
-      __syncthreads();
-      unsigned long long before = inc - v;
-      for (int i = 0; i < warp; ++i) before += s.scan[i];
-      return before;
+  bool summed = false;  // s.run has the weights above f_hi, where top-p's cut is not
+  float f_hi = 0.f, f_lo = 0.f;
+#pragma unroll 1
+  for (int top_p = 0; top_p < 2; ++top_p) {
+    if (top_p ? !(set.p < 1.f) : !set.k) continue;
+    // What top-k left for top-p, when it is few, is one bin.
+    const bool whole = top_p && set.k && set.k <= kList;
+    enum { kUnits, kStretch, kRanks, kOne } by = whole ? kOne : kUnits;
+    float scale = 0.f;
+    u64 hi = 0, lo = 0;
+    int shift = 0, bin = 0;
+    Step step = kCount;
+    bool estimate = top_p;  // the first histogram tells where to look
+    auto bin_of = [&](float f, int i) {  // of an alive entry, or -1
+      if (by == kUnits) return (int)units(f);
+      if (by == kOne) return 0;
+      if (!(f <= f_hi && f >= f_lo)) return -1;
+      if (by == kStretch) return min((int)((f_hi - f) * scale), kBins - 1);
+      const u64 r = rank_of(f, i);
+      return r >= lo && r <= hi ? (int)((hi - r) >> shift) : -1;
     };
-    // the entries of the leader's bin, of all CTAs, sorted into its list; too many: *crowded
-    auto gather = [&](int* crowded) {
-      const int bin = lead.bin;
-      each([&](uint32_t key, int i) {
-        if (key == 0 || bin_of(key) != bin) return;
-        const int at = atomicAdd(&lead.n_list, 1);
-        if (at < kList) {
-          lead.list.key[at] = key;
-          lead.list.idx[at] = i;
+    auto add_all = [&] {
+#pragma unroll 1
+      for (int v = 0; v < nv; ++v)
+#pragma unroll 1
+        for (int e = 0; e < VEC; ++e) {
+          const float f = entry(v * kThreads + tid, e);
+          const int b = alive(f) ? bin_of(f, index(v, e)) : -1;
+          if (b >= 0) add(b, w(f));
         }
-      });
-      cluster.sync();
-      if (rank == 0) {
-        List& t = s.list;
-        const int n = s.n_list;
-        if (n > kList) {
-          if (tid == 0) *crowded = 1;
+    };
+    if (whole) {
+      if (rank == 0 && tid == 0) s.n_list = 0;
+      sync();
+    }
+    while (!whole) {
+      for (int i = tid; i < kBins; i += kThreads)
+        s.h.digit[0][i] = s.h.digit[1][i] = s.h.digit[2][i] = s.h.count[i] = 0;
+      if (tid == 0 && step == kSums) s.n_near = 0;
+      __syncthreads();
+      if (step == kSums) {  // every weight: above the stretch, in its bins, below it
+        double below = 0.0;
+#pragma unroll 1
+        for (int v = 0; v < rounds; ++v) {
+          double above = 0.0;
+          if (v < nv) {
+            float f[VEC];
+            load(v, f);
+            unsigned some = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {  // no branch: the chains of operations overlap
+              const double x = w(f[e]);
+              if (f[e] > f_hi) above += x;
+              if (f[e] < f_lo) below += x;
+              some |= (unsigned)(f[e] <= f_hi && f[e] >= f_lo) << e;
+            }
+            while (some) {  // their bins come later, from all threads at once
+              const int at = atomicAdd(&s.n_near, 1);
+              if (at < kNear) s.near[at] = (v * kThreads + tid) * VEC + __ffs(some) - 1;
+              some &= some - 1;
+            }
+          }
+          above = warp_sum_d(above);
+          if (lane == 0) s.run[v * kWarps + warp] = above;
+        }
+        below = warp_sum_d(below);
+        if (lane == 0) s.red[warp] = below;
+        __syncthreads();
+        if (s.n_near <= kNear) {
+          for (int i = tid; i < s.n_near; i += kThreads) {
+            const float f = entry(s.near[i] / VEC, s.near[i] % VEC);
+            add(bin_of(f, 0), w(f));
+          }
         } else {
-          for (int i = tid; i < n; i += kThreads) {
-            const uint32_t key = t.key[i], idx = t.idx[i];
-            int before = 0;
-            for (int j = 0; j < n; ++j) before += t.key[j] > key || (t.key[j] == key && t.idx[j] < idx);
-            t.key_sorted[before] = key;
-            t.idx_sorted[before] = idx;
-            t.weight[before] = w(key);
+          add_all();
+        }
+        if (warp == 0) {
+          double t = 0.0;
+          for (int i = lane; i < rounds * kWarps; i += 32) t += s.run[i];
+          t = warp_sum_d(t);
+          const double y = warp_sum_d(lane < kWarps ? s.red[lane] : 0.0);
+          if (lane == 0) {
+            s.above_w = t;
+            s.below_w = y;
           }
         }
-        __syncthreads();
+      } else if (step == kCount && by == kUnits) {
+#pragma unroll 1
+        for (int v = 0; v < nv; ++v) {
+          float f[VEC];
+          load(v, f);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (alive(f[e])) atomicAdd(&s.h.count[(int)units(f[e])], 1u);
+        }
+      } else {
+        add_all();
       }
-    };
-
-    // The leader's decisions are read by the others only behind the next cluster.sync, and a field is
-    // written again only behind a later one.
-    bool by_bisection = false;
-    if (cut_k) {
+      // the leader's bins from every CTA's; each CTA adds up its share of them
+      sync();
+      const int share = kBins / C;
+      const bool counts = step == kCount && by == kUnits;
+      if (C > 1 || !counts) {
+        for (int i = rank * share + tid; i < (rank + 1) * share; i += kThreads) {
+          u64 ms = 0;
+          uint32_t cs = 0;
+#pragma unroll 4
+          for (int c = 0; c < C; ++c) {
+            const Bins& h = peer(c).h;
+            cs += h.count[i];
+            if (!counts) ms += h.digit[0][i] + ((u64)h.digit[1][i] << 15) + ((u64)h.digit[2][i] << 30);
+          }
+          lead.h.count[i] = cs;
+          if (!counts) {
+            lead.h.digit[0][i] = (uint32_t)ms;
+            lead.h.digit[1][i] = (uint32_t)(ms >> 32);
+          }
+        }
+      }
+      sync();
+      // The leader's decision, read by the others behind the next sync and changed behind a later one:
+      // the bin where the goal (a number of entries, or fixed-point weight) is reached.
       if (rank == 0) {
-        uint32_t c[PER], mine = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) mine += c[i] = s.all.count[tid * PER + i];
-        uint32_t before = (uint32_t)scan(mine);
-        if (tid == kThreads - 1 && before + mine < (uint32_t)kf) s.bisect_k = 1;  // outside the bins
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          if (before < (uint32_t)kf && before + c[i] >= (uint32_t)kf) {
-            s.bin = tid * PER + i;
-            s.need = kf - before;
-          }
-          before += c[i];
-        }
-      }
-      cluster.sync();
-      if (!lead.bisect_k) {
-        cluster.sync();  // (gather may raise it)
-        gather(&s.bisect_k);
-      }
-      if (rank == 0 && !s.bisect_k) {  // the first s.need of the list are kept
-        if (cut_p) {
-          // weight of the first k: the bins above and the kept entries
-          unsigned long long ms = 0;
-          for (int i = tid; i < s.bin; i += kThreads) ms += s.all.mass[i];
-          double d = (double)ms / kFixed;
-          for (int i = tid; i < (int)s.need; i += kThreads) d += s.list.weight[i];
-          d = warp_sum_d(d);
-          if (lane == 0) s.red[warp] = d;
-          __syncthreads();
-          if (tid == 0) {
-            double t = 0.0;
-            for (int i = 0; i < kWarps; ++i) t += s.red[i];
-            s.target = p * t;
-          }
-        }
-        if (tid == 0) {
-          s.tau = s.list.key_sorted[s.need - 1];
-          s.last = s.list.idx_sorted[s.need - 1];
-        }
-        __syncthreads();
-      }
-      cluster.sync();
-      by_bisection = lead.bisect_k;
-    }
-    if (cut_p && !by_bisection) {
-      if (rank == 0) {
-        const int k_bin = cut_k ? s.bin : kBins;  // its list is there already
-        unsigned long long c[PER], mine = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) mine += c[i] = s.all.mass[tid * PER + i];
-        unsigned long long before = scan(mine);
-        if (!cut_k && tid == kThreads - 1) {
-          const double in = (double)(before + mine) / kFixed;
-          s.target = p * (in + (double)s.rest_all / kFixed);
-          if (in < s.target) s.bisect_p = 1;  // outside the bins
-        }
-        __syncthreads();
-        const double target = s.target;
+        constexpr int PER = kBins / kThreads;
+        u64 c[PER], mine = 0, inc, above = 0, goal, all = 0;
+        double real = 0.0, square = 0.0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int b = tid * PER + i;
-          const double lo = (double)before / kFixed, hi = (double)(before + c[i]) / kFixed;
-          if (b < k_bin && lo < target && hi >= target) {
-            s.bin = b;
-            s.above = lo;
-            s.need = kList;
-            s.n_list = 0;
-            s.regather = 1;
+          if (estimate) {
+            const double x = exp2(-(b + 0.5) / per_bin * rate) * kFixed;
+            c[i] = (u64)(s.h.count[b] * x);
+            square += s.h.count[b] * x * x;
+          } else {
+            c[i] = !top_p ? s.h.count[b] : s.h.digit[0][b] | (u64)s.h.digit[1][b] << 32;
           }
-          if (b == k_bin && lo < target) s.above = lo;
-          before += c[i];
+          mine += c[i];
         }
-      }
-      cluster.sync();
-      const bool again = lead.regather && !lead.bisect_p;
-      cluster.sync();  // (gather may raise it)
-      if (again) gather(&s.bisect_p);
-      if (rank == 0 && !s.bisect_p) {
-        if (warp == 0) {
-          // entries kept: those whose predecessors weigh less than the target
-          const int n = min(s.n_list, (int)s.need);
-          double run = s.above;
-          int kept = 0;
-          for (int base = 0; base < n; base += 32) {
-            double inc = base + lane < n ? s.list.weight[base + lane] : 0.0;
+        inc = mine;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const double y = __shfl_up_sync(0xffffffffu, inc, o);
-              if (lane >= o) inc += y;
-            }
-            const double prev = __shfl_up_sync(0xffffffffu, inc, 1);
-            const bool in = base + lane < n && run + (lane ? prev : 0.0) < s.target;
-            kept += __popc(__ballot_sync(0xffffffffu, in));
-            run += __shfl_sync(0xffffffffu, inc, 31);
-          }
-          if (lane == 0) {
-            kept = max(kept, 1);
-            s.tau = s.list.key_sorted[kept - 1];
-            s.last = s.list.idx_sorted[kept - 1];
-          }
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += y;
+        }
+        square = warp_sum_d(square);
+        if (lane == 31) {
+          s.scan[warp] = inc;
+          s.red[warp] = square;
         }
         __syncthreads();
+        square = 0.0;
+        u64 before = inc - mine;
+        for (int i = 0; i < kWarps; ++i) {
+          if (i < warp) before += s.scan[i];
+          all += s.scan[i];
+          square += s.red[i];
+        }
+        if (by == kRanks) {
+          above = s.above;
+          goal = s.goal;
+          real = s.real_goal;
+        } else if (!top_p) {
+          goal = min((u64)set.k, all);
+        } else {
+          double beside = 0.0;
+          if (step == kSums) {
+            for (int i = 0; i < C; ++i) beside += peer(i).above_w;
+            above = (u64)(beside * kFixed);
+            for (int i = 0; i < C; ++i) beside += peer(i).below_w;
+          }
+          real = (double)set.p * (beside * kFixed + (double)all);
+          goal = max((u64)ceil(real), 1ull);
+        }
+        __syncthreads();  // everyone has read s.above and s.goal
+        before += above;
+        // A weight per bin is off by up to half a bin, T / 96, either way at each entry, 0.6% on average:
+        // the cut is looked for within 3.5 standard deviations of their sum.
+        const double slack = 0.02 * sqrt(square);
+        const u64 goal0 = (u64)max((double)goal - slack, 1.0), goal1 = min((u64)((double)goal + slack), all);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int b = tid * PER + i;
+          const u64 up_to = before + c[i];
+          if (!estimate) {
+            if (before < goal && up_to >= goal) {
+              s.above = before;
+              s.bin = b;
+              s.in_bin = s.h.count[b];
+            }
+          } else {
+            if (before < goal0 && up_to >= goal0) s.f_hi = b == 0 ? max_ : max_ - b / per_bin;
+            if (before < goal1 && up_to >= goal1) s.f_lo = b == kBins - 1 ? -3.4028235e38f : max_ - (b + 1) / per_bin;
+          }
+          before = up_to;
+        }
+        __syncthreads();
+        if (tid == 0) {
+          s.goal = goal;
+          s.real_goal = real;
+          s.n_list = 0;
+          s.next = estimate                                 ? kSums
+                   : goal <= above || goal > above + all    ? kWeigh  // the estimate was off
+                   : s.in_bin <= (uint32_t)kList            ? kGather
+                                                            : kDivide;
+        }
       }
-      cluster.sync();
-      by_bisection = lead.bisect_p;
-    }
-    if (!by_bisection) {
-      tau = lead.tau;
-      last = lead.last;
-    } else {
-      auto count = [&](uint32_t above) {
-        int c = 0;
-        each([&](uint32_t key, int) { c += key > above; });
-        return (int64_t)cluster_sum((double)c);
-      };
-      auto mass = [&](uint32_t above) {
-        double c = 0.0;
-        each([&](uint32_t key, int) {
-          if (key > above) c += w(key);
-        });
-        return cluster_sum(c);
-      };
-      const int64_t alive = count(0);
-      int64_t ties = a.vocab;
-      tau = K::kLowest;
-      if (cut_k && kf < alive) tau = cut_by_count<DT>(count, top, kf, ties);
-      if (cut_p) tau = cut_by_weight<DT>(count, mass, w, top, tau, p, a.vocab, ties);
-      int lo = 0, hi = a.vocab;  // entries equal to tau below index lo: fewer than ties; below hi: enough
-      while (hi - lo > 1) {
-        const int mid = lo + (hi - lo) / 2;
-        int c = 0;
-        each([&](uint32_t key, int i) { c += key == tau && i < mid; });
-        if ((int64_t)cluster_sum((double)c) >= ties) hi = mid; else lo = mid;
+      sync();
+      step = (Step)lead.next;
+      bin = lead.bin;
+      estimate = false;
+      if (step == kGather) break;
+      if (step == kSums) {
+        f_hi = lead.f_hi;
+        f_lo = lead.f_lo;
+        scale = (float)kBins / fmaxf(f_hi - f_lo, 1e-30f);
+        by = kStretch;
+        summed = true;
+      } else if (step == kWeigh) {
+        by = kUnits;
+        summed = false;
+      } else {  // kDivide: the bin's range of ranks
+        u64 a_hi = 0, a_lo = ~0ull;
+#pragma unroll 1
+        for (int v = 0; v < nv; ++v)
+#pragma unroll 1
+          for (int e = 0; e < VEC; ++e) {
+            const float f = entry(v * kThreads + tid, e);
+            if (!alive(f) || bin_of(f, index(v, e)) != bin) continue;
+            const u64 r = rank_of(f, index(v, e));
+            a_hi = max(a_hi, r);
+            a_lo = min(a_lo, r);
+          }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          a_hi = max(a_hi, __shfl_xor_sync(0xffffffffu, a_hi, o));
+          a_lo = min(a_lo, __shfl_xor_sync(0xffffffffu, a_lo, o));
+        }
+        if (lane == 0) {
+          s.scan[warp] = a_hi;
+          s.scan2[warp] = a_lo;
+        }
+        __syncthreads();
+        if (tid == 0) {
+          for (int i = 1; i < kWarps; ++i) {
+            a_hi = max(a_hi, s.scan[i]);
+            a_lo = min(a_lo, s.scan2[i]);
+          }
+          s.hi = a_hi;
+          s.lo = a_lo;
+        }
+        sync();
+        hi = 0;
+        lo = ~0ull;
+        for (int c = 0; c < C; ++c) {
+          hi = max(hi, peer(c).hi);
+          lo = min(lo, peer(c).lo);
+        }
+        if (!summed) {  // (the stretch stays as it is)
+          f_hi = value_of((uint32_t)(hi >> 32));
+          f_lo = value_of((uint32_t)(lo >> 32));
+        }
+        by = kRanks;
+        shift = max(64 - __clzll((long long)(hi - lo)) - 10, 0);  // at most 1024 bins
+        step = top_p ? kWeigh : kCount;
       }
-      last = hi - 1;
     }
+    // the bin's few entries, to the leader's list; few others pass the first comparison
+    const float g_hi = by == kOne ? INFINITY : by != kUnits ? f_hi : max_ - (bin - 0.5f) / per_bin;
+    const float g_lo = by == kOne || (by == kUnits && bin == kBins - 1) ? -INFINITY
+                       : by != kUnits                                   ? f_lo
+                                                                        : max_ - (bin + 1.5f) / per_bin;
+    auto offer = [&](int j, int e) {
+      const float f = entry(j, e);
+      const int i = first + (j - tid) * VEC + e;
+      if (bin_of(f, i) == bin) lead.list[atomicAdd(&lead.n_list, 1)] = rank_of(f, i);
+    };
+    const bool listed = summed && s.n_near <= kNear;
+    if (listed)
+      for (int i = tid; i < s.n_near; i += kThreads) offer(s.near[i] / VEC, s.near[i] % VEC);
+#pragma unroll 1
+    for (int v = 0; v < nv && !listed; ++v) {
+      float f[VEC];
+      load(v, f);
+      unsigned some = 0;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) some |= (unsigned)(f[e] <= g_hi && f[e] >= g_lo && alive(f[e])) << e;
+      while (some) {
+        offer(v * kThreads + tid, __ffs(some) - 1);
+        some &= some - 1;
+      }
+    }
+    sync();
+    if (rank == 0) {  // sorted, and cut at the goal
+      const int n = s.n_list;
+      if (tid < n) {
+        const u64 r = s.list[tid];
+        int before = 0;
+        for (int j = 0; j < n; ++j) before += s.list[j] > r;
+        s.sorted[before] = r;
+        if (top_p) s.weight[before] = w(value_of((uint32_t)(r >> 32))) * kFixed;
+      }
+      __syncthreads();
+      if (!top_p) {
+        if (tid == 0) s.cut = s.sorted[s.goal - s.above - 1];
+      } else if (warp == 0) {  // the last entry whose predecessors weigh less than the goal
+        double run = whole ? 0.0 : (double)s.above, goal = s.real_goal;
+        if (whole) {
+          double t = 0.0;
+          for (int i = lane; i < n; i += 32) t += s.weight[i];
+          goal = (double)set.p * warp_sum_d(t);
+        }
+        int kept = 0;
+#pragma unroll 1
+        for (int at = 0; at < n; at += 32) {
+          double inc = at + lane < n ? s.weight[at + lane] : 0.0;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+          }
+          const double prev = __shfl_up_sync(0xffffffffu, inc, 1);
+          const bool in = at + lane < n && run + (lane ? prev : 0.0) < goal;
+          kept += __popc(__ballot_sync(0xffffffffu, in));
+          run += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        if (lane == 0) s.cut = s.sorted[max(kept, 1) - 1];
+      }
+    }
+    sync();
+    cut_f = value_of((uint32_t)(lead.cut >> 32));
+    cut_i = (int)~(uint32_t)lead.cut;
+    if (!top_p) kill([&](float f, int i) { return keep(f, i) ? f : -INFINITY; });
   }
 
-  // 3: kept weights up to and with each run of 32 vectors (a warp's v-th), in index order
-  auto kept = [&](uint32_t key, int i) {
-    if (key == 0 || key < tau || (key == tau && (uint32_t)i > last)) return 0.0;
-    const double x = w(key);
-    return x >= m ? x : 0.0;
-  };
-  const int most = (rounds * kWarps + 31) / 32 * 32;  // runs, padded to whole warps
-  for (int i = tid; i < most; i += kThreads) s.run[i] = 0.0;
-  __syncthreads();
+  // 4: kept weights up to and with each run of 32 vectors (a warp's v-th), in index order
+  summed = summed && set.m == 0.0;  // the stretch of the cut adds to the sums above it
+  const float most = summed ? f_hi : INFINITY;
+  const int runs = (rounds * kWarps + 31) / 32 * 32;  // padded to whole warps
+  if (tid < runs - rounds * kWarps) s.run[rounds * kWarps + tid] = 0.0;
 #pragma unroll 1
   for (int v = 0; v < rounds; ++v) {
     double t = 0.0;
     if (v < nv) {
-      uint32_t key[VEC];
-      keys_of(v, key);
+      float f[VEC];
+      load(v, f);
+      unsigned some = 0;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) t += kept(key[e], index(v, e));
+      for (int e = 0; e < VEC; ++e)
+        some |= (unsigned)(f[e] >= cut_f && f[e] <= most && keep(f[e], index(v, e))) << e;
+      if (__popc(some) > 1) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const double x = w(f[e]);
+          t += (some >> e & 1) && x >= set.m ? x : 0.0;
+        }
+      } else if (some) {
+        const double x = w(entry(v * kThreads + tid, __ffs(some) - 1));
+        t = x >= set.m ? x : 0.0;
+      }
     }
-    t = warp_sum_d(t);
-    if (lane == 0) s.run[v * kWarps + warp] = t;
+    if (__any_sync(0xffffffffu, t != 0.0)) {
+      t = warp_sum_d(t);
+      if (lane == 0) s.run[v * kWarps + warp] = summed ? s.run[v * kWarps + warp] + t : t;
+    } else if (lane == 0 && !summed) {
+      s.run[v * kWarps + warp] = 0.0;
+    }
   }
   __syncthreads();
   if (warp == 0) {
     double carry = 0.0;
-    for (int base = 0; base < most; base += 32) {
-      double inc = s.run[base + lane];
+#pragma unroll 1
+    for (int at = 0; at < runs; at += 32) {
+      double inc = s.run[at + lane];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const double y = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += y;
       }
       inc += carry;
-      s.run[base + lane] = inc;
+      s.run[at + lane] = inc;
       carry = __shfl_sync(0xffffffffu, inc, 31);
     }
     if (lane == 0) s.total = carry;
   }
-  cluster.sync();
-  double start = 0.0, total = 0.0;
-  for (int i = 0; i < C; ++i) {
-    if (i == rank) start = total;
-    total += cluster.map_shared_rank(&s, i)->total;
-  }
-  float uf = a.u[row];
-  uf = uf > 0.f ? fminf(uf, 0.99999994f) : 0.f;
-  const double goal = (double)uf * total;
-  // the CTAs' stretches [start, start + total) share their borders' very values: one holds the goal
-  if (warp == 0 && start <= goal && goal < start + s.total) {
-    double here = goal - start;
-    int run = -1;
-    for (int base = 0; base < most && run < 0; base += 32) {
-      const unsigned hit = __ballot_sync(0xffffffffu, s.run[base + lane] > here);
-      if (hit) run = base + __ffs(hit) - 1;
+  sync();
+  if (warp == 0) {
+    double start = 0.0, total = 0.0;
+    for (int c = 0; c < C; ++c) {
+      if (c == rank) start = total;
+      total += peer(c).total;
     }
-    if (run < 0) {  // (by rounding alone) the last run with any weight
-      run = 0;
-      for (int i = 1; i < most; ++i)
-        if (s.run[i] > s.run[i - 1]) run = i;
-    }
-    here -= run ? s.run[run - 1] : 0.0;
-    // this warp reads the run's vectors in the place of the warp that owns them
-    const int j = run * 32 + lane, v0 = j * VEC + first - tid * VEC;
-    double part[VEC], t = 0.0;
-    const uint4 raw = j < per ? slice[j] : make_uint4(~0u, ~0u, ~0u, ~0u);
-    const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const uint32_t key = VEC == 4 ? K::of(word[e]) : K::of((e & 1) ? word[e / 2] >> 16 : word[e / 2] & 0xffffu);
-      t += part[e] = kept(key, v0 + e);
-    }
-    double inc = t;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double y = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += y;
-    }
-    const unsigned some = __ballot_sync(0xffffffffu, t > 0.0);
-    const unsigned hit = __ballot_sync(0xffffffffu, t > 0.0 && inc > here);
-    if (lane == (hit ? __ffs(hit) - 1 : 31 - __clz(some))) {
-      here -= inc - t;
-      double c = 0.0;
-      int at = 0;
-      bool done = false;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (done || !(part[e] > 0.0)) continue;
-        c += part[e];
-        at = e;
-        done = c > here;
+    const double goal = set.u * total;
+    // the CTAs' stretches [start, start + total) share their borders' very values: one holds the goal
+    if (start <= goal && goal < start + s.total) {
+      double here = goal - start;
+      int run = -1;
+#pragma unroll 1
+      for (int at = 0; at < runs && run < 0; at += 32) {
+        const unsigned hit = __ballot_sync(0xffffffffu, s.run[at + lane] > here);
+        if (hit) run = at + __ffs(hit) - 1;
       }
-      a.out[row] = v0 + at;
+      if (run < 0) {  // (by rounding alone) the last run with any weight
+        run = 0;
+        for (int i = 1; i < runs; ++i)
+          if (s.run[i] > s.run[i - 1]) run = i;
+      }
+      here -= run ? s.run[run - 1] : 0.0;
+      const int j = run * 32 + lane, i0 = first + (j - tid) * VEC;
+      auto kept = [&](int e) {
+        const float f = entry(j, e);
+        const double x = keep(f, i0 + e) ? w(f) : 0.0;
+        return x >= set.m ? x : 0.0;
+      };
+      double t = 0.0;
+      if (j < per)
+#pragma unroll 1
+        for (int e = 0; e < VEC; ++e) t += kept(e);
+      double inc = t;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      const unsigned some = __ballot_sync(0xffffffffu, t > 0.0);
+      const unsigned hit = __ballot_sync(0xffffffffu, t > 0.0 && inc > here);
+      if (some && lane == (hit ? __ffs(hit) - 1 : 31 - __clz(some))) {
+        here -= inc - t;
+        double c = 0.0;
+        int at = 0;
+#pragma unroll 1
+        for (int e = 0; e < VEC; ++e) {
+          const double x = kept(e);
+          c += x;
+          if (x > 0.0) at = e;
+          if (x > 0.0 && c > here) break;
+        }
+        a.out[row] = i0 + at;
+      }
     }
   }
-  cluster.sync();  // no CTA leaves while another may read its memory
+  if (C > 1) cluster.sync();  // no CTA leaves while another may read its memory
 }
 
 template <int DT>
@@ -713,10 +794,10 @@ int run_sample(const SampleArgs& a, cudaStream_t st) {
   const int64_t vectors = (a.vocab + VEC - 1) / VEC + 1;
   const int sms = device_info().sm_count;
   auto slice = [&](int c) { return (vectors + c - 1) / c * 16; };
-  // Larger clusters while a slice is large enough to keep a second CTA off the SM, or while SMs would
+  // The smallest cluster whose slices leave room for a second CTA on the SM; larger while SMs would
   // stay empty and every thread still has a vector.
   int c = 1;
-  while (c < 8 && (slice(c) > 48 * 1024 || (a.rows * c < sms && slice(c) > kThreads * 16))) c *= 2;
+  while (c < 8 && (slice(c) > 66 * 1024 || (a.rows * c < sms && slice(c) > kThreads * 16))) c *= 2;
   if (slice(c) > kMaxSlice || a.vocab > kMaxVocab) {
     sample_kernel<DT><<<(unsigned)a.rows, 512, 0, st>>>(a);
     return launch_status("sample");
