@@ -26,6 +26,10 @@ Every arithmetic step is one of this package's kernels:
                          reduces each vocab tile to (max, sum exp) and the target logit
                          (the logits are never stored; ignore_index masks the last position)
 Glue left to torch: the embedding gather.
+
+Answering (extend, generate) runs the same layers over a paged cache of keys and values
+(paged.PagedCache): the projections' q and k are rotated and k, v stored by ops.paged_append,
+the new tokens attend by ops.paged_attention, and ops.sample draws the next token.
 """
 from __future__ import annotations
 
@@ -34,6 +38,7 @@ from dataclasses import dataclass
 import torch
 
 from . import ops, shard
+from .paged import Batch, PagedCache
 
 
 @dataclass
@@ -221,6 +226,100 @@ class LlamaB200:
         return ops.linear(self.hidden(tokens), self.w["output.weight"])
 
     __call__ = forward
+
+    # ------------------------------------------------------------ over a paged cache
+
+    def new_cache(self, num_pages: int, page_size: int = 64) -> PagedCache:
+        """A paged cache for this model's layers, in its dtype and on its device."""
+        e = self.w["tok_embeddings.weight"]
+        return PagedCache(self.cfg.n_layers, self.cfg.n_kv_heads, self.cfg.head_dim, num_pages, page_size,
+                          e.dtype, e.device)
+
+    def _cached_attention(self, i: int, q, k, v, batch: Batch, cache: PagedCache, cos, sin) -> torch.Tensor:
+        """q [N, n_heads * hd] and k, v [N, n_kv_heads * hd] of layer i's new tokens: rotate q and k, store
+        k and v, attend."""
+        c, N = self.cfg, q.shape[0]
+        q = q.view(N, c.n_heads, c.head_dim)
+        ops.paged_append(k.view(N, c.n_kv_heads, c.head_dim), v.view(N, c.n_kv_heads, c.head_dim),
+                         cache.k[i], cache.v[i], *batch.lists, q=q, cos=cos, sin=sin, q_out=q)
+        return ops.paged_attention(q, cache.k[i], cache.v[i], *batch.lists).view(N, -1)
+
+    @torch.no_grad()
+    def extend(self, tokens: torch.Tensor, batch: Batch, cache: PagedCache) -> torch.Tensor:
+        """Run the packed new tokens [N] of a batch (cache.extend) and return the logits [B, vocab] that
+        follow the last one of each sequence."""
+        c, w = self.cfg, self.w
+        if tokens.shape != (batch.n_tokens,):
+            raise ValueError(f"extend: the batch holds {batch.n_tokens} tokens, got {tuple(tokens.shape)}")
+        # tables to the next power of two, so that decoding does not rebuild them at every step
+        cos, sin = self._tables(max(2048, 1 << (batch.max_len - 1).bit_length()), tokens.device)
+        h = torch.nn.functional.embedding(tokens, w["tok_embeddings.weight"])
+        ss = ops.row_sumsq(h) if self.fuse_norms else None
+        for i in range(c.n_layers):
+            p = f"layers.{i}."
+            wo, w2 = w[p + "attention.wo.weight"], w[p + "feed_forward.w2.weight"]
+            if self.fuse_norms:
+                wq, wk, wv, w1, w3 = self._fold(i)
+                q, k, v = (ops.linear_rms(h, x, ss, c.norm_eps) for x in (wq, wk, wv))
+                o = self._cached_attention(i, q, k, v, batch, cache, cos, sin)
+                _, ss = ops.linear_rms(o, wo, residual=h, out=h, want_ss=True)
+                hidden = ops.mlp_hidden_rms(h, w1, w3, ss, c.norm_eps)
+                _, ss = ops.linear_rms(hidden, w2, residual=h, out=h, want_ss=True)
+            else:
+                x = ops.rmsnorm_fp32(h, w[p + "attention_norm.weight"], c.norm_eps)
+                q, k, v = (ops.linear(x, w[p + f"attention.{n}.weight"]) for n in ("wq", "wk", "wv"))
+                o = self._cached_attention(i, q, k, v, batch, cache, cos, sin)
+                ops.linear(o, wo, residual=h, out=h)
+                x = ops.rmsnorm_fp32(h, w[p + "ffn_norm.weight"], c.norm_eps)
+                hidden = ops.mlp_hidden(x, w[p + "feed_forward.w1.weight"], w[p + "feed_forward.w3.weight"])
+                ops.linear(hidden, w2, residual=h, out=h)
+        last = h.index_select(0, batch.cu_q[1:] - 1)
+        return ops.linear(ops.rmsnorm_fp32(last, w["norm.weight"], c.norm_eps), w["output.weight"])
+
+    @torch.no_grad()
+    def generate(self, prompts: list[list[int]], max_new_tokens: int, temperature: float = 1.0,
+                 top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, stop: int | None = None,
+                 generator: torch.Generator | None = None,
+                 cache: PagedCache | None = None) -> list[list[int]]:
+        """Continue each prompt (token lists, at least one token each) by up to max_new_tokens sampled
+        tokens (ops.sample's settings; temperature 0 takes the likeliest).  A sequence ends with the
+        token `stop`, if given.  All sequences decode together; with `cache` they share its pages and
+        give them back at the end, otherwise one of the right size is made."""
+        if not prompts or min(len(p) for p in prompts) < 1 or max_new_tokens < 0:
+            raise ValueError("generate: need prompts of at least one token")
+        if max_new_tokens == 0:
+            return [[] for _ in prompts]
+        device = self.w["tok_embeddings.weight"].device
+        if cache is None:
+            size = 64
+            cache = self.new_cache(sum(-(-(len(p) + max_new_tokens) // size) for p in prompts), size)
+        live = list(range(len(prompts)))
+        seqs = [cache.add() for _ in prompts]
+        tokens = torch.tensor([t for p in prompts for t in p], device=device)
+        counts = [len(p) for p in prompts]
+        steps: list[tuple[list[int], torch.Tensor]] = []
+        try:
+            for step in range(max_new_tokens):
+                batch = cache.extend([seqs[i] for i in live], counts)
+                logits = self.extend(tokens, batch, cache)
+                u = torch.rand(len(live), device=device, generator=generator)
+                tokens = ops.sample(logits, u, temperature, top_k, top_p, min_p)
+                steps.append((live, tokens))
+                if stop is not None:
+                    on = (tokens != stop).tolist()
+                    tokens = tokens[torch.tensor(on, device=device)]
+                    live = [i for i, x in zip(live, on) if x]
+                    if not live:
+                        break
+                counts = [1] * len(live)
+        finally:
+            for s in seqs:
+                cache.release(s)
+        out: list[list[int]] = [[] for _ in prompts]
+        for rows, t in steps:
+            for i, x in zip(rows, t.tolist()):
+                out[i].append(x)
+        return out
 
     @staticmethod
     def next_token_targets(tokens: torch.Tensor) -> torch.Tensor:

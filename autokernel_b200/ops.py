@@ -596,41 +596,58 @@ def flash_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, causal: b
 
 # ---------------------------------------------------------------- serving
 
-def _i64s(*v: int):
-    return (ctypes.c_int64 * len(v))(*v)
+# Decoding calls these once per layer and token, so the checks read each property of a tensor once:
+# the call itself takes a few microseconds on the GPU.
+
+_I64x10, _I64x14 = ctypes.c_int64 * 10, ctypes.c_int64 * 14
 
 
-def _paged_lists(name: str, k_cache, v_cache, page_table, cu_q, kv_lens) -> tuple:
-    """Check the cache and the lists of a paged call; (B, Hkv, D)."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+def _same_device(*ts: torch.Tensor) -> torch.device:
+    """require_cuda, for tensors that are most often on the current device."""
+    i = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != i or i < 0:
+            return require_cuda(*ts)
+    if torch.cuda.current_device() != i:
+        torch.cuda.set_device(i)
+    return ts[0].device
+
+
+def _paged_cache(name: str, k_cache, v_cache, page_table, cu_q, kv_lens) -> tuple:
+    """Check the cache and the lists of a paged call: the cache's shape and strides, B and the
+    table's width and row stride."""
+    shape, ks, vs, dt = k_cache.shape, k_cache.stride(), v_cache.stride(), k_cache.dtype
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != dt:
         raise ValueError(f"{name}: k_cache and v_cache must be [pages, kv_heads, page_size, head_dim] alike")
-    if k_cache.shape[2] == 0 or k_cache.shape[1] == 0 or k_cache.shape[3] == 0:
+    if 0 in shape[1:]:
         raise ValueError(f"{name}: empty page")
-    for c in (k_cache, v_cache):
-        if c.stride(3) != 1 and c.shape[3] > 1:
-            raise ValueError(f"{name}: the caches' last dim must be contiguous")
+    if (ks[3] != 1 or vs[3] != 1) and shape[3] > 1:
+        raise ValueError(f"{name}: the caches' last dim must be contiguous")
     for what, t in (("page_table", page_table), ("cu_q", cu_q), ("kv_lens", kv_lens)):
         if t.dtype != torch.int32:
             raise ValueError(f"{name}: {what} must be int32, got {t.dtype}")
-    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    if B < 0 or cu_q.shape != (B + 1,) or page_table.dim() != 2 or page_table.shape[0] != B:
+    table, lens = page_table.shape, kv_lens.shape
+    if len(lens) != 1 or len(table) != 2 or table[0] != lens[0] or cu_q.shape != (lens[0] + 1,):
         raise ValueError(f"{name}: need kv_lens [B], cu_q [B + 1] and page_table [B, pages per sequence]")
-    if not (cu_q.is_contiguous() and kv_lens.is_contiguous()) or (
-            page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    ld, one = page_table.stride()
+    if not cu_q.is_contiguous() or not kv_lens.is_contiguous() or (one != 1 and table[1] > 1):
         raise ValueError(f"{name}: the lists (and the rows of page_table) must be contiguous")
-    return B, k_cache.shape[1], k_cache.shape[3]
+    return shape, ks, vs, dt, lens[0], table[1], ld
 
 
-def _tokens(name: str, what: str, x: torch.Tensor, heads, like: torch.Tensor, n=None) -> None:
-    """x must be [N, heads, D] of the cache's dtype and head_dim with a contiguous last dim."""
-    if (x.dim() != 3 or x.shape[2] != like.shape[3] or (heads is not None and x.shape[1] != heads)
-            or (n is not None and x.shape[0] != n) or x.shape[1] == 0):
-        raise ValueError(f"{name}: {what} must be [N, heads, head_dim] to go with the cache "
-                         f"{tuple(like.shape)}, got {tuple(x.shape)}")
-    if x.dtype != like.dtype:
-        raise ValueError(f"{name}: {what} is {x.dtype}, the cache {like.dtype}")
-    if x.stride(2) != 1 and x.shape[2] > 1:
+def _tokens(name: str, what: str, x: torch.Tensor, n, heads, D: int, dt: torch.dtype) -> tuple:
+    """x must be [n, heads, D] (n, heads: any if None) of the cache's type with a contiguous last
+    dim: its shape and strides."""
+    shape, st = x.shape, x.stride()
+    if (len(shape) != 3 or shape[2] != D or (heads is not None and shape[1] != heads)
+            or (n is not None and shape[0] != n) or shape[1] == 0):
+        raise ValueError(f"{name}: {what} must be [{'N' if n is None else n}, "
+                         f"{'heads' if heads is None else heads}, {D}] to go with the cache, got {tuple(shape)}")
+    if x.dtype != dt:
+        raise ValueError(f"{name}: {what} is {x.dtype}, the cache {dt}")
+    if st[2] != 1 and D > 1:
         raise ValueError(f"{name}: the last dim of {what} must be contiguous")
+    return shape, st
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -652,48 +669,50 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     is negative or has no page in the table is not stored; positions outside cos / sin give NaN.
     Two tokens of a call must not share a slot: what such a slot holds is undefined."""
     name = "paged_append"
-    B, Hkv, D = _paged_lists(name, k_cache, v_cache, page_table, cu_q, kv_lens)
-    N = k.shape[0] if k.dim() == 3 else None
-    _tokens(name, "k", k, Hkv, k_cache)
-    _tokens(name, "v", v, Hkv, k_cache, N)
+    (P, Hkv, S, D), kcs, vcs, dt, B, width, ld = _paged_cache(name, k_cache, v_cache, page_table, cu_q, kv_lens)
+    (N, _, _), ks = _tokens(name, "k", k, None, Hkv, D, dt)
+    _, vs = _tokens(name, "v", v, N, Hkv, D, dt)
     if D % 2:
         raise ValueError(f"{name}: head_dim must be even, got {D}")
-    if q is not None:
-        _tokens(name, "q", q, None, k_cache, N)
-    elif q_out is not None:
-        raise ValueError(f"{name}: q_out without q")
-    if (cos is None) != (sin is None):
-        raise ValueError(f"{name}: cos and sin go together")
-    if q is not None and cos is None:
-        raise ValueError(f"{name}: q is only rotated, so it needs cos and sin")
-    positions = 0
-    if cos is not None:
-        if (cos.shape != sin.shape or cos.dim() < 2 or cos.shape[-1] != D // 2
-                or cos.numel() != cos.shape[0] * (D // 2) or cos.shape[0] == 0):
+    on = [k_cache, v_cache, k, v, page_table, cu_q, kv_lens]
+    qp = op = cp = sp = None
+    positions = H = 0
+    if cos is not None and sin is not None:
+        shape = cos.shape
+        if (len(shape) < 2 or sin.shape != shape or shape[-1] != D // 2 or shape[0] == 0
+                or cos.numel() != shape[0] * shape[-1]):
             raise ValueError(f"{name}: cos and sin must be [positions, {D // 2}]")
         if cos.dtype != torch.float32 or sin.dtype != torch.float32:
             raise ValueError(f"{name}: cos and sin must be float32")
         if not (cos.is_contiguous() and sin.is_contiguous()):
             raise ValueError(f"{name}: cos and sin must be contiguous")
-        positions = cos.shape[0]
-    if q_out is not None:
-        _tokens(name, "q_out", q_out, q.shape[1], k_cache, N)
-    code = dtype_code(k_cache.dtype)
-    require_cuda(k_cache, *(t for t in (k, v, v_cache, page_table, cu_q, kv_lens, q, cos, sin, q_out)
-                            if t is not None))
-    if q is not None and q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    st = [_i64s(*t.stride()[:2]) if t is not None else None for t in (k, v, q, q_out)]
-    st += [_i64s(*t.stride()[:3]) for t in (k_cache, v_cache)]
-
-    def ptr(t):
-        return t.data_ptr() if t is not None else None
-
-    call("ak_paged_append", k.data_ptr(), v.data_ptr(), ptr(q), ptr(q_out), k_cache.data_ptr(),
-         v_cache.data_ptr(), page_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), ptr(cos),
-         ptr(sin), N, B, q.shape[1] if q is not None else 0, Hkv, D, k_cache.shape[0],
-         k_cache.shape[2], page_table.shape[1], page_table.stride(0), positions,
-         *st, code, stream_ptr(k.device))
+        positions, cp, sp = shape[0], cos.data_ptr(), sin.data_ptr()
+        on += (cos, sin)
+    elif cos is not None or sin is not None:
+        raise ValueError(f"{name}: cos and sin go together")
+    elif q is not None:
+        raise ValueError(f"{name}: q is only rotated, so it needs cos and sin")
+    qs = os = (0, 0)
+    if q is not None:
+        (_, H, _), qs = _tokens(name, "q", q, N, None, D, dt)
+        on.append(q)
+        if q_out is not None:
+            _, os = _tokens(name, "q_out", q_out, N, H, D, dt)
+            on.append(q_out)
+    elif q_out is not None:
+        raise ValueError(f"{name}: q_out without q")
+    code = dtype_code(dt)
+    dev = _same_device(*on)
+    if q is not None:
+        if q_out is None:
+            q_out = torch.empty_like(q)
+            os = q_out.stride()
+        qp, op = q.data_ptr(), q_out.data_ptr()
+    st = _I64x14(ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os[0], os[1], *kcs[:3], *vcs[:3])
+    at = ctypes.addressof(st)
+    call("ak_paged_append", k.data_ptr(), v.data_ptr(), qp, op, k_cache.data_ptr(), v_cache.data_ptr(),
+         page_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), cp, sp, N, B, H, Hkv, D, P, S, width, ld,
+         positions, at, at + 16, at + 32, at + 48, at + 64, at + 88, code, stream_ptr(dev))
     return q_out
 
 
@@ -712,9 +731,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (a fresh result is not initialised there).  Nothing behind a sequence's last key matters,
     whatever the cache holds there."""
     name = "paged_attention"
-    B, Hkv, D = _paged_lists(name, k_cache, v_cache, page_table, cu_q, kv_lens)
-    _tokens(name, "q", q, None, k_cache)
-    N, H, _ = q.shape
+    (P, Hkv, S, D), kcs, vcs, dt, B, width, ld = _paged_cache(name, k_cache, v_cache, page_table, cu_q, kv_lens)
+    (N, H, _), qs = _tokens(name, "q", q, None, None, D, dt)
     if H % Hkv:
         raise ValueError(f"{name}: {H} query heads are not a multiple of {Hkv} key/value heads")
     if D > 256:
@@ -723,19 +741,23 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         sm_scale = D ** -0.5
     if not 0 < sm_scale <= 3e38:
         raise ValueError(f"{name}: sm_scale must be positive and finite, got {sm_scale}")
-    if out is not None:
-        _tokens(name, "out", out, H, k_cache, N)
-    code = dtype_code(k_cache.dtype)
-    require_cuda(q, k_cache, v_cache, page_table, cu_q, kv_lens, *([out] if out is not None else []))
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    ws = torch.empty(_lib.load().ak_paged_attention_workspace_size(N, B, H, Hkv, D, code),
-                     dtype=torch.uint8, device=q.device)
-    st = [_i64s(*t.stride()[:2]) for t in (q, o)] + [_i64s(*t.stride()[:3]) for t in (k_cache, v_cache)]
-    call("ak_paged_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
-         page_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), N, B, H, Hkv, D,
-         k_cache.shape[0], k_cache.shape[2], page_table.shape[1], page_table.stride(0), *st,
-         1 if causal else 0, float(sm_scale), code, ws.data_ptr(), ws.numel(), stream_ptr(q.device))
-    return o
+    code = dtype_code(dt)
+    if out is None:
+        dev = _same_device(q, k_cache, v_cache, page_table, cu_q, kv_lens)
+        out = torch.empty_like(q)
+        os = out.stride()
+    else:
+        _, os = _tokens(name, "out", out, N, H, D, dt)
+        dev = _same_device(q, k_cache, v_cache, page_table, cu_q, kv_lens, out)
+    nbytes = _lib.load().ak_paged_attention_workspace_size(N, B, H, Hkv, D, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    st = _I64x10(qs[0], qs[1], os[0], os[1], *kcs[:3], *vcs[:3])
+    at = ctypes.addressof(st)
+    call("ak_paged_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+         page_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), N, B, H, Hkv, D, P, S, width, ld,
+         at, at + 16, at + 32, at + 56, 1 if causal else 0, sm_scale, code,
+         ws.data_ptr() if nbytes else None, nbytes, stream_ptr(dev))
+    return out
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: float | torch.Tensor = 1.0,
@@ -753,31 +775,37 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: float | torch.Ten
     (fp32; top_k int32).  NaN and -inf logits are never drawn (a row of nothing else gives -1);
     entries of +inf share all weight."""
     name = "sample"
-    if logits.dim() != 2 or logits.shape[1] == 0:
-        raise ValueError(f"{name}: logits must be [rows, vocab], got {tuple(logits.shape)}")
-    rows = logits.shape[0]
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"{name}: logits must be [rows, vocab], got {tuple(shape)}")
+    rows, vocab = shape
     if u.shape != (rows,) or u.dtype != torch.float32:
         raise ValueError(f"{name}: u must be float32 [{rows}]")
     code = dtype_code(logits.dtype)
-    settings = []
-    for what, v, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+    on, arrays, numbers = [], [], []
+    for what, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
         if isinstance(v, torch.Tensor):
+            dt = torch.int32 if what == "top_k" else torch.float32
             if v.shape != (rows,) or v.dtype != dt:
                 raise ValueError(f"{name}: a tensor of {what} must be {dt} [{rows}]")
-            settings.append(v.contiguous())
+            on.append(v if v.is_contiguous() else v.contiguous())
+            arrays.append(on[-1].data_ptr())
+            numbers.append(0)
         else:
-            settings.append(min(int(v), 2 ** 31 - 1) if dt == torch.int32 else float(v))
-            if settings[-1] < 0 or settings[-1] != settings[-1]:
+            if not v >= 0:
                 raise ValueError(f"{name}: {what} must not be negative, got {v}")
-    require_cuda(logits, u, *(v for v in settings if isinstance(v, torch.Tensor)))
-    x = logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
-    u = u.contiguous()
-    out = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    arrays = [v.data_ptr() if isinstance(v, torch.Tensor) else None for v in settings]
-    numbers = [0 if isinstance(v, torch.Tensor) else v for v in settings]
-    call("ak_sample", x.data_ptr(), u.data_ptr(), rows, x.shape[1], x.stride(0), code, *arrays,
-         *numbers, out.data_ptr(), stream_ptr(logits.device))
+            arrays.append(None)
+            numbers.append(min(int(v), 2 ** 31 - 1) if what == "top_k" else v)
+    dev = _same_device(logits, u, *on)
+    ld, one = logits.stride()
+    if one != 1 and vocab > 1:
+        logits = logits.contiguous()
+        ld = vocab
+    if not u.is_contiguous():
+        u = u.contiguous()
+    out = torch.empty(rows, dtype=torch.int64, device=dev)
+    call("ak_sample", logits.data_ptr(), u.data_ptr(), rows, vocab, ld, code, *arrays, *numbers,
+         out.data_ptr(), stream_ptr(dev))
     return out
 
 

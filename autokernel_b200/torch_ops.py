@@ -1,4 +1,5 @@
-"""The nine operators as a PyTorch dispatcher op set: ``torch.ops.autokernel_b200.<op>``.
+"""The nine operators, and the three that serve a model (paged_append, paged_attention, sample), as a
+PyTorch dispatcher op set: ``torch.ops.autokernel_b200.<op>``.
 
 AutoKernel exports an optimized kernel to the Hugging Face kernels layout as a TORCH_LIBRARY
 op set (export_hf.py:367-420; examples/hf_kernels_test/torch-ext/torch_binding.cpp:6-9:
@@ -35,6 +36,12 @@ _SCHEMAS = {
                   "str activation='silu') -> Tensor"),
     "flash_attention": ("flash_attention(Tensor Q, Tensor K, Tensor V, bool causal=True, "
                         "float? sm_scale=None) -> Tensor"),
+    "paged_append": ("paged_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+                     "Tensor page_table, Tensor cu_q, Tensor kv_lens, Tensor q, Tensor cos, Tensor sin) -> Tensor"),
+    "paged_attention": ("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, "
+                        "Tensor cu_q, Tensor kv_lens, bool causal=True, float? sm_scale=None) -> Tensor"),
+    "sample": ("sample(Tensor logits, Tensor u, float temperature=1.0, int top_k=0, float top_p=1.0, "
+               "float min_p=0.0) -> Tensor"),
 }
 
 
@@ -73,6 +80,18 @@ def _fake_attention(Q, K, V, causal=True, sm_scale=None):
     return Q.new_empty((*lead, Q.shape[-2], Q.shape[-1]))
 
 
+def _fake_paged_append(k, v, k_cache, v_cache, page_table, cu_q, kv_lens, q, cos, sin):
+    return torch.empty_like(q)
+
+
+def _fake_paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, causal=True, sm_scale=None):
+    return torch.empty_like(q)
+
+
+def _fake_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    return logits.new_empty(logits.shape[0], dtype=torch.int64)
+
+
 _IMPLS = {
     "rmsnorm": (_ops.rmsnorm, _fake_rows),
     "layernorm": (_ops.layernorm, _fake_rows),
@@ -83,6 +102,9 @@ _IMPLS = {
     "matmul": (_ops.matmul, _fake_matmul),
     "fused_mlp": (_ops.fused_mlp, _fake_fused_mlp),
     "flash_attention": (_ops.flash_attention, _fake_attention),
+    "paged_append": (_ops.paged_append, _fake_paged_append),
+    "paged_attention": (_ops.paged_attention, _fake_paged_attention),
+    "sample": (_ops.sample, _fake_sample),
 }
 
 for _name, _schema in _SCHEMAS.items():
