@@ -49,6 +49,19 @@ inline bool cache_tmap(CUtensorMap* m, const AttnArgs& a, const void* base, cons
   return make_tmap(m, a.dtype, 4, base, dims, strides, b);
 }
 
+// The same cache as [pages, heads, D / 64, slots, 64]: one box is `box` slots of a page with all of D,
+// chunk after chunk, so that one copy brings what cache_tmap's maps bring in D / 64.
+inline bool cache_tmap_5d(CUtensorMap* m, const AttnArgs& a, const void* base, const int64_t* st,
+                          int box) {
+  const uint64_t dims[5] = {64, (uint64_t)a.l.page_size, (uint64_t)a.D / 64, (uint64_t)a.Hkv,
+                            (uint64_t)a.l.num_pages};
+  const uint64_t strides[4] = {(uint64_t)(a.l.page_size > 1 ? st[2] : a.D) * 2, 128,
+                               (uint64_t)(a.Hkv > 1 ? st[1] : a.D) * 2,
+                               (uint64_t)(a.l.num_pages > 1 ? st[0] : a.D) * 2};
+  const uint32_t b[5] = {64, (uint32_t)box, (uint32_t)a.D / 64, 1, 1};
+  return make_tmap(m, a.dtype, 5, base, dims, strides, b);
+}
+
 // Launch a kernel that may begin while its predecessor on the stream finishes (it waits for it
 // with griddepcontrol.wait before it reads what that one wrote).
 template <class... P, class... A>

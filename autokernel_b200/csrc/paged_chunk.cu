@@ -127,14 +127,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     while (ok && walk.next(s)) {
       if (s.blk0 == s.blk1) continue;  // no keys: nothing to load
       const Ends ends = ends_of(a, p, s);
-      auto page_at = [&](int blk) {
-        const int key = blk * BKV + lane * p.box;
-        return lane < boxes && key < s.kv_hi ? page_of(a.l, s.b, key / a.l.page_size) : -2;
-      };
-      int ahead = page_at(s.blk0);
+      PageFeed feed;
+      feed.start(a, s, s.blk0 * boxes, p.box);
       for (int blk = s.blk0; blk < s.blk1; ++blk, ++g) {
-        const int st = g & 1, page = ahead;
-        if (blk + 1 < s.blk1) ahead = page_at(blk + 1);
+        const int st = g & 1;
+        feed.reach(a, s, blk * boxes, p.box);
         if (blk == s.blk0) {
           ok = nq == 0 || mbar_wait(&q_empty, (nq - 1) & 1, abort_p);
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
@@ -149,30 +146,29 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         ok = mbar_wait(&kv_empty[st], ((g >> 1) & 1) ^ 1, abort_p);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        const int key = blk * BKV + lane * p.box;
-        const int bad = __reduce_min_sync(0xffffffffu, page == -1 ? key : 0x7fffffff);
         // slots of a loaded page behind the last visible key: V must read as zeros there
         const int live = s.kv_hi - blk * BKV;
         const bool tail = live < BKV && live % p.box != 0;
         uint64_t* v_bar = tail ? &v_land : &v_full[st];
-        if (lane == 0) {
+        int bad = 0x7fffffff;
+        for (int i = 0; i < boxes; ++i) {
+          int page, slot;
+          feed.get(a.l, blk * boxes + i, page, slot, bad);
+          if (lane == 0) {
+            uint8_t* dst = smem + st * C::TILE_BYTES + i * p.box * 128;
+#pragma unroll
+            for (int c = 0; c < C::NC; ++c) {
+              tma_load_4d(dst + C::K_OFF + c * CHUNK_BYTES, &tk, &k_full[st], c * 64, slot, s.h, page);
+              tma_load_4d(dst + C::V_OFF + c * CHUNK_BYTES, &tv, v_bar, c * 64, slot, s.h, page);
+            }
+          }
+        }
+        if (lane == 0) {  // the phases cannot end before these arrivals
           s_bad[st] = bad;
           mbar_expect_tx(&k_full[st], C::TILE_BYTES);
           mbar_expect_tx(v_bar, C::TILE_BYTES);
         }
         __syncwarp();
-        if (lane < boxes) {
-          // no page: the coordinate behind the last page, which reads as zeros
-          const int pg = page < 0 ? a.l.num_pages : page;
-          const int slot = page < 0 ? 0 : key % a.l.page_size;
-          uint8_t* dst = smem + st * C::TILE_BYTES + lane * p.box * 128;
-#pragma unroll
-          for (int c = 0; c < C::NC; ++c)
-            tma_load_4d(dst + C::K_OFF + c * CHUNK_BYTES, &tk, &k_full[st], c * 64, slot, s.h, pg);
-#pragma unroll
-          for (int c = 0; c < C::NC; ++c)
-            tma_load_4d(dst + C::V_OFF + c * CHUNK_BYTES, &tv, v_bar, c * 64, slot, s.h, pg);
-        }
         if (tail) {
           ok = mbar_wait(&v_land, nv++ & 1, abort_p);
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }

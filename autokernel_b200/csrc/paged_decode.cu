@@ -4,9 +4,12 @@
 // types); the matrix work is small, so it runs on warp-level MMAs whose operands come from shared
 // memory, and everything else serves keeping loads in flight.  A tile is 16 query rows: the
 // heads of one key/value head's group (and the next tokens) share every key that is read.
-//   warp 0      TMA producer: a ring of {K, V} blocks of 64 keys, gathered page by page
-//               (a box is gcd(page_size, 64) slots of one page; 128-byte swizzle)
-//   warps 1..8  two groups of four take alternate blocks, a warp 16 keys of its block, each with
+//   warps 0..3  TMA producers of a ring of {K, V} blocks of 64 keys, gathered page by page (a box is
+//               gcd(page_size, 64) slots of one page; 128-byte swizzle): K and V, even and odd
+//               boxes.  One warp's copies leave about 140 cycles apart whatever their size, so
+//               a single producer took 1140 cycles for a block of 16-slot pages, more than the
+//               1400 / 2 that HBM needs (decode of 64 x 8K: 253 us; four producers: see below)
+//   warps 4..11 two groups of four take alternate blocks, a warp 16 keys of its block, each with
 //               its own running maximum, sum and output, joined through shared memory per segment
 // One CTA per SM; the line of paged_sched.cuh gives each the same number of keys.
 //
@@ -20,17 +23,20 @@ namespace paged {
 
 using namespace sm100;
 
-constexpr int kRows = 16, kBlk = 64, kWarps = 8, kThreads = 32 * (kWarps + 1);
-constexpr int kChunk = kBlk * 128;  // 64 keys x 64 16-bit elements
+constexpr int kRows = 16, kBlk = 64, kWarps = 8, kProducers = 4, kThreads = 32 * (kWarps + kProducers);
 
 template <int D>
 struct DecodeCfg {
   static constexpr int NC = D / 64;
-  static constexpr int HALF = NC * kChunk;       // K or V of one block
+  static constexpr int HALF = kBlk * D * 2;      // K or V of one block
   static constexpr int STAGE = 2 * HALF;
-  static constexpr int STAGES = 160 * 1024 / STAGE;
-  static constexpr int O_OFF = STAGES * STAGE;   // float [8][16][D]
-  static constexpr int SMEM = O_OFF + kWarps * kRows * D * 4 + 1024;
+  // Even: then a ring slot always belongs to the same group of consumer warps, which waits for each of
+  // its phases in turn.  (A group that came to a slot every other phase could take the phase
+  // before last, whose parity is the same, for the one it waits for.)
+  static constexpr int STAGES = 192 * 1024 / STAGE;
+  static_assert(STAGES % 2 == 0, "a ring slot must belong to one group");
+  static constexpr int O_OFF = STAGES * STAGE;   // float [4][16][D]
+  static constexpr int SMEM = O_OFF + kWarps / 2 * kRows * D * 4 + 1024;
 };
 
 static TileRule decode_rule() { return TileRule{kRows, 0, kBlk, 64, 256}; }
@@ -99,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* s_o = reinterpret_cast<float*>(smem + C::O_OFF);
   __shared__ uint64_t full[C::STAGES], empty[C::STAGES];
   __shared__ int s_bad[C::STAGES];  // first key of the block without a page
-  __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+  __shared__ float s_m[kWarps / 2][kRows], s_l[kWarps / 2][kRows];
   __shared__ int s_badw[kWarps];
   __shared__ int s_again;           // rows to look at again (bits)
   __shared__ int abort_flag, s_stop;
@@ -108,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::STAGES; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], kProducers);
       mbar_init(&empty[i], 4);
     }
     abort_flag = 0;
@@ -124,47 +130,44 @@ __global__ void __launch_bounds__(kThreads, 1)
   Segment s;
   int g = 0;  // ring slots used so far
 
-  if (warp == 0) {  // ---------------------------------------------------- TMA producer
+  if (warp < kProducers) {  // ------------------------------------------- TMA producers
     const int boxes = kBlk / box;
+    const CUtensorMap* map = (warp & 1) ? &tv : &tk;
+    const int i0 = warp >> 1, mine = (boxes - i0 + 1) / 2;  // boxes i0, i0 + 2, ...
+    uint8_t* const dst = smem + ((warp & 1) ? C::HALF : 0);
     while (walk.next(s)) {
-      // this lane's page of block blk
-      auto page_at = [&](int blk) {
-        const int key = blk * kBlk + lane * box;
-        return lane < boxes && key < s.kv_hi ? page_of(a.l, s.b, key / a.l.page_size) : -2;
-      };
-      int ahead = s.blk0 < s.blk1 ? page_at(s.blk0) : -2;
+      PageFeed feed;
+      if (s.blk0 < s.blk1) feed.start(a, s, s.blk0 * boxes, box);
       for (int blk = s.blk0; blk < s.blk1; ++blk, ++g) {
-        const int st = g % C::STAGES, page = ahead;
-        if (blk + 1 < s.blk1) ahead = page_at(blk + 1);
+        const int st = g % C::STAGES;
+        feed.reach(a, s, blk * boxes, box);
         const bool ok = mbar_wait(&empty[st], ((g / C::STAGES) & 1) ^ 1, abort_p);
         if (!__all_sync(0xffffffffu, ok)) break;
-        const int key = blk * kBlk + lane * box;
-        const int bad = __reduce_min_sync(0xffffffffu, page == -1 ? key : 0x7fffffff);
-        if (lane == 0) {
-          s_bad[st] = bad;
-          mbar_expect_tx(&full[st], C::STAGE);
+        int bad = 0x7fffffff;
+        for (int i = 0; i < boxes; ++i) {
+          int page, slot;
+          feed.get(a.l, blk * boxes + i, page, slot, bad);
+          if (lane == 0 && (i & 1) == i0)
+            tma_load_5d(dst + st * C::STAGE + i * (C::NC * box * 128), map, &full[st], 0, slot, 0, s.h, page);
         }
-        __syncwarp();
-        if (lane < boxes) {
-          // no page: the coordinate behind the last page, which reads as zeros
-          const int p = page < 0 ? a.l.num_pages : page;
-          const int slot = page < 0 ? 0 : key % a.l.page_size;
-          uint8_t* dst = smem + st * C::STAGE + lane * box * 128;
-#pragma unroll
-          for (int c = 0; c < C::NC; ++c) {
-            tma_load_4d(dst + c * kChunk, &tk, &full[st], c * 64, slot, s.h, p);
-            tma_load_4d(dst + C::HALF + c * kChunk, &tv, &full[st], c * 64, slot, s.h, p);
-          }
+        if (lane == 0) {  // the phase cannot end before these arrivals, so `bad` is there with the data
+          if (warp == 0) s_bad[st] = bad;
+          if (mine) mbar_expect_tx(&full[st], mine * C::NC * box * 128); else mbar_arrive(&full[st]);
         }
       }
       if (*abort_p) break;
     }
     // giving up: the copies in flight still land in this CTA's shared memory
-    if (*abort_p && lane == 0) drain_ring(full, C::STAGES, g);
+    if (*abort_p && lane == 0 && warp == 0) drain_ring(full, C::STAGES, g);
   } else {  // ---------------------------------------------------------------- consumers
-    const int cw = warp - 1, grp = cw >> 2, k16 = (cw & 3) * 16;  // the warp's keys of its blocks
+    const int cw = warp - kProducers, grp = cw >> 2, k16 = (cw & 3) * 16;  // the warp's keys of its blocks
     const int r0 = lane >> 2, cq = 2 * (lane & 3);
     const uint32_t ring = smem_u32(smem);
+    // a block lies box by box: [64 / box][D / 64][box slots][128 bytes]
+    const uint32_t chunk = box * 128;
+    auto row_at = [&](int row) { return (uint32_t)(row / box * (C::NC * box) + row % box) * 128; };
+    const uint32_t krow[2] = {row_at(k16 + (lane & 7)), row_at(k16 + 8 + (lane & 7))};
+    const uint32_t vrow = row_at(k16 + (lane & 15));
     const int cap = capacity(a.l);
     bool ok = true;
     while (ok && walk.next(s)) {
@@ -208,12 +211,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-          const int row = k16 + n * 8 + (lane & 7);
 #pragma unroll
           for (int kk = 0; kk < D / 32; ++kk) {  // 32 dims a load
             const int unit = (kk & 1) * 4 + (lane >> 3);
             uint32_t kf[4];
-            ldmatrix4(kf, kbase + (kk >> 1) * kChunk + row * 128 + ((unit ^ (row & 7)) << 4));
+            ldmatrix4(kf, kbase + krow[n] + (kk >> 1) * chunk + ((unit ^ (lane & 7)) << 4));
             mma16816<DT>(sc[n], q[2 * kk], kf[0], kf[1]);
             mma16816<DT>(sc[n], q[2 * kk + 1], kf[2], kf[3]);
           }
@@ -271,12 +273,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int k = key0 + 8 * i + cq;
           mask[i] = k + 1 < s.kv_hi ? 0xffffffffu : k < s.kv_hi ? 0x0000ffffu : 0u;
         }
-        const int vrow = k16 + (lane & 15);
 #pragma unroll
         for (int n = 0; n < NF / 2; ++n) {  // 16 dims a load
           const int unit = (n & 3) * 2 + (lane >> 4);
           uint32_t vf[4];
-          ldmatrix4t(vf, vbase + (n >> 2) * kChunk + vrow * 128 + ((unit ^ (vrow & 7)) << 4));
+          ldmatrix4t(vf, vbase + vrow + (n >> 2) * chunk + ((unit ^ (lane & 7)) << 4));
           vf[0] &= mask[0];
           vf[1] &= mask[1];
           vf[2] &= mask[0];
@@ -289,22 +290,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
       }
-      // join the eight warps
+      // join the eight warps: the second group's into the first's registers, then those four
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        const int row = r0 + 8 * i;
-        if (row < nr) {
+      }
+      const int w4 = cw & 3;
+      auto put = [&] {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = r0 + 8 * i;
+          if (row >= nr) continue;
           if ((lane & 3) == 0) {
-            s_m[cw][row] = m[i];
-            s_l[cw][row] = l[i];
+            s_m[w4][row] = m[i];
+            s_l[w4][row] = l[i];
           }
 #pragma unroll
           for (int n = 0; n < NF; ++n)
-            *reinterpret_cast<float2*>(s_o + (cw * kRows + row) * D + ((n * 8 + cq) ^ ((row & 7) * 8))) =
+            *reinterpret_cast<float2*>(s_o + (w4 * kRows + row) * D + ((n * 8 + cq) ^ ((row & 7) * 8))) =
                 make_float2(o[n][2 * i], o[n][2 * i + 1]);
         }
+      };
+      if (grp == 1) put();
+      group_sync();
+      if (grp == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = r0 + 8 * i;
+          if (row >= nr) continue;
+          const float m1 = s_m[w4][row], mn = fmaxf(m[i], m1), ref = mn == -INFINITY ? 0.f : mn;
+          const float f0 = ex2_approx(m[i] - ref), f1 = ex2_approx(m1 - ref);
+          l[i] = l[i] * f0 + s_l[w4][row] * f1;
+          m[i] = mn;
+#pragma unroll
+          for (int n = 0; n < NF; ++n) {
+            const float2 x = *reinterpret_cast<const float2*>(s_o + (w4 * kRows + row) * D +
+                                                              ((n * 8 + cq) ^ ((row & 7) * 8)));
+            o[n][2 * i] = o[n][2 * i] * f0 + x.x * f1;
+            o[n][2 * i + 1] = o[n][2 * i + 1] * f0 + x.y * f1;
+          }
+        }
+        __syncwarp();  // a row's four lanes have read its m and l
+        put();
       }
       if (lane == 0) s_badw[cw] = bad;
       // a warp that gave up still meets the others here; the results no longer count then
@@ -314,15 +342,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int w = 0; w < kWarps; ++w) first_bad = min(first_bad, s_badw[w]);
       const bool again = a.causal && s.t_hi - s.t_lo > 1;  // rows of the tile hide keys from one another
       float* part = ws + ((int64_t)blockIdx.x * 2 + s.slot) * (kRows * (D + 2));
-      for (int e = threadIdx.x - 32; e < nr * D; e += 32 * kWarps) {
+      for (int e = threadIdx.x - 32 * kProducers; e < nr * D; e += 32 * kWarps) {
         const int row = e / D, d = e % D;
         float top = s_m[0][row];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][row]);
+        for (int w = 1; w < kWarps / 2; ++w) top = fmaxf(top, s_m[w][row]);
         const float ref = top == -INFINITY ? 0.f : top;
         float sum = 0.f, x = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < kWarps / 2; ++w) {
           const float f = ex2_approx(s_m[w][row] - ref);
           sum = fmaf(s_l[w][row], f, sum);
           x = fmaf(s_o[(w * kRows + row) * D + (d ^ ((row & 7) * 8))], f, x);
@@ -344,13 +372,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (threadIdx.x == 32) s_stop = *abort_p;  // one reading, so that all warps leave together
+      if (threadIdx.x == 32 * kProducers) s_stop = *abort_p;  // one reading, so that all warps leave together
       group_sync();
       ok = !s_stop;
       if (s.whole && again) {
         const int rows = s_again;
         group_sync();
-        if (threadIdx.x == 32) s_again = 0;
+        if (threadIdx.x == 32 * kProducers) s_again = 0;
         for (int row = cw; row < nr; row += kWarps) {
           if (!(rows >> row & 1)) continue;
           const int t = (int)((row0 + row) / a.G), h = s.h * a.G + (int)((row0 + row) % a.G);
@@ -433,7 +461,7 @@ template <int DT, int D>
 static int launch_decode(const AttnArgs& a, float* ws, cudaStream_t st) {
   const int box = gcd_int(a.l.page_size, kBlk);
   CUtensorMap tk, tv;
-  if (!cache_tmap(&tk, a, a.k, a.kcs, box) || !cache_tmap(&tv, a, a.v, a.vcs, box))
+  if (!cache_tmap_5d(&tk, a, a.k, a.kcs, box) || !cache_tmap_5d(&tv, a, a.v, a.vcs, box))
     return AK_ERR_LAUNCH;
   const cudaError_t attr = smem_optin<decode_kernel<DT, D>>(DecodeCfg<D>::SMEM);
   AK_REQUIRE(attr == cudaSuccess, AK_ERR_LAUNCH, "paged_attention smem attribute: %s",

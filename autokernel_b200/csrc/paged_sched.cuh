@@ -210,6 +210,49 @@ struct Walker {
   }
 };
 
+// Page numbers of consecutive boxes of a tile's keys, for a whole warp: 32 are loaded at once and the
+// next 32 while those are used (a load per block, used at once, bounded the producer: about 2000
+// cycles a block).  Nothing touches a loaded number before its box is asked for.
+struct PageFeed {
+  int raw, slot, key;                 // this lane's box of the current 32: table entry, slot, first key
+  int next_raw, next_slot, next_key;
+  int base;                           // first box of the current 32
+  AK_D void fetch(const AttnArgs& a, const Segment& s, int first, int box, int& r, int& sl, int& k) {
+    const int64_t at = ((int64_t)first + (threadIdx.x & 31)) * box;
+    r = -2;  // behind the last key
+    k = 0x7fffffff;
+    sl = 0;
+    if (at < s.kv_hi) {
+      k = (int)at;
+      const int i = k / a.l.page_size;
+      sl = k - i * a.l.page_size;
+      r = __ldg(a.l.page_table + (int64_t)s.b * a.l.table_ld + i);  // kv_hi is within the table
+    }
+  }
+  AK_D void start(const AttnArgs& a, const Segment& s, int first, int box) {
+    base = first;
+    fetch(a, s, first, box, raw, slot, key);
+    fetch(a, s, first + 32, box, next_raw, next_slot, next_key);
+  }
+  // makes box i (at most 32 behind the last one asked for) current
+  AK_D void reach(const AttnArgs& a, const Segment& s, int i, int box) {
+    if (i < base + 32) return;
+    base += 32;
+    raw = next_raw;
+    slot = next_slot;
+    key = next_key;
+    fetch(a, s, base + 32, box, next_raw, next_slot, next_key);
+  }
+  // page and slot of box i: a page that does not exist (and slot 0) where the key has none, its key
+  // then in `bad` if the tile needs it
+  AK_D void get(const PagedLists& l, int i, int& page, int& slot_, int& bad) const {
+    const bool ok = (unsigned)raw < (unsigned)l.num_pages;
+    page = __shfl_sync(0xffffffffu, ok ? raw : l.num_pages, i - base);
+    slot_ = __shfl_sync(0xffffffffu, ok ? slot : 0, i - base);
+    bad = min(bad, __shfl_sync(0xffffffffu, ok ? 0x7fffffff : key, i - base));
+  }
+};
+
 // ------------------------------------------------------------------ rows read key by key
 // The matrix instructions multiply a hidden key's value by a weight of 0, which is NaN when the
 // value is not finite.  A row whose result is not finite although its sum of weights is, and
