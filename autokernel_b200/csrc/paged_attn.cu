@@ -120,7 +120,7 @@ static bool tc_ok(const AttnArgs& a) {
   if (force_simt() || a.dtype == AK_F32 || (a.D != 64 && a.D != 128) || a.l.page_size % 8 || a.G > 128)
     return false;
   if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.o)) return false;
-  if (a.l.num_pages == 0) return false;
+  if (a.l.num_pages == 0 || (int64_t)a.l.N * a.G >= (1LL << 31)) return false;
   auto ok = [](int64_t size, int64_t stride) {
     return size <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1LL << 38));
   };

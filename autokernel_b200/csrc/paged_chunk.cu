@@ -443,49 +443,52 @@ __global__ void __launch_bounds__(128)
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr int V = D / 16;  // float4 of a row per thread
-  const int c = blockIdx.x + 1;
-  const Line line = find_piece(a, p.rule, pieces, c);
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // in every block, also one without a part
-  if (line.x < 0) return;
-  Segment s;
-  s.b = line.b;
-  s.r = seq_range(a.l, s.b);
-  const SeqCost sc = seq_cost(a, p.rule, s.r);
-  const int64_t head = sc.total();
-  int64_t y = line.x - line.b_at;
-  s.h = (int)(y / head);
-  y -= s.h * head;
-  s.tile = sc.find(y);
-  const int64_t at = line.x - (y - sc.prefix(s.tile)), cost = sc.cost(s.tile);
-  if (at == line.x || at < (int64_t)(c - 1) * line.q) return;  // not the item's first boundary
-  const int last = (int)((at + cost - 1) / line.q);
+  __shared__ int s_slot[kParts];
+  __shared__ int s_whole, s_again;
+  if (threadIdx.x == 0) s_whole = s_again = 0;
+  Line line;
+  const Parts parts = find_parts(a, p.rule, pieces, line);
+  if (parts.n == 0) return;
+  const Segment& s = parts.s;
   const int lane = threadIdx.x & 31, part_d = threadIdx.x >> 5;
   const int prow = blockIdx.y * 32 + lane, x = prow / BQ, row = prow % BQ;
-  set_blocks(a, p.rule, cost, 0, cost, s);
   const int tok = s.t_lo + x * p.tt + row / a.G;
   const bool valid = row < p.tt * a.G && tok < s.t_hi;
   float top = -INFINITY, sum = 0.f;
   float4 acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int q = c - 1; q <= last; ++q) {
-    const int64_t from = (int64_t)q * line.q;
-    set_blocks(a, p.rule, cost, max(from - at, (int64_t)0), min(cost, from + line.q - at), s);
-    if (s.whole || s.nb == 0) return;  // written by the CTA that has all of it
-    if (s.blk0 >= s.blk1 || !valid) continue;
-    const float* part = p.ws + ((int64_t)q * 2 + (from >= at ? 0 : 1)) * C::PART;
-    const float m = __ldcg(part + ROWS * D + prow), l = __ldcg(part + ROWS * D + ROWS + prow);
-    const float mn = fmaxf(top, m), ref = mn == -INFINITY ? 0.f : mn;
-    const float f0 = ex2_approx(top - ref), f1 = ex2_approx(m - ref);
-    top = mn;
-    sum = sum * f0 + l * f1;
+  for (int i0 = 0; i0 < parts.n; i0 += kParts) {
+    const int n = min(kParts, parts.n - i0);
+    __syncthreads();
+    if (threadIdx.x < n) {
+      bool whole;
+      s_slot[threadIdx.x] = part_slot(a, p.rule, line, parts, i0 + threadIdx.x, whole);
+      if (whole) s_whole = 1;
+    }
+    __syncthreads();
+    if (s_whole) return;  // written by the CTA that has all of it
+    if (!valid) continue;
+#pragma unroll 2
+    for (int i = 0; i < n; ++i) {
+      if (s_slot[i] < 0) continue;
+      const float* part = p.ws + (int64_t)s_slot[i] * C::PART;
+      float4 v[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(part) + (part_d * V + i) * ROWS + prow);
-      acc[i].x = acc[i].x * f0 + v.x * f1;
-      acc[i].y = acc[i].y * f0 + v.y * f1;
-      acc[i].z = acc[i].z * f0 + v.z * f1;
-      acc[i].w = acc[i].w * f0 + v.w * f1;
+      for (int k = 0; k < V; ++k)
+        v[k] = __ldcg(reinterpret_cast<const float4*>(part) + (part_d * V + k) * ROWS + prow);
+      const float m = __ldcg(part + ROWS * D + prow), l = __ldcg(part + ROWS * D + ROWS + prow);
+      const float mn = fmaxf(top, m), ref = mn == -INFINITY ? 0.f : mn;
+      const float f0 = ex2_approx(top - ref), f1 = ex2_approx(m - ref);
+      top = mn;
+      sum = sum * f0 + l * f1;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        acc[k].x = acc[k].x * f0 + v[k].x * f1;
+        acc[k].y = acc[k].y * f0 + v[k].y * f1;
+        acc[k].z = acc[k].z * f0 + v[k].z * f1;
+        acc[k].w = acc[k].w * f0 + v[k].w * f1;
+      }
     }
   }
   bool odd = false;
@@ -508,9 +511,6 @@ __global__ void __launch_bounds__(128)
     }
   }
   odd = odd && fabsf(sum) <= 3.4028235e38f && visible_keys(s.r, tok, a.causal) < s.kv_hi;
-  __shared__ int s_again;
-  if (threadIdx.x == 0) s_again = 0;
-  __syncthreads();
   if (odd) atomicOr(&s_again, 1 << lane);
   __syncthreads();
   for (int i = part_d; i < 32 && s_again; i += 4) {
@@ -526,7 +526,7 @@ static int launch(const AttnArgs& a, float* ws, cudaStream_t st) {
   Params p{};
   p.tt = BQ / a.G;
   p.box = gcd_int(a.l.page_size, BKV);
-  p.rule = TileRule{0, 2 * p.tt, BKV, 128, 512};
+  p.rule = TileRule{0, 2 * p.tt, 7, 128, 512};
   const int fmt = DT == AK_BF16 ? 1 : 0;
   p.idesc_qk = idesc_f16(fmt, BQ, BKV, false, false);
   p.idesc_pv = idesc_f16(fmt, BQ, D, false, true);

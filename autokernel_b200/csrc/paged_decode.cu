@@ -39,7 +39,7 @@ struct DecodeCfg {
   static constexpr int SMEM = O_OFF + kWarps / 2 * kRows * D * 4 + 1024;
 };
 
-static TileRule decode_rule() { return TileRule{kRows, 0, kBlk, 64, 256}; }
+static TileRule decode_rule() { return TileRule{kRows, 0, 6, 64, 256}; }
 
 static size_t decode_part_floats(int D) { return (size_t)kRows * (D + 2); }
 
@@ -171,14 +171,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int cap = capacity(a.l);
     bool ok = true;
     while (ok && walk.next(s)) {
-      const int64_t row0 = (int64_t)s.tile * kRows;
-      const int nr = (int)min((int64_t)kRows, (int64_t)s.r.n * a.G - row0);
+      const int row0 = s.tile * kRows;
+      const int nr = min(kRows, s.r.n * a.G - row0);
       const T* qrow[2];
       int vis[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int rr = min(r0 + 8 * i, nr - 1);
-        const int t = (int)((row0 + rr) / a.G), hg = (int)((row0 + rr) % a.G);
+        const int t = (row0 + rr) / a.G, hg = (row0 + rr) % a.G;
         qrow[i] = reinterpret_cast<const T*>(a.q) + (int64_t)(s.r.begin + t) * a.qs[0] +
                   (int64_t)(s.h * a.G + hg) * a.qs[1];
         vis[i] = visible_keys(s.r, t, a.causal);
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           sum = fmaf(s_l[w][row], f, sum);
           x = fmaf(s_o[(w * kRows + row) * D + (d ^ ((row & 7) * 8))], f, x);
         }
-        const int t = (int)((row0 + row) / a.G), hg = (int)((row0 + row) % a.G);
+        const int t = (row0 + row) / a.G, hg = (row0 + row) % a.G;
         const int v = visible_keys(s.r, t, a.causal);
         if (v > first_bad) sum = __int_as_float(0x7fffffff);
         if (s.whole) {
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (threadIdx.x == 32 * kProducers) s_again = 0;
         for (int row = cw; row < nr; row += kWarps) {
           if (!(rows >> row & 1)) continue;
-          const int t = (int)((row0 + row) / a.G), h = s.h * a.G + (int)((row0 + row) % a.G);
+          const int t = (row0 + row) / a.G, h = s.h * a.G + (row0 + row) % a.G;
           if (hidden_not_finite<DT>(a, s.b, s.h, visible_keys(s.r, t, a.causal), s.kv_hi))
             row_by_key<DT>(a, s.b, s.r, t, h);
         }
@@ -391,57 +391,82 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of the tile that boundary blockIdx.x + 1 cuts first.
+// Joins the parts of the tile that boundary blockIdx.x + 1 cuts first.  The parts' maxima and sums
+// come first, all at once; then every output element is a sum of independent loads.
 template <int DT, int D>
 __global__ void __launch_bounds__(128)
     decode_join_kernel(const __grid_constant__ AttnArgs a, const TileRule rule, int pieces,
                        const float* ws) {
   using E = Elem<DT>;
   using T = typename E::T;
-  const int c = blockIdx.x + 1;
-  const Line line = find_piece(a, rule, pieces, c);
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // in every block, also one without a part
-  if (line.x < 0) return;
-  Segment s;
-  s.b = line.b;
-  s.r = seq_range(a.l, s.b);
-  const SeqCost sc = seq_cost(a, rule, s.r);
-  const int64_t head = sc.total();
-  int64_t y = line.x - line.b_at;
-  s.h = (int)(y / head);
-  y -= s.h * head;
-  s.tile = sc.find(y);
-  const int64_t at = line.x - (y - sc.prefix(s.tile)), cost = sc.cost(s.tile);
-  if (at == line.x || at < (int64_t)(c - 1) * line.q) return;  // not the tile's first boundary
-  const int last = (int)((at + cost - 1) / line.q);
-  const int64_t row0 = (int64_t)s.tile * kRows;
-  const int nr = (int)min((int64_t)kRows, (int64_t)s.r.n * a.G - row0);
-  __shared__ int s_again;
-  if (threadIdx.x == 0) s_again = 0;
-  __syncthreads();
-  bool final = false;
-  for (int e = threadIdx.x; e < nr * D; e += blockDim.x) {
-    const int row = e / D, d = e % D;
-    float top = -INFINITY, sum = 0.f, x = 0.f;
-    for (int p = c - 1; p <= last; ++p) {
-      const int64_t from = (int64_t)p * line.q;
-      set_blocks(a, rule, cost, max(from - at, (int64_t)0), min(cost, from + line.q - at), s);
-      if (s.whole || s.nb == 0) final = true;
-      if (final) break;
-      if (s.blk0 >= s.blk1) continue;
-      const float* part = ws + ((int64_t)p * 2 + (from >= at ? 0 : 1)) * (kRows * (D + 2));
-      const float m = __ldcg(part + kRows * D + row), l = __ldcg(part + kRows * D + kRows + row);
-      const float mn = fmaxf(top, m);
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      const float f0 = ex2_approx(top - ref), f1 = ex2_approx(m - ref);
-      top = mn;
-      sum = sum * f0 + l * f1;
-      x = x * f0 + __ldcg(part + row * D + d) * f1;
+  constexpr int PART = kRows * (D + 2);
+  __shared__ int s_slot[kParts];
+  __shared__ float s_w[kParts][kRows];  // a part's weight in each row
+  __shared__ int s_whole, s_again;
+  if (threadIdx.x == 0) s_whole = s_again = 0;
+  Line line;
+  const Parts p = find_parts(a, rule, pieces, line);
+  if (p.n == 0) return;
+  const Segment& s = p.s;
+  const int row0 = s.tile * kRows, nr = min(kRows, s.r.n * a.G - row0);
+  float x[kRows * D / 128], top = -INFINITY, sum = 0.f;  // top, sum: of row threadIdx.x
+#pragma unroll
+  for (int i = 0; i < kRows * D / 128; ++i) x[i] = 0.f;
+  for (int i0 = 0; i0 < p.n; i0 += kParts) {
+    const int n = min(kParts, p.n - i0);
+    __syncthreads();
+    if (threadIdx.x < n) {
+      bool whole;
+      s_slot[threadIdx.x] = part_slot(a, rule, line, p, i0 + threadIdx.x, whole);
+      if (whole) s_whole = 1;
     }
-    if (final) break;
-    const float out = sum == 0.f ? 0.f : x / sum;
-    const int t = (int)((row0 + row) / a.G), hg = (int)((row0 + row) % a.G);
-    if (!(fabsf(out) <= 3.4028235e38f) && fabsf(sum) <= 3.4028235e38f &&
+    __syncthreads();
+    if (s_whole) return;  // written by the CTA that has all of it
+    // row r: maxima and sums of the parts so far
+    __shared__ float s_scale[kRows];
+    if (threadIdx.x < nr) {
+      const int r = threadIdx.x;
+      float mx = top;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float m = s_slot[i] < 0 ? -INFINITY : __ldcg(ws + (int64_t)s_slot[i] * PART + kRows * D + r);
+        s_w[i][r] = m;
+        mx = fmaxf(mx, m);
+      }
+      const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(top - ref);
+      sum *= old;
+      s_scale[r] = old;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float w = ex2_approx(s_w[i][r] - ref);
+        const float l = s_slot[i] < 0 ? 0.f : __ldcg(ws + (int64_t)s_slot[i] * PART + kRows * D + kRows + r);
+        s_w[i][r] = w;
+        sum = fmaf(l, w, sum);
+      }
+      top = mx;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRows * D / 128; ++k) {
+      const int e = k * 128 + threadIdx.x, row = e / D;
+      if (row >= nr) break;
+      float y = x[k] * s_scale[row];
+#pragma unroll 4
+      for (int i = 0; i < n; ++i)
+        if (s_slot[i] >= 0) y = fmaf(__ldcg(ws + (int64_t)s_slot[i] * PART + e), s_w[i][row], y);
+      x[k] = y;
+    }
+  }
+  __shared__ float s_sum[kRows];
+  if (threadIdx.x < nr) s_sum[threadIdx.x] = sum;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kRows * D / 128; ++k) {
+    const int e = k * 128 + threadIdx.x, row = e / D, d = e % D;
+    if (row >= nr) break;
+    const float l = s_sum[row], out = l == 0.f ? 0.f : x[k] / l;
+    const int t = (row0 + row) / a.G, hg = (row0 + row) % a.G;
+    if (!(fabsf(out) <= 3.4028235e38f) && fabsf(l) <= 3.4028235e38f &&
         visible_keys(s.r, t, a.causal) < s.kv_hi)
       atomicOr(&s_again, 1 << row);
     reinterpret_cast<T*>(a.o)[(int64_t)(s.r.begin + t) * a.os[0] +
@@ -451,7 +476,7 @@ __global__ void __launch_bounds__(128)
   const int rows = s_again;
   for (int row = threadIdx.x >> 5; row < nr && rows; row += 4) {
     if (!(rows >> row & 1)) continue;
-    const int t = (int)((row0 + row) / a.G), h = s.h * a.G + (int)((row0 + row) % a.G);
+    const int t = (row0 + row) / a.G, h = s.h * a.G + (row0 + row) % a.G;
     if (hidden_not_finite<DT>(a, s.b, s.h, visible_keys(s.r, t, a.causal), s.kv_hi))
       row_by_key<DT>(a, s.b, s.r, t, h);
   }

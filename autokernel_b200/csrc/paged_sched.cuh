@@ -17,7 +17,7 @@ namespace paged {
 struct TileRule {
   int rows;    // query rows (token, head of the group) per tile, when tiles are cut by rows; or 0
   int tokens;  // tokens per tile otherwise
-  int blk;     // keys per block
+  int shift;   // log2 of the keys per block
   int over;    // cost of a tile beside its keys, in keys
   int64_t min_piece;  // shortest piece of the line that a CTA gets
 };
@@ -49,7 +49,7 @@ AK_D SeqCost seq_cost(const AttnArgs& a, const TileRule& t, const SeqRange& r) {
   if (r.n == 0) return c;
   const int kv = min(r.kv_len, capacity(a.l));
   if (t.rows) {
-    c.tiles = (int)(((int64_t)r.n * a.G + t.rows - 1) / t.rows);
+    c.tiles = (r.n * a.G + t.rows - 1) / t.rows;  // (N G < 2^31)
     c.base = c.last = (int64_t)kv + t.over;
   } else {
     c.tiles = (r.n + t.tokens - 1) / t.tokens;
@@ -79,17 +79,17 @@ struct Segment {
 AK_D void set_blocks(const AttnArgs& a, const TileRule& t, int64_t cost, int64_t z0, int64_t z1,
                      Segment& s) {
   if (t.rows) {
-    const int64_t r0 = (int64_t)s.tile * t.rows, r1 = min(r0 + t.rows, (int64_t)s.r.n * a.G);
-    s.t_lo = (int)(r0 / a.G);
-    s.t_hi = (int)((r1 - 1) / a.G) + 1;
+    const int r0 = s.tile * t.rows, r1 = min(r0 + t.rows, s.r.n * a.G);  // (N G < 2^31)
+    s.t_lo = r0 / a.G;
+    s.t_hi = (r1 - 1) / a.G + 1;
   } else {
     s.t_lo = s.tile * t.tokens;
     s.t_hi = min(s.t_lo + t.tokens, s.r.n);
   }
   s.kv_hi = min(visible_keys(s.r, s.t_hi - 1, a.causal), capacity(a.l));
-  s.nb = (int)(((int64_t)s.kv_hi + t.blk - 1) / t.blk);
+  s.nb = (int)(((int64_t)s.kv_hi + (1 << t.shift) - 1) >> t.shift);
   auto block = [&](int64_t z) {
-    return z >= cost ? s.nb : (int)min((int64_t)s.nb, (z + t.blk / 2) / t.blk);
+    return z >= cost ? s.nb : (int)min((int64_t)s.nb, (z + (1 << t.shift) / 2) >> t.shift);
   };
   s.blk0 = block(z0);
   s.blk1 = block(z1);
@@ -105,56 +105,70 @@ struct Line {
   int64_t total;
 };
 
-// Run by the whole CTA.
+// Run by the whole CTA, whose threads each take one sequence at a time.
 AK_D Line find_piece(const AttnArgs& a, const TileRule& t, int pieces, int piece) {
-  __shared__ int64_t s_warp[32];
-  __shared__ int64_t s_at;
+  __shared__ int64_t s_warp[32], s_at;
   __shared__ int s_b;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = (blockDim.x + 31) >> 5;
-  auto cost_of = [&](int b) {
-    return b < a.l.B ? a.Hkv * seq_cost(a, t, seq_range(a.l, b)).total() : (int64_t)0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  auto cost_of = [&](int64_t b) {
+    return b < a.l.B ? a.Hkv * seq_cost(a, t, seq_range(a.l, (int)b)).total() : (int64_t)0;
   };
-  Line line;
-  int64_t mine = 0;
-  const int64_t first = cost_of(threadIdx.x);
-  mine = first;
-  for (int64_t b = (int64_t)threadIdx.x + blockDim.x; b < a.l.B; b += blockDim.x) mine += cost_of((int)b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) s_warp[warp] = mine;
-  if (threadIdx.x == 0) s_b = -1;
-  __syncthreads();
-  line.total = 0;
-  for (int i = 0; i < nw; ++i) line.total += s_warp[i];
-  line.q = max((line.total + pieces - 1) / pieces, t.min_piece);
-  line.x = (int64_t)piece * line.q;
-  if (line.x >= line.total) {
-    line.x = -1;
-    return line;
-  }
-  int64_t run = 0;
-  for (int64_t base = 0; base < a.l.B; base += blockDim.x) {
-    const int64_t v = base == 0 ? first : cost_of((int)min(base + threadIdx.x, (int64_t)a.l.B));
+  // sum of the values before this thread's, and of all
+  auto scan = [&](int64_t v, int64_t& all) {
     int64_t inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
     }
-    __syncthreads();
     if (lane == 31) s_warp[warp] = inc;
     __syncthreads();
-    int64_t at = run + inc - v;
-    for (int i = 0; i < nw; ++i) {
-      if (i < warp) at += s_warp[i];
-      run += s_warp[i];
+    int64_t part = lane < nw ? s_warp[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, part, o);
+      if (lane >= o) part += y;
     }
-    if (line.x >= at && line.x < at + v) {
+    all = __shfl_sync(0xffffffffu, part, 31);
+    const int64_t up_to = __shfl_sync(0xffffffffu, part, warp);
+    return up_to - __shfl_sync(0xffffffffu, inc, 31) + inc - v;
+  };
+  Line line;
+  const int64_t first = cost_of(threadIdx.x);
+  int64_t at = scan(first, line.total);  // all there is, up to as many sequences as threads
+  if (a.l.B > (int)blockDim.x) {
+    int64_t more = 0, all;
+    for (int64_t b = (int64_t)threadIdx.x + blockDim.x; b < a.l.B; b += blockDim.x) more += cost_of(b);
+    __syncthreads();
+    scan(more, all);
+    line.total += all;
+  }
+  line.q = max((line.total + pieces - 1) / pieces, t.min_piece);
+  line.x = (int64_t)piece * line.q;
+  if (line.x >= line.total) {
+    line.x = -1;
+    return line;
+  }
+  int64_t v = first, run = 0;
+  for (int64_t base = 0;; base += blockDim.x) {
+    if (base) {
+      int64_t all;
+      v = cost_of(base + threadIdx.x);
+      __syncthreads();
+      at = run + scan(v, all);
+      run += all;
+    } else if (a.l.B > (int)blockDim.x) {
+      run = __syncthreads_or(0);  // (all have read s_warp)
+      int64_t all;
+      at = scan(v, all);
+      run = all;
+    }
+    const bool mine = line.x >= at && line.x < at + v;
+    if (mine) {
       s_b = (int)(base + threadIdx.x);
       s_at = at;
     }
-    __syncthreads();
-    if (s_b >= 0) break;
+    if (__syncthreads_or(mine)) break;
   }
   line.b = s_b;
   line.b_at = s_at;
@@ -209,6 +223,50 @@ struct Walker {
     return false;
   }
 };
+
+// ------------------------------------------------------------------ joining a tile's parts
+
+// The parts of the tile that boundary blockIdx.x + 1 between two pieces cuts first, for a whole CTA.
+struct Parts {
+  Segment s;        // the tile
+  int n;            // parts there are: none if the boundary is not the tile's first, or one CTA had it all
+  int64_t at, cost;
+  int first;        // piece of part 0
+};
+constexpr int kParts = 32;  // parts looked at in one go
+
+AK_D Parts find_parts(const AttnArgs& a, const TileRule& t, int pieces, Line& line) {
+  Parts p;
+  p.n = 0;
+  const int c = blockIdx.x + 1;
+  line = find_piece(a, t, pieces, c);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // in every block, also one without a part
+  if (line.x < 0) return p;
+  p.s.b = line.b;
+  p.s.r = seq_range(a.l, line.b);
+  const SeqCost sc = seq_cost(a, t, p.s.r);
+  const int64_t head = sc.total();
+  int64_t y = line.x - line.b_at;
+  p.s.h = (int)(y / head);
+  y -= p.s.h * head;
+  p.s.tile = sc.find(y);
+  p.at = line.x - (y - sc.prefix(p.s.tile));
+  p.cost = sc.cost(p.s.tile);
+  if (p.at == line.x || p.at < (int64_t)(c - 1) * line.q) return p;  // not the tile's first boundary
+  set_blocks(a, t, p.cost, 0, p.cost, p.s);
+  p.first = c - 1;
+  if (p.s.nb) p.n = (int)((p.at + p.cost - 1) / line.q) - (c - 1) + 1;
+  return p;
+}
+
+// Workspace slot (2 * piece + which) of part i, or -1 when it holds no block; *whole when it holds all.
+AK_D int part_slot(const AttnArgs& a, const TileRule& t, const Line& line, const Parts& p, int i, bool& whole) {
+  Segment s = p.s;
+  const int64_t from = (int64_t)(p.first + i) * line.q;
+  set_blocks(a, t, p.cost, max(from - p.at, (int64_t)0), min(p.cost, from + line.q - p.at), s);
+  whole = s.whole;
+  return s.blk0 < s.blk1 ? 2 * (p.first + i) + (from >= p.at ? 0 : 1) : -1;
+}
 
 // Page numbers of consecutive boxes of a tile's keys, for a whole warp: 32 are loaded at once and the
 // next 32 while those are used (a load per block, used at once, bounded the producer: about 2000

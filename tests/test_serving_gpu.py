@@ -507,3 +507,20 @@ def test_sample_follows_the_distribution():
     got = torch.bincount(ops.sample(x.expand(n, 12), u, temperature=0.8), minlength=12).double() / n
     want = torch.softmax(x[0].double() / float(np.float32(0.8)), 0)
     assert (got - want).abs().max() <= 1.0 / n
+
+
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("B", [150, 700])
+def test_attention_many_sequences(B, new):
+    """More sequences than a block has threads, many of them empty."""
+    b = Batch("bf16", [(new if i % 3 else 0, (7 * i) % 90 + new) for i in range(B)], 1, 64, 16, seed=B)
+    q, o = attend(b, 2)
+    check_attention(b, q, o)
+
+
+@pytest.mark.parametrize("seqs", [[(1, 20000)], [(1, 20000), (1, 3)], [(40, 30000), (1, 5), (1, 700)]])
+def test_attention_one_long_sequence(seqs):
+    """One tile cut into more parts than the join looks at in one go."""
+    b = Batch("bf16", seqs, 1, 128, 64, seed=18)
+    q, o = attend(b, 2)
+    check_attention(b, q, o)
