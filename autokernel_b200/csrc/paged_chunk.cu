@@ -111,13 +111,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
-  const Line line = find_piece(a, p.rule, gridDim.x, blockIdx.x);
+  const Line line = find_piece(a, p.rule, blockIdx.x);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   volatile int* abort_p = &abort_flag;
-  Walker walk(a, p.rule, line);
+  Walker walk(a, p.rule, line, blockIdx.x);
   Segment s;
 
   if (warp == 0) {  // ------------------------------------------------------- TMA producer
@@ -437,8 +437,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 // rows per CTA and four threads along D.
 template <int DT, int D>
 __global__ void __launch_bounds__(128)
-    chunk_join_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Params p,
-                      int pieces) {
+    chunk_join_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Params p) {
   using C = Cfg<D>;
   using E = Elem<DT>;
   using T = typename E::T;
@@ -447,7 +446,8 @@ __global__ void __launch_bounds__(128)
   __shared__ int s_whole, s_again;
   if (threadIdx.x == 0) s_whole = s_again = 0;
   Line line;
-  const Parts parts = find_parts(a, p.rule, pieces, line);
+  const Parts parts = find_parts(a, p.rule, line);
+  wait_for_parts();
   if (parts.n == 0) return;
   const Segment& s = parts.s;
   const int lane = threadIdx.x & 31, part_d = threadIdx.x >> 5;
@@ -526,7 +526,7 @@ static int launch(const AttnArgs& a, float* ws, cudaStream_t st) {
   Params p{};
   p.tt = BQ / a.G;
   p.box = gcd_int(a.l.page_size, BKV);
-  p.rule = TileRule{0, 2 * p.tt, 7, 128, 512};
+  p.rule = TileRule{0, 2 * p.tt, 7, 128, 512, device_info().sm_count, 1};
   const int fmt = DT == AK_BF16 ? 1 : 0;
   p.idesc_qk = idesc_f16(fmt, BQ, BKV, false, false);
   p.idesc_pv = idesc_f16(fmt, BQ, D, false, true);
@@ -542,11 +542,11 @@ static int launch(const AttnArgs& a, float* ws, cudaStream_t st) {
   const cudaError_t attr = smem_optin<chunk_kernel<DT, D>>(Cfg<D>::SMEM);
   AK_REQUIRE(attr == cudaSuccess, AK_ERR_LAUNCH, "paged_attention smem attribute: %s",
              cudaGetErrorString(attr));
-  const int pieces = device_info().sm_count;
+  const int pieces = p.rule.ctas;
   chunk_kernel<DT, D><<<pieces, THREADS, Cfg<D>::SMEM, st>>>(tq, tk, tv, a, p);
   const int rc = launch_status("paged_attention");
   if (rc || pieces < 2) return rc;
-  return launch_after(chunk_join_kernel<DT, D>, dim3(pieces - 1, ROWS / 32), 128, st, a, p, pieces);
+  return launch_after(chunk_join_kernel<DT, D>, dim3(pieces - 1, ROWS / 32), 128, st, a, p);
 }
 
 }  // namespace chunk

@@ -39,7 +39,14 @@ struct DecodeCfg {
   static constexpr int SMEM = O_OFF + kWarps / 2 * kRows * D * 4 + 1024;
 };
 
-static TileRule decode_rule() { return TileRule{kRows, 0, 6, 64, 256}; }
+// Rounds of pieces where the tables could name a long line (paged_sched.cuh; a shorter one that turns
+// out is cut into single pieces, whose spare CTAs then only cost their cancellation).
+static TileRule decode_rule(const AttnArgs& a) {
+  const int ctas = device_info().sm_count;
+  const double tiles = (double)a.l.B + (double)a.l.N * a.G / kRows;
+  const double keys = tiles * a.Hkv * ((double)a.l.max_pages * a.l.page_size + 64);
+  return TileRule{kRows, 0, 6, 64, 256, ctas, keys / ctas >= 4 * kLongPiece && a.l.B <= 512 ? kRounds : 1};
+}
 
 static size_t decode_part_floats(int D) { return (size_t)kRows * (D + 2); }
 
@@ -109,10 +116,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int s_badw[kWarps];
   __shared__ int s_again;           // rows to look at again (bits)
   __shared__ int abort_flag, s_stop;
+  __shared__ __align__(16) uint4 s_next[4];  // answers to the requests for another piece
+  __shared__ uint64_t next_full[4], next_empty[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (rule.rounds == 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&next_full[i], 1);
+      mbar_init(&next_empty[i], kWarps + kProducers);
+    }
     for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(&full[i], kProducers);
       mbar_init(&empty[i], 4);
@@ -123,11 +136,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
   }
-  const Line line = find_piece(a, rule, gridDim.x, blockIdx.x);
+  int piece = blockIdx.x;
+  Line line = find_piece(a, rule, piece);
   __syncthreads();
   volatile int* abort_p = &abort_flag;
-  Walker walk(a, rule, line);
+  Walker walk(a, rule, line, piece);
   Segment s;
+  // Each warp comes here when it is done with a piece, the first producer first (it asks for the next
+  // one when its copies are under way); false when there is none.
+  int asked = 0;
+  auto next_piece = [&]() -> bool {
+    if (rule.rounds == 1 || piece < 0) return false;
+    while (true) {
+      const int slot = asked & 3, phase = (asked >> 2) & 1;
+      bool got = true;
+      if (warp == 0) {
+        got = mbar_wait(&next_empty[slot], phase ^ 1, abort_p);
+        if (lane == 0 && got) {
+          mbar_expect_tx(&next_full[slot], 16);
+          clc_try_cancel(&s_next[slot], &next_full[slot]);
+        }
+        __syncwarp();
+      }
+      if (got) got = mbar_wait(&next_full[slot], phase, abort_p);
+      if (!got && warp == 0 && lane == 0) drain_ring(next_full, 4, asked + 1);  // the answer still lands
+      piece = __all_sync(0xffffffffu, got) ? clc_answer(&s_next[slot]) : -1;
+      ++asked;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&next_empty[slot]);
+      if (piece < 0) break;
+      move_to_piece(a, rule, line, piece);
+      if (line.x >= 0) {
+        walk.go(line, piece);
+        return true;
+      }
+    }
+    // nothing is left to launch: the join may
+    if (warp == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    return false;
+  };
   int g = 0;  // ring slots used so far
 
   if (warp < kProducers) {  // ------------------------------------------- TMA producers
@@ -135,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const CUtensorMap* map = (warp & 1) ? &tv : &tk;
     const int i0 = warp >> 1, mine = (boxes - i0 + 1) / 2;  // boxes i0, i0 + 2, ...
     uint8_t* const dst = smem + ((warp & 1) ? C::HALF : 0);
-    while (walk.next(s)) {
+    do while (walk.next(s)) {
       PageFeed feed;
       if (s.blk0 < s.blk1) feed.start(a, s, s.blk0 * boxes, box);
       for (int blk = s.blk0; blk < s.blk1; ++blk, ++g) {
@@ -156,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (*abort_p) break;
-    }
+    } while (!*abort_p && next_piece());
     // giving up: the copies in flight still land in this CTA's shared memory
     if (*abort_p && lane == 0 && warp == 0) drain_ring(full, C::STAGES, g);
   } else {  // ---------------------------------------------------------------- consumers
@@ -170,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t vrow = row_at(k16 + (lane & 15));
     const int cap = capacity(a.l);
     bool ok = true;
-    while (ok && walk.next(s)) {
+    do while (ok && walk.next(s)) {
       const int row0 = s.tile * kRows;
       const int nr = min(kRows, s.r.n * a.G - row0);
       const T* qrow[2];
@@ -341,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) first_bad = min(first_bad, s_badw[w]);
       const bool again = a.causal && s.t_hi - s.t_lo > 1;  // rows of the tile hide keys from one another
-      float* part = ws + ((int64_t)blockIdx.x * 2 + s.slot) * (kRows * (D + 2));
+      float* part = ws + ((int64_t)piece * 2 + s.slot) * (kRows * (D + 2));
       for (int e = threadIdx.x - 32 * kProducers; e < nr * D; e += 32 * kWarps) {
         const int row = e / D, d = e % D;
         float top = s_m[0][row];
@@ -387,84 +435,82 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         group_sync();
       }
-    }
+    } while (ok && next_piece());
   }
 }
 
-// Joins the parts of the tile that boundary blockIdx.x + 1 cuts first.  The parts' maxima and sums
-// come first, all at once; then every output element is a sum of independent loads.
+// Joins the parts of the tile that boundary blockIdx.x + 1 cuts first, every output element from
+// independent loads.
 template <int DT, int D>
 __global__ void __launch_bounds__(128)
-    decode_join_kernel(const __grid_constant__ AttnArgs a, const TileRule rule, int pieces,
-                       const float* ws) {
+    decode_join_kernel(const __grid_constant__ AttnArgs a, const TileRule rule, const float* ws) {
   using E = Elem<DT>;
   using T = typename E::T;
-  constexpr int PART = kRows * (D + 2);
+  constexpr int PART = kRows * (D + 2), U = 6;
   __shared__ int s_slot[kParts];
-  __shared__ float s_w[kParts][kRows];  // a part's weight in each row
   __shared__ int s_whole, s_again;
   if (threadIdx.x == 0) s_whole = s_again = 0;
   Line line;
-  const Parts p = find_parts(a, rule, pieces, line);
-  if (p.n == 0) return;
-  const Segment& s = p.s;
-  const int row0 = s.tile * kRows, nr = min(kRows, s.r.n * a.G - row0);
-  float x[kRows * D / 128], top = -INFINITY, sum = 0.f;  // top, sum: of row threadIdx.x
-#pragma unroll
-  for (int i = 0; i < kRows * D / 128; ++i) x[i] = 0.f;
-  for (int i0 = 0; i0 < p.n; i0 += kParts) {
-    const int n = min(kParts, p.n - i0);
+  const Parts p = find_parts(a, rule, line);
+  auto slots = [&](int i0) {  // of parts i0 .. i0 + kParts - 1
     __syncthreads();
-    if (threadIdx.x < n) {
+    if (threadIdx.x < min(kParts, p.n - i0)) {
       bool whole;
       s_slot[threadIdx.x] = part_slot(a, rule, line, p, i0 + threadIdx.x, whole);
       if (whole) s_whole = 1;
     }
     __syncthreads();
-    if (s_whole) return;  // written by the CTA that has all of it
-    // row r: maxima and sums of the parts so far
-    __shared__ float s_scale[kRows];
-    if (threadIdx.x < nr) {
-      const int r = threadIdx.x;
-      float mx = top;
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float m = s_slot[i] < 0 ? -INFINITY : __ldcg(ws + (int64_t)s_slot[i] * PART + kRows * D + r);
-        s_w[i][r] = m;
-        mx = fmaxf(mx, m);
-      }
-      const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(top - ref);
-      sum *= old;
-      s_scale[r] = old;
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float w = ex2_approx(s_w[i][r] - ref);
-        const float l = s_slot[i] < 0 ? 0.f : __ldcg(ws + (int64_t)s_slot[i] * PART + kRows * D + kRows + r);
-        s_w[i][r] = w;
-        sum = fmaf(l, w, sum);
-      }
-      top = mx;
-    }
-    __syncthreads();
+  };
+  if (p.n) slots(0);
+  wait_for_parts();
+  if (p.n == 0) return;
+  const Segment& s = p.s;
+  const int row0 = s.tile * kRows, nr = min(kRows, s.r.n * a.G - row0);
+  constexpr int K = kRows * D / 128;  // elements of this thread
+  float x[K], top[K], sum[K];
 #pragma unroll
-    for (int k = 0; k < kRows * D / 128; ++k) {
+  for (int k = 0; k < K; ++k) {
+    x[k] = sum[k] = 0.f;
+    top[k] = -INFINITY;
+  }
+  for (int i0 = 0; i0 < p.n; i0 += kParts) {
+    const int n = min(kParts, p.n - i0);
+    if (i0) slots(i0);
+    if (s_whole) return;  // written by the CTA that has all of it
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
       const int e = k * 128 + threadIdx.x, row = e / D;
       if (row >= nr) break;
-      float y = x[k] * s_scale[row];
-#pragma unroll 4
-      for (int i = 0; i < n; ++i)
-        if (s_slot[i] >= 0) y = fmaf(__ldcg(ws + (int64_t)s_slot[i] * PART + e), s_w[i][row], y);
-      x[k] = y;
+      for (int i = 0; i < n; i += U) {
+        float m[U], l[U], y[U], mx = top[k];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {  // all loads first
+          const bool in = i + u < n && s_slot[i + u] >= 0;
+          const float* part = ws + (int64_t)(in ? s_slot[i + u] : 0) * PART;
+          m[u] = in ? __ldcg(part + kRows * D + row) : -INFINITY;
+          l[u] = in ? __ldcg(part + kRows * D + kRows + row) : 0.f;
+          y[u] = in ? __ldcg(part + e) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) mx = fmaxf(mx, m[u]);
+        const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(top[k] - ref);
+        x[k] *= old;
+        sum[k] *= old;
+        top[k] = mx;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float w = ex2_approx(m[u] - ref);
+          x[k] = fmaf(y[u], w, x[k]);
+          sum[k] = fmaf(l[u], w, sum[k]);
+        }
+      }
     }
   }
-  __shared__ float s_sum[kRows];
-  if (threadIdx.x < nr) s_sum[threadIdx.x] = sum;
-  __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kRows * D / 128; ++k) {
+  for (int k = 0; k < K; ++k) {
     const int e = k * 128 + threadIdx.x, row = e / D, d = e % D;
     if (row >= nr) break;
-    const float l = s_sum[row], out = l == 0.f ? 0.f : x[k] / l;
+    const float l = sum[k], out = l == 0.f ? 0.f : x[k] / l;
     const int t = (row0 + row) / a.G, hg = (row0 + row) % a.G;
     if (!(fabsf(out) <= 3.4028235e38f) && fabsf(l) <= 3.4028235e38f &&
         visible_keys(s.r, t, a.causal) < s.kv_hi)
@@ -491,17 +537,16 @@ static int launch_decode(const AttnArgs& a, float* ws, cudaStream_t st) {
   const cudaError_t attr = smem_optin<decode_kernel<DT, D>>(DecodeCfg<D>::SMEM);
   AK_REQUIRE(attr == cudaSuccess, AK_ERR_LAUNCH, "paged_attention smem attribute: %s",
              cudaGetErrorString(attr));
-  const int pieces = device_info().sm_count;
-  const TileRule rule = decode_rule();
+  const TileRule rule = decode_rule(a);
+  const int pieces = rule.ctas * rule.rounds;
   decode_kernel<DT, D><<<pieces, kThreads, DecodeCfg<D>::SMEM, st>>>(tk, tv, a, rule, box, ws);
   const int rc = launch_status("paged_attention");
   if (rc || pieces < 2) return rc;
-  return launch_after(decode_join_kernel<DT, D>, dim3(pieces - 1), 128, st, a, rule, pieces,
-                      (const float*)ws);
+  return launch_after(decode_join_kernel<DT, D>, dim3(pieces - 1), 128, st, a, rule, (const float*)ws);
 }
 
 size_t decode_workspace(int D) {
-  return 2 * (size_t)device_info().sm_count * decode_part_floats(D) * sizeof(float);
+  return 2 * (size_t)device_info().sm_count * kRounds * decode_part_floats(D) * sizeof(float);
 }
 
 int run_decode(const AttnArgs& a, void* ws, cudaStream_t st) {

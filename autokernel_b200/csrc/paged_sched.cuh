@@ -4,9 +4,15 @@
 // tiles are laid end to end on one line (sequence, head, tile), each as long as its keys plus a
 // constant for its prologue and epilogue, and the line is cut into one equal piece per CTA: every
 // SM gets the same number of keys whatever the lengths are, and no host code has to know them.  A
-// piece may end inside a tile.  Such a tile's parts go to the workspace, at most two per CTA (its
+// piece may end inside a tile.  Such a tile's parts go to the workspace, at most two per piece (its
 // first and its last segment), and a second kernel joins them in the line's order, so results do
 // not depend on timing.
+//
+// Equal pieces do not take equal time when memory is the bound: decoding 64 sequences of up to 8K
+// keys, the first of 148 CTAs was done after 164 us and the last after 215.  Long lines are
+// therefore cut into five rounds of pieces, 46, 8, 5, 3 and 2 64ths of an equal share, and a CTA
+// that is done takes the next piece that has not begun (the hardware's cancellation of a CTA that
+// waits to be launched hands its number over).
 #pragma once
 #include "paged_attn.cuh"
 
@@ -20,6 +26,8 @@ struct TileRule {
   int shift;   // log2 of the keys per block
   int over;    // cost of a tile beside its keys, in keys
   int64_t min_piece;  // shortest piece of the line that a CTA gets
+  int ctas;           // CTAs that run at once
+  int rounds;         // kRounds: a long line may be cut into rounds of pieces; or 1
 };
 
 // A sequence on the line: tile i of a head is base + slope * (i + 1) long, the last one `last`.
@@ -96,23 +104,78 @@ AK_D void set_blocks(const AttnArgs& a, const TileRule& t, int64_t cost, int64_t
   s.whole = s.blk0 == 0 && s.blk1 == s.nb;
 }
 
-// The line and the piece of it that starts at `piece` (in units of q).
+// How a line is cut into pieces.
+constexpr int kRounds = 5;
+constexpr int64_t kLongPiece = 4096;  // shortest equal share that is worth rounds
+struct Cut {
+  int64_t unit;  // a piece of round r is size(r) units long
+  int ctas;
+  bool rounds;
+  // 46, 8, 5, 3, 2 of 64
+  AK_D static int size(int r) { return r == 0 ? 46 : r == 1 ? 8 : r == 2 ? 5 : r == 3 ? 3 : 2; }
+  AK_D static int before(int r) { return r == 0 ? 0 : r == 1 ? 46 : r == 2 ? 54 : r == 3 ? 59 : r == 4 ? 62 : 64; }
+  AK_D int64_t start(int piece) const {
+    if (!rounds) return piece * unit;
+    const int r = piece / ctas;
+    return ((int64_t)ctas * before(r) + (int64_t)(piece - r * ctas) * size(r)) * unit;
+  }
+  AK_D int holds(int64_t x) const {  // the piece that holds point x
+    const int64_t y = x / unit;
+    if (!rounds) return (int)y;
+    int r = 0;
+    while (r < kRounds - 1 && y >= (int64_t)ctas * before(r + 1)) ++r;
+    return r * ctas + (int)((y - (int64_t)ctas * before(r)) / size(r));
+  }
+};
+
+// The line, how it is cut, and one of its pieces.
 struct Line {
-  int64_t q;      // length of a piece
+  Cut cut;
+  int64_t total;
   int64_t x;      // the piece's start, or -1: there is no such piece
   int b;          // sequence that holds x
   int64_t b_at;   // where that sequence starts
-  int64_t total;
 };
 
+AK_D int64_t line_cost(const AttnArgs& a, const TileRule& t, int64_t b) {
+  return b < a.l.B ? a.Hkv * seq_cost(a, t, seq_range(a.l, (int)b)).total() : (int64_t)0;
+}
+
+// Another piece, for a whole warp: 32 sequences at a time.
+AK_D void move_to_piece(const AttnArgs& a, const TileRule& t, Line& line, int piece) {
+  const int lane = threadIdx.x & 31;
+  line.x = line.cut.start(piece);
+  if (line.x >= line.total) {
+    line.x = -1;
+    return;
+  }
+  int64_t run = 0;
+  for (int64_t base = 0; base < a.l.B; base += 32) {
+    const int64_t v = line_cost(a, t, base + lane);
+    int64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    const int64_t at = run + inc - v;
+    const unsigned hit = __ballot_sync(0xffffffffu, line.x >= at && line.x < at + v);
+    if (hit) {
+      line.b = (int)base + __ffs(hit) - 1;
+      line.b_at = __shfl_sync(0xffffffffu, at, __ffs(hit) - 1);
+      return;
+    }
+    run += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  line.x = -1;
+}
+
 // Run by the whole CTA, whose threads each take one sequence at a time.
-AK_D Line find_piece(const AttnArgs& a, const TileRule& t, int pieces, int piece) {
+AK_D Line find_piece(const AttnArgs& a, const TileRule& t, int piece) {
   __shared__ int64_t s_warp[32], s_at;
   __shared__ int s_b;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  auto cost_of = [&](int64_t b) {
-    return b < a.l.B ? a.Hkv * seq_cost(a, t, seq_range(a.l, (int)b)).total() : (int64_t)0;
-  };
+  auto cost_of = [&](int64_t b) { return line_cost(a, t, b); };
   // sum of the values before this thread's, and of all
   auto scan = [&](int64_t v, int64_t& all) {
     int64_t inc = v;
@@ -143,8 +206,11 @@ AK_D Line find_piece(const AttnArgs& a, const TileRule& t, int pieces, int piece
     scan(more, all);
     line.total += all;
   }
-  line.q = max((line.total + pieces - 1) / pieces, t.min_piece);
-  line.x = (int64_t)piece * line.q;
+  line.cut.ctas = t.ctas;
+  line.cut.unit = max((line.total + t.ctas - 1) / t.ctas, t.min_piece);
+  line.cut.rounds = t.rounds > 1 && line.cut.unit >= kLongPiece;
+  if (line.cut.rounds) line.cut.unit = (line.cut.unit + 63) / 64;
+  line.x = line.cut.start(piece);
   if (line.x >= line.total) {
     line.x = -1;
     return line;
@@ -185,10 +251,16 @@ struct Walker {
   SeqCost c;
   int64_t head;  // length of one head of sequence b
 
-  AK_D Walker(const AttnArgs& a_, const TileRule& t_, const Line& line)
-      : a(a_), t(t_), x(line.x), start(line.x), end(min(line.x + line.q, line.total)),
-        b_at(line.b_at), b(line.b), loaded(-1), head(0) {
-    if (line.x < 0) end = x;
+  AK_D Walker(const AttnArgs& a_, const TileRule& t_, const Line& line, int piece)
+      : a(a_), t(t_), head(0) {
+    go(line, piece);
+  }
+  AK_D void go(const Line& line, int piece) {
+    x = start = line.x;
+    end = line.x < 0 ? x : min(line.cut.start(piece + 1), line.total);
+    b_at = line.b_at;
+    b = line.b;
+    loaded = -1;
   }
   AK_D bool next(Segment& s) {
     while (x < end) {
@@ -226,6 +298,10 @@ struct Walker {
 
 // ------------------------------------------------------------------ joining a tile's parts
 
+// The predecessor on the stream has written its parts: every block of a join waits, also one that
+// has nothing to join.
+AK_D void wait_for_parts() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // The parts of the tile that boundary blockIdx.x + 1 between two pieces cuts first, for a whole CTA.
 struct Parts {
   Segment s;        // the tile
@@ -235,12 +311,11 @@ struct Parts {
 };
 constexpr int kParts = 32;  // parts looked at in one go
 
-AK_D Parts find_parts(const AttnArgs& a, const TileRule& t, int pieces, Line& line) {
+AK_D Parts find_parts(const AttnArgs& a, const TileRule& t, Line& line) {
   Parts p;
   p.n = 0;
   const int c = blockIdx.x + 1;
-  line = find_piece(a, t, pieces, c);
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // in every block, also one without a part
+  line = find_piece(a, t, c);
   if (line.x < 0) return p;
   p.s.b = line.b;
   p.s.r = seq_range(a.l, line.b);
@@ -252,18 +327,18 @@ AK_D Parts find_parts(const AttnArgs& a, const TileRule& t, int pieces, Line& li
   p.s.tile = sc.find(y);
   p.at = line.x - (y - sc.prefix(p.s.tile));
   p.cost = sc.cost(p.s.tile);
-  if (p.at == line.x || p.at < (int64_t)(c - 1) * line.q) return p;  // not the tile's first boundary
+  if (p.at == line.x || p.at < line.cut.start(c - 1)) return p;  // not the tile's first boundary
   set_blocks(a, t, p.cost, 0, p.cost, p.s);
   p.first = c - 1;
-  if (p.s.nb) p.n = (int)((p.at + p.cost - 1) / line.q) - (c - 1) + 1;
+  if (p.s.nb) p.n = line.cut.holds(p.at + p.cost - 1) - (c - 1) + 1;
   return p;
 }
 
 // Workspace slot (2 * piece + which) of part i, or -1 when it holds no block; *whole when it holds all.
 AK_D int part_slot(const AttnArgs& a, const TileRule& t, const Line& line, const Parts& p, int i, bool& whole) {
   Segment s = p.s;
-  const int64_t from = (int64_t)(p.first + i) * line.q;
-  set_blocks(a, t, p.cost, max(from - p.at, (int64_t)0), min(p.cost, from + line.q - p.at), s);
+  const int64_t from = line.cut.start(p.first + i), to = line.cut.start(p.first + i + 1);
+  set_blocks(a, t, p.cost, max(from - p.at, (int64_t)0), min(p.cost, to - p.at), s);
   whole = s.whole;
   return s.blk0 < s.blk1 ? 2 * (p.first + i) + (from >= p.at ? 0 : 1) : -1;
 }

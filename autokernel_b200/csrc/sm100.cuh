@@ -121,6 +121,30 @@ AK_D void tma_load_5d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, in
       : "memory");
 }
 
+// Asks for the cancellation of a CTA of this grid that has not been launched; the answer (16 bytes)
+// lands in `resp`, counted on `bar`.  Not to be asked again after an answer of "none".
+AK_D void clc_try_cancel(uint4* resp, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_u32(resp)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// The x index of the cancelled CTA, or -1 for none.
+AK_D int clc_answer(const uint4* resp) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, h;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(resp))
+      : "memory");
+  return ok ? (int)x : -1;
+}
+
 // ------------------------------------------------------------------ UMMA descriptors
 AK_D uint64_t desc_sw128(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
   uint64_t d = 0;

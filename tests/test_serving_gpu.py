@@ -524,3 +524,23 @@ def test_attention_one_long_sequence(seqs):
     b = Batch("bf16", seqs, 1, 128, 64, seed=18)
     q, o = attend(b, 2)
     check_attention(b, q, o)
+
+
+@pytest.mark.parametrize("D,dt", [(64, "f16"), (128, "bf16")])
+def test_attention_decode_long_line(D, dt):
+    """Enough keys that CTAs take further pieces of the line when they are done."""
+    b = Batch(dt, [(1, 40000), (1, 7), (1, 45000), (0, 0), (1, 300)], 8, D, 64, seed=19)
+    q, o = attend(b, 16)
+    check_attention(b, q, o)
+    for _ in range(5):
+        assert torch.equal(attend(b, 16, q=q)[1], o)
+
+
+def test_attention_decode_wide_table():
+    """A table that could name far more keys than there are."""
+    b = Batch("bf16", [(1, 100), (1, 2000), (1, 1)], 4, 64, 16, seed=20, stale=float("nan"))
+    wide = torch.full((3, 60000), -1, dtype=torch.int32, device=DEV)
+    wide[:, :b.table.shape[1]] = b.table
+    b.table = wide
+    q, o = attend(b, 8)
+    check_attention(b, q, o)
