@@ -150,10 +150,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int live = s.kv_hi - blk * BKV;
         const bool tail = live < BKV && live % p.box != 0;
         uint64_t* v_bar = tail ? &v_land : &v_full[st];
-        int bad = 0x7fffffff;
+        const int bad = feed.missing(a.l, blk * boxes, boxes);
         for (int i = 0; i < boxes; ++i) {
           int page, slot;
-          feed.get(a.l, blk * boxes + i, page, slot, bad);
+          feed.get(a.l, blk * boxes + i, page, slot);
           if (lane == 0) {
             uint8_t* dst = smem + st * C::TILE_BYTES + i * p.box * 128;
 #pragma unroll

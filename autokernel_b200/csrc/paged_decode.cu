@@ -53,14 +53,12 @@ static size_t decode_part_floats(int D) { return (size_t)kRows * (D + 2); }
 template <int DT>
 AK_D void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   if constexpr (DT == AK_BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -116,15 +114,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int s_badw[kWarps];
   __shared__ int s_again;           // rows to look at again (bits)
   __shared__ int abort_flag, s_stop;
-  __shared__ __align__(16) uint4 s_next[4];  // answers to the requests for another piece
-  __shared__ uint64_t next_full[4], next_empty[4];
+  // Segments, from the first producer to all other warps: finding one takes about 1000 cycles, so it is
+  // done once and ahead of time.  part < 0: there are no more.
+  struct Posted {
+    Segment s;
+    int part;  // workspace slot of its part
+  };
+  constexpr int POSTS = 4;
+  __shared__ Posted s_post[POSTS];
+  __shared__ uint64_t post_full[POSTS], post_empty[POSTS], next_full;
+  __shared__ __align__(16) uint4 s_next;  // answer to the request for another piece
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (rule.rounds == 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&next_full[i], 1);
-      mbar_init(&next_empty[i], kWarps + kProducers);
+    mbar_init(&next_full, 1);
+    for (int i = 0; i < POSTS; ++i) {
+      mbar_init(&post_full[i], 1);
+      mbar_init(&post_empty[i], kWarps + kProducers - 1);
     }
     for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(&full[i], kProducers);
@@ -136,66 +143,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
   }
-  int piece = blockIdx.x;
-  Line line = find_piece(a, rule, piece);
+  Line line = find_piece(a, rule, blockIdx.x);
   __syncthreads();
   volatile int* abort_p = &abort_flag;
-  Walker walk(a, rule, line, piece);
-  Segment s;
-  // Each warp comes here when it is done with a piece, the first producer first (it asks for the next
-  // one when its copies are under way); false when there is none.
-  int asked = 0;
-  auto next_piece = [&]() -> bool {
-    if (rule.rounds == 1 || piece < 0) return false;
-    while (true) {
-      const int slot = asked & 3, phase = (asked >> 2) & 1;
-      bool got = true;
-      if (warp == 0) {
-        got = mbar_wait(&next_empty[slot], phase ^ 1, abort_p);
-        if (lane == 0 && got) {
-          mbar_expect_tx(&next_full[slot], 16);
-          clc_try_cancel(&s_next[slot], &next_full[slot]);
-        }
-        __syncwarp();
-      }
-      if (got) got = mbar_wait(&next_full[slot], phase, abort_p);
-      if (!got && warp == 0 && lane == 0) drain_ring(next_full, 4, asked + 1);  // the answer still lands
-      piece = __all_sync(0xffffffffu, got) ? clc_answer(&s_next[slot]) : -1;
-      ++asked;
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&next_empty[slot]);
-      if (piece < 0) break;
-      move_to_piece(a, rule, line, piece);
-      if (line.x >= 0) {
-        walk.go(line, piece);
-        return true;
-      }
-    }
-    // nothing is left to launch: the join may
-    if (warp == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    return false;
-  };
   int g = 0;  // ring slots used so far
+  // the n-th segment: null when there is none (or another warp gave up); free it when done with it
+  auto segment = [&](int n) -> const Posted* {
+    const bool got = mbar_wait(&post_full[n % POSTS], (n / POSTS) & 1, abort_p);
+    return __all_sync(0xffffffffu, got) && s_post[n % POSTS].part >= 0 ? &s_post[n % POSTS] : nullptr;
+  };
+  auto release = [&](int n) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&post_empty[n % POSTS]);
+  };
 
   if (warp < kProducers) {  // ------------------------------------------- TMA producers
     const int boxes = kBlk / box;
     const CUtensorMap* map = (warp & 1) ? &tv : &tk;
     const int i0 = warp >> 1, mine = (boxes - i0 + 1) / 2;  // boxes i0, i0 + 2, ...
     uint8_t* const dst = smem + ((warp & 1) ? C::HALF : 0);
-    do while (walk.next(s)) {
+    auto load = [&](const Segment& s) {
       PageFeed feed;
       if (s.blk0 < s.blk1) feed.start(a, s, s.blk0 * boxes, box);
       for (int blk = s.blk0; blk < s.blk1; ++blk, ++g) {
         const int st = g % C::STAGES;
         feed.reach(a, s, blk * boxes, box);
         const bool ok = mbar_wait(&empty[st], ((g / C::STAGES) & 1) ^ 1, abort_p);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        int bad = 0x7fffffff;
-        for (int i = 0; i < boxes; ++i) {
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        const int bad = warp == 0 ? feed.missing(a.l, blk * boxes, boxes) : 0;
+        for (int i = i0; i < boxes; i += 2) {
           int page, slot;
-          feed.get(a.l, blk * boxes + i, page, slot, bad);
-          if (lane == 0 && (i & 1) == i0)
+          feed.get(a.l, blk * boxes + i, page, slot);
+          if (lane == 0)
             tma_load_5d(dst + st * C::STAGE + i * (C::NC * box * 128), map, &full[st], 0, slot, 0, s.h, page);
         }
         if (lane == 0) {  // the phase cannot end before these arrivals, so `bad` is there with the data
@@ -203,10 +182,57 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (mine) mbar_expect_tx(&full[st], mine * C::NC * box * 128); else mbar_arrive(&full[st]);
         }
       }
-      if (*abort_p) break;
-    } while (!*abort_p && next_piece());
-    // giving up: the copies in flight still land in this CTA's shared memory
-    if (*abort_p && lane == 0 && warp == 0) drain_ring(full, C::STAGES, g);
+      return true;
+    };
+    if (warp == 0) {  // walks the line, posts its segments and asks for further pieces
+      int piece = blockIdx.x, posted = 0, asked = 0;
+      Walker walk(a, rule, line, piece);
+      Segment s;
+      auto post = [&](int part) {
+        const bool ok = mbar_wait(&post_empty[posted % POSTS], ((posted / POSTS) & 1) ^ 1, abort_p);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        if (lane == 0) {
+          s_post[posted % POSTS].s = s;
+          s_post[posted % POSTS].part = part;
+          mbar_arrive(&post_full[posted % POSTS]);
+        }
+        __syncwarp();
+        ++posted;
+        return true;
+      };
+      bool ok = true;
+      while (ok) {
+        while (ok && walk.next(s)) ok = post(2 * piece + s.slot) && load(s);
+        if (!ok || rule.rounds == 1) break;
+        if (lane == 0) {
+          mbar_expect_tx(&next_full, 16);
+          clc_try_cancel(&s_next, &next_full);
+        }
+        ok = mbar_wait(&next_full, asked++ & 1, abort_p);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {  // giving up: the answer still lands
+          if (lane == 0) drain_ring(&next_full, 1, asked);
+          break;
+        }
+        piece = clc_answer(&s_next);
+        fence_proxy_async();
+        __syncwarp();
+        if (piece < 0) break;
+        move_to_piece(a, rule, line, piece);
+        walk.go(line, piece);
+      }
+      if (ok) post(-1);
+      // nothing is left to launch: the join may
+      if (rule.rounds > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+      // giving up: the copies in flight still land in this CTA's shared memory
+      if (*abort_p && lane == 0) drain_ring(full, C::STAGES, g);
+    } else {
+      for (int n = 0;; ++n) {
+        const Posted* p = segment(n);
+        if (!p || !load(p->s)) break;
+        release(n);
+      }
+    }
   } else {  // ---------------------------------------------------------------- consumers
     const int cw = warp - kProducers, grp = cw >> 2, k16 = (cw & 3) * 16;  // the warp's keys of its blocks
     const int r0 = lane >> 2, cq = 2 * (lane & 3);
@@ -217,12 +243,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t krow[2] = {row_at(k16 + (lane & 7)), row_at(k16 + 8 + (lane & 7))};
     const uint32_t vrow = row_at(k16 + (lane & 15));
     const int cap = capacity(a.l);
-    bool ok = true;
-    do while (ok && walk.next(s)) {
-      const int row0 = s.tile * kRows;
-      const int nr = min(kRows, s.r.n * a.G - row0);
+    uint32_t q[D / 16][4];
+    int vis[2];
+    // this lane's part of a segment's queries and what its two rows see
+    auto load_q = [&](const Segment& s) {
+      const int row0 = s.tile * kRows, nr = min(kRows, s.r.n * a.G - row0);
       const T* qrow[2];
-      int vis[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int rr = min(r0 + 8 * i, nr - 1);
@@ -231,12 +257,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                   (int64_t)(s.h * a.G + hg) * a.qs[1];
         vis[i] = visible_keys(s.r, t, a.causal);
       }
-      uint32_t q[D / 16][4];
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           q[kk][i] = __ldg(reinterpret_cast<const unsigned int*>(qrow[i & 1] + kk * 16 + cq + (i >> 1) * 8));
+    };
+    bool ok = true;
+    const Posted* now = segment(0);
+    if (now) load_q(now->s);
+    for (int n_seg = 0; ok && now; ++n_seg) {
+      const Segment& s = now->s;
+      const int row0 = s.tile * kRows;
+      const int nr = min(kRows, s.r.n * a.G - row0);
       float o[NF][4];
 #pragma unroll
       for (int i = 0; i < NF; ++i)
@@ -246,10 +279,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       int bad = cap;
       // every row of the tile sees keys below this
       const int vis_all = visible_keys(s.r, s.t_lo, a.causal);
-      for (int blk = s.blk0; blk < s.blk1; ++blk, ++g) {
-        if ((g & 1) != grp) continue;
-        const int st = g % C::STAGES;
-        const bool got = mbar_wait(&full[st], (g / C::STAGES) & 1, abort_p);
+      const int blk0 = s.blk0, blk1 = s.blk1, kv_hi = s.kv_hi;
+      for (int blk = blk0 + ((g & 1) != grp); blk < blk1; blk += 2) {
+        const int at = g + blk - blk0, st = at % C::STAGES;
+        const bool got = mbar_wait(&full[st], (at / C::STAGES) & 1, abort_p);
         if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
         bad = min(bad, s_bad[st]);
         const uint32_t kbase = ring + st * C::STAGE, vbase = kbase + C::HALF;
@@ -257,11 +290,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         // S = Q K^T for 16 keys
         float sc[2][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int kk = 0; kk < D / 32; ++kk) {  // 32 dims a load
-            const int unit = (kk & 1) * 4 + (lane >> 3);
+          for (int j = 0; j < 4; ++j) sc[n][j] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk) {  // 32 dims a load
+          const int unit = (kk & 1) * 4 + (lane >> 3);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
             uint32_t kf[4];
             ldmatrix4(kf, kbase + krow[n] + (kk >> 1) * chunk + ((unit ^ (lane & 7)) << 4));
             mma16816<DT>(sc[n], q[2 * kk], kf[0], kf[1]);
@@ -319,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int k = key0 + 8 * i + cq;
-          mask[i] = k + 1 < s.kv_hi ? 0xffffffffu : k < s.kv_hi ? 0x0000ffffu : 0u;
+          mask[i] = k + 1 < kv_hi ? 0xffffffffu : k < kv_hi ? 0x0000ffffu : 0u;
         }
 #pragma unroll
         for (int n = 0; n < NF / 2; ++n) {  // 16 dims a load
@@ -338,6 +374,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
       }
+      g += blk1 - blk0;
+      // the next segment's queries are on their way while this one is put together
+      const Posted* next = segment(n_seg + 1);
+      if (next) load_q(next->s);
       // join the eight warps: the second group's into the first's registers, then those four
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -389,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) first_bad = min(first_bad, s_badw[w]);
       const bool again = a.causal && s.t_hi - s.t_lo > 1;  // rows of the tile hide keys from one another
-      float* part = ws + ((int64_t)piece * 2 + s.slot) * (kRows * (D + 2));
+      float* part = ws + (int64_t)now->part * (kRows * (D + 2));
       for (int e = threadIdx.x - 32 * kProducers; e < nr * D; e += 32 * kWarps) {
         const int row = e / D, d = e % D;
         float top = s_m[0][row];
@@ -435,7 +475,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         group_sync();
       }
-    } while (ok && next_piece());
+      release(n_seg);
+      now = next;
+    }
   }
 }
 
@@ -466,23 +508,17 @@ __global__ void __launch_bounds__(128)
   if (p.n == 0) return;
   const Segment& s = p.s;
   const int row0 = s.tile * kRows, nr = min(kRows, s.r.n * a.G - row0);
-  constexpr int K = kRows * D / 128;  // elements of this thread
-  float x[K], top[K], sum[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    x[k] = sum[k] = 0.f;
-    top[k] = -INFINITY;
-  }
-  for (int i0 = 0; i0 < p.n; i0 += kParts) {
-    const int n = min(kParts, p.n - i0);
-    if (i0) slots(i0);
-    if (s_whole) return;  // written by the CTA that has all of it
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int e = k * 128 + threadIdx.x, row = e / D;
-      if (row >= nr) break;
+  if (s_whole) return;  // written by the CTA that has all of it
+#pragma unroll 1
+  for (int at = 0; at < nr * D; at += 128) {
+    const int e = at + threadIdx.x, row = e / D, d = e % D;
+    float x = 0.f, sum = 0.f, top = -INFINITY;
+    for (int i0 = 0; i0 < p.n; i0 += kParts) {
+      const int n = min(kParts, p.n - i0);
+      if (p.n > kParts) slots(i0);
+      if (row >= nr) continue;
       for (int i = 0; i < n; i += U) {
-        float m[U], l[U], y[U], mx = top[k];
+        float m[U], l[U], y[U], mx = top;
 #pragma unroll
         for (int u = 0; u < U; ++u) {  // all loads first
           const bool in = i + u < n && s_slot[i + u] >= 0;
@@ -493,24 +529,20 @@ __global__ void __launch_bounds__(128)
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) mx = fmaxf(mx, m[u]);
-        const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(top[k] - ref);
-        x[k] *= old;
-        sum[k] *= old;
-        top[k] = mx;
+        const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(top - ref);
+        x *= old;
+        sum *= old;
+        top = mx;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const float w = ex2_approx(m[u] - ref);
-          x[k] = fmaf(y[u], w, x[k]);
-          sum[k] = fmaf(l[u], w, sum[k]);
+          x = fmaf(y[u], w, x);
+          sum = fmaf(l[u], w, sum);
         }
       }
     }
-  }
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int e = k * 128 + threadIdx.x, row = e / D, d = e % D;
     if (row >= nr) break;
-    const float l = sum[k], out = l == 0.f ? 0.f : x[k] / l;
+    const float l = sum, out = l == 0.f ? 0.f : x / l;
     const int t = (row0 + row) / a.G, hg = (row0 + row) % a.G;
     if (!(fabsf(out) <= 3.4028235e38f) && fabsf(l) <= 3.4028235e38f &&
         visible_keys(s.r, t, a.causal) < s.kv_hi)

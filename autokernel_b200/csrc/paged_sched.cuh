@@ -376,13 +376,17 @@ struct PageFeed {
     key = next_key;
     fetch(a, s, base + 32, box, next_raw, next_slot, next_key);
   }
-  // page and slot of box i: a page that does not exist (and slot 0) where the key has none, its key
-  // then in `bad` if the tile needs it
-  AK_D void get(const PagedLists& l, int i, int& page, int& slot_, int& bad) const {
+  // page and slot of box i: a page that does not exist (and slot 0) where the key has none
+  AK_D void get(const PagedLists& l, int i, int& page, int& slot_) const {
     const bool ok = (unsigned)raw < (unsigned)l.num_pages;
     page = __shfl_sync(0xffffffffu, ok ? raw : l.num_pages, i - base);
     slot_ = __shfl_sync(0xffffffffu, ok ? slot : 0, i - base);
-    bad = min(bad, __shfl_sync(0xffffffffu, ok ? 0x7fffffff : key, i - base));
+  }
+  // first key of boxes [i, i + n) that the tile needs and that has no page
+  AK_D int missing(const PagedLists& l, int i, int n) const {
+    const int lane = threadIdx.x & 31;
+    const bool bad = (unsigned)raw >= (unsigned)l.num_pages && lane >= i - base && lane < i - base + n;
+    return __reduce_min_sync(0xffffffffu, bad ? key : 0x7fffffff);
   }
 };
 
