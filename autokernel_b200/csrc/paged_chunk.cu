@@ -7,16 +7,22 @@
 // 128, and the line of paged_sched.cuh gives every CTA (one per SM) the same number of keys, over item
 // boundaries and inside items: one long prompt occupies the whole GPU.
 //
-// 320 threads:
-//   warp 0      TMA producer: Q of each segment (3-D map [N, H, D], boxes of {128 / G tokens, G
-//               heads, 64}), then a 2-stage ring of {K, V} blocks gathered page by page (a box
-//               is gcd(page_size, 128) slots of a page)
+// 352 threads:
+//   warp 0      walks the line and posts its segments; TMA producer of Q (3-D map [N, H, D], boxes of
+//               {128 / G tokens, G heads, 64}) and of a 2-stage ring of K blocks, gathered page by
+//               page (a box is gcd(page_size, 128) slots of a page)
+//   warp 10     TMA producer of a 2-stage ring of V blocks
 //   warp 1      TMEM allocator and MMA issuer (S = Q K^T, O += P V with P from TMEM)
 //   warps 2..5  softmax and epilogue of tile 0, one thread per query row; warps 6..9 of tile 1
-// While one tile is in its softmax the tensor core works on the other.  P is rounded to 16 bits
-// once, as the matrix unit takes it; maximum, sum and output are fp32.  Slots of the last page
-// behind the last visible key may hold anything, NaN included: the producer zeroes their V rows
-// before the matrix unit sees them (their scores are masked).
+// While one tile is in its softmax the tensor core works on the other.  An item of one tile is split
+// instead: tile 0's threads take its even key blocks and tile 1's its odd ones, with a maximum, sum
+// and output of their own, and tile 0's threads join the two in the epilogue (a warp reads the
+// TMEM lanes of its quarter of either tile).
+//
+// P is rounded to 16 bits once, as the matrix unit takes it; maximum, sum and output are fp32.
+// Slots of the last page behind the last visible key may hold anything, NaN included: the
+// producer zeroes their V rows before the matrix unit sees them (their scores are masked).
+#include "attn_softmax.cuh"
 #include "paged_sched.cuh"
 
 namespace ak {
@@ -26,7 +32,7 @@ using namespace sm100;
 
 namespace chunk {
 
-constexpr int BQ = 128, BKV = 128, THREADS = 320;
+constexpr int BQ = 128, BKV = 128, THREADS = 352;
 constexpr int CHUNK_BYTES = 128 * 64 * 2;  // 128 rows x 64 16-bit elements
 constexpr int ROWS = 2 * BQ;               // rows of an item
 
@@ -48,25 +54,32 @@ struct Params {
   int box;  // slots per TMA box
   uint32_t idesc_qk, idesc_pv;
   float* ws;
+  Cutting* cuts;  // one per piece, behind the parts
 };
 
-// Key blocks of the segment that tile x takes, as an end: [blk0, end).  A tile whose tokens lie
-// behind the sequence takes none; under the causal mask tile 0 may stop before tile 1.
-struct Ends {
-  int e[2];
-  int lead;  // the tile that takes every block
+// A segment and what each tile does in it.  Tile x takes key blocks first[x], first[x] + step, ...
+// below end[x]: both take all of theirs (under the causal mask tile 0 may stop before tile 1, even
+// before it has begun), or a lone tile's blocks are split between them, or tile 1 takes none.
+struct Posted {
+  Segment s;
+  int part;  // workspace slot of its part; negative: there are no more segments
+  int two, split, step;
+  int first[2], end[2];
+  int bad;   // first key without a page of the blocks that have been loaded so far
 };
-AK_D Ends ends_of(const AttnArgs& a, const Params& p, const Segment& s) {
-  Ends x;
-  const bool two = s.t_lo + p.tt < s.t_hi;
-  x.lead = two ? 1 : 0;
-  x.e[1] = two ? s.blk1 : s.blk0;
-  x.e[0] = s.blk1;
-  if (two && a.causal) {
+AK_D void plan(const AttnArgs& a, const Params& p, Posted& x) {
+  const Segment& s = x.s;
+  x.two = s.t_lo + p.tt < s.t_hi;
+  x.split = !x.two && s.blk1 - s.blk0 >= 2;
+  x.step = x.split ? 2 : 1;
+  x.first[0] = s.blk0;
+  x.first[1] = s.blk0 + x.split;
+  x.end[0] = s.blk1;
+  x.end[1] = x.two || x.split ? s.blk1 : s.blk0;
+  if (x.two && a.causal) {
     const int hi = min(visible_keys(s.r, s.t_lo + p.tt - 1, 1), capacity(a.l));
-    x.e[0] = max(s.blk0, min(s.blk1, (hi + BKV - 1) / BKV));
+    x.end[0] = max(s.blk0, min(s.blk1, (hi + BKV - 1) / BKV));
   }
-  return x;
 }
 
 template <int DT, int D>
@@ -80,9 +93,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~(uintptr_t)1023);
-  __shared__ uint64_t q_full, q_empty, k_full[2], v_full[2], kv_empty[2], s_full[2], p_full[2],
-      o_done[2], o_free[2], v_land;
-  __shared__ int s_bad[2];  // first key of the block in a ring slot that has no page
+  constexpr int POSTS = 4;
+  __shared__ uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2],
+      p_full[2], o_done[2], o_free[2], v_land, ml_full, ml_free, post_full[POSTS], post_empty[POSTS];
+  __shared__ Posted s_post[POSTS];
+  __shared__ float2 s_ml[BQ];  // a split tile's second maximum and sum
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -92,14 +107,21 @@ __global__ void __launch_bounds__(THREADS, 1)
     mbar_init(&q_full, 1);
     mbar_init(&q_empty, 1);
     mbar_init(&v_land, 1);
+    mbar_init(&ml_full, 4);
+    mbar_init(&ml_free, 4);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_done[i], 1);
       mbar_init(&o_free[i], 4);
+    }
+    for (int i = 0; i < POSTS; ++i) {
+      mbar_init(&post_full[i], 1);
+      mbar_init(&post_empty[i], 10);  // the V producer, the MMA issuer and eight softmax warps
     }
     abort_flag = 0;
     fence_mbar_init();
@@ -117,57 +139,108 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   volatile int* abort_p = &abort_flag;
-  Walker walk(a, p.rule, line, blockIdx.x);
-  Segment s;
+  // the n-th segment, or null when there is none (or another role gave up); released when done with
+  auto segment = [&](int n) -> const Posted* {
+    return mbar_wait(&post_full[n % POSTS], (n / POSTS) & 1, abort_p) && s_post[n % POSTS].part >= 0
+               ? &s_post[n % POSTS]
+               : nullptr;
+  };
+  const int boxes = BKV / p.box;
 
-  if (warp == 0) {  // ------------------------------------------------------- TMA producer
-    const int boxes = BKV / p.box;
-    int g = 0, nq = 0, nv = 0;  // ring slots, Q loads and tail blocks so far
+  if (warp == 0) {  // ----------------------------------------------- segments, Q and K
+    Walker walk(a, p.rule, line, blockIdx.x);
+    Posted x;
+    int g = 0, nq = 0, posted = 0;  // K blocks, Q loads and segments so far
+    auto post = [&]() -> bool {
+      bool ok = mbar_wait(&post_empty[posted % POSTS], ((posted / POSTS) & 1) ^ 1, abort_p);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok && lane == 0) {
+        s_post[posted % POSTS] = x;
+        mbar_arrive(&post_full[posted % POSTS]);
+      }
+      __syncwarp();
+      ++posted;
+      return ok;
+    };
     bool ok = true;
-    while (ok && walk.next(s)) {
-      if (s.blk0 == s.blk1) continue;  // no keys: nothing to load
-      const Ends ends = ends_of(a, p, s);
+    while (ok && walk.next(x.s)) {
+      const Segment& s = x.s;
+      x.part = 2 * blockIdx.x + s.slot;
+      x.bad = 0x7fffffff;
+      plan(a, p, x);
+      ok = post();
+      if (!ok || s.blk0 == s.blk1) continue;  // no keys: nothing to load
       PageFeed feed;
       feed.start(a, s, s.blk0 * boxes, p.box);
+      ok = nq == 0 || mbar_wait(&q_empty, (nq - 1) & 1, abort_p);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      if (lane == 0) {
+        mbar_expect_tx(&q_full, (1 + x.two) * C::NC * p.tt * a.G * 128);
+        for (int t = 0; t <= x.two; ++t)
+          for (int c = 0; c < C::NC; ++c)
+            tma_load_3d(smem + C::Q_OFF + t * C::TILE_BYTES + c * CHUNK_BYTES, &tq, &q_full, c * 64,
+                        s.h * a.G, s.r.begin + s.t_lo + t * p.tt);
+      }
+      ++nq;
       for (int blk = s.blk0; blk < s.blk1; ++blk, ++g) {
         const int st = g & 1;
         feed.reach(a, s, blk * boxes, p.box);
-        if (blk == s.blk0) {
-          ok = nq == 0 || mbar_wait(&q_empty, (nq - 1) & 1, abort_p);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          if (lane == 0) {
-            mbar_expect_tx(&q_full, (1 + ends.lead) * C::NC * p.tt * a.G * 128);
-            for (int x = 0; x <= ends.lead; ++x)
-              for (int c = 0; c < C::NC; ++c)
-                tma_load_3d(smem + C::Q_OFF + x * C::TILE_BYTES + c * CHUNK_BYTES, &tq, &q_full,
-                            c * 64, s.h * a.G, s.r.begin + s.t_lo + x * p.tt);
-          }
-          ++nq;
+        ok = mbar_wait(&k_empty[st], ((g >> 1) & 1) ^ 1, abort_p);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        x.bad = min(x.bad, feed.missing(a.l, blk * boxes, boxes));
+        for (int i = 0; i < boxes; ++i) {
+          int page, slot;
+          feed.get(a.l, blk * boxes + i, page, slot);
+          if (lane == 0)
+#pragma unroll
+            for (int c = 0; c < C::NC; ++c)
+              tma_load_4d(smem + C::K_OFF + st * C::TILE_BYTES + i * p.box * 128 + c * CHUNK_BYTES, &tk,
+                          &k_full[st], c * 64, slot, s.h, page);
         }
-        ok = mbar_wait(&kv_empty[st], ((g >> 1) & 1) ^ 1, abort_p);
+        if (lane == 0) {  // the phase cannot end before this arrival
+          s_post[(posted - 1) % POSTS].bad = x.bad;
+          mbar_expect_tx(&k_full[st], C::TILE_BYTES);
+        }
+      }
+    }
+    x.part = -1;
+    if (ok) post();
+    if (lane == 0) p.cuts[blockIdx.x] = cutting_of(walk, line);
+    if (*abort_p && lane == 0) {  // giving up: wait for the copies in flight
+      drain_ring(k_full, 2, g);
+      if (nq) drain_ring(&q_full, 1, nq);
+    }
+  } else if (warp == 10) {  // ------------------------------------------------------- V
+    int g = 0, nv = 0;  // V blocks and tail blocks so far
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const Posted* x = segment(n);
+      x = __all_sync(0xffffffffu, x != nullptr) ? x : nullptr;
+      if (!x) break;
+      const Segment s = x->s;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&post_empty[n % POSTS]);
+      PageFeed feed;
+      if (s.blk0 < s.blk1) feed.start(a, s, s.blk0 * boxes, p.box);
+      for (int blk = s.blk0; blk < s.blk1; ++blk, ++g) {
+        const int st = g & 1;
+        feed.reach(a, s, blk * boxes, p.box);
+        ok = mbar_wait(&v_empty[st], ((g >> 1) & 1) ^ 1, abort_p);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         // slots of a loaded page behind the last visible key: V must read as zeros there
         const int live = s.kv_hi - blk * BKV;
         const bool tail = live < BKV && live % p.box != 0;
         uint64_t* v_bar = tail ? &v_land : &v_full[st];
-        const int bad = feed.missing(a.l, blk * boxes, boxes);
         for (int i = 0; i < boxes; ++i) {
           int page, slot;
           feed.get(a.l, blk * boxes + i, page, slot);
-          if (lane == 0) {
-            uint8_t* dst = smem + st * C::TILE_BYTES + i * p.box * 128;
+          if (lane == 0)
 #pragma unroll
-            for (int c = 0; c < C::NC; ++c) {
-              tma_load_4d(dst + C::K_OFF + c * CHUNK_BYTES, &tk, &k_full[st], c * 64, slot, s.h, page);
-              tma_load_4d(dst + C::V_OFF + c * CHUNK_BYTES, &tv, v_bar, c * 64, slot, s.h, page);
-            }
-          }
+            for (int c = 0; c < C::NC; ++c)
+              tma_load_4d(smem + C::V_OFF + st * C::TILE_BYTES + i * p.box * 128 + c * CHUNK_BYTES, &tv,
+                          v_bar, c * 64, slot, s.h, page);
         }
-        if (lane == 0) {  // the phases cannot end before these arrivals
-          s_bad[st] = bad;
-          mbar_expect_tx(&k_full[st], C::TILE_BYTES);
-          mbar_expect_tx(v_bar, C::TILE_BYTES);
-        }
+        if (lane == 0) mbar_expect_tx(v_bar, C::TILE_BYTES);
         __syncwarp();
         if (tail) {
           ok = mbar_wait(&v_land, nv++ & 1, abort_p);
@@ -184,22 +257,23 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
     }
-    if (*abort_p && lane == 0) {  // giving up: wait for the copies in flight
-      drain_ring(k_full, 2, g);
+    if (*abort_p && lane == 0) {
       drain_ring(v_full, 2, g);
-      if (nq) drain_ring(&q_full, 1, nq);
+      if (nv) drain_ring(&v_land, 1, nv);
     }
   } else if (warp == 1) {
     if (lane == 0) {  // ------------------------------------------------------ MMA issuer
       const uint32_t sq = smem_u32(smem + C::Q_OFF);
       const uint32_t sk = smem_u32(smem + C::K_OFF);
       const uint32_t sv = smem_u32(smem + C::V_OFF);
-      auto qk = [&](int x, int st) {  // S_x = Q_x K_st^T
+      // (tile numbers below are constants of unrolled loops: this thread's arithmetic is on the way of
+      // every product)
+      auto qk = [&](int x, uint32_t q, int st) {  // S_x = Q K_st^T
         const uint32_t d = tmem + x * C::TMEM_TILE;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk >> 2) * CHUNK_BYTES + (kk & 3) * 32;
-          umma_ss(d, desc_kmajor(sq + x * C::TILE_BYTES + off),
+          umma_ss(d, desc_kmajor(q + off),
                   desc_kmajor(sk + st * C::TILE_BYTES + off), p.idesc_qk, kk > 0);
         }
       };
@@ -212,57 +286,66 @@ __global__ void __launch_bounds__(THREADS, 1)
                   desc_mnmajor(sv + st * C::TILE_BYTES + kk * 16 * 128, CHUNK_BYTES), p.idesc_pv,
                   (acc || kk > 0) ? 1 : 0);
       };
-      int g = 0, nq = 0;
+      int g = 0, nq = 0;     // blocks before the segment, segments with blocks
+      int kw = 0;            // K blocks that have been waited for
       int cnt[2] = {0, 0};   // key blocks processed so far by each tile (S / P phases)
       int used[2] = {0, 0};  // segments in which each tile had blocks (O phases)
       bool ok = true;
-      while (ok && walk.next(s)) {
-        if (s.blk0 == s.blk1) continue;
-        const Ends ends = ends_of(a, p, s);
-        const int lead = ends.lead;
-        if (!mbar_wait(&q_full, nq++ & 1, abort_p) ||
-            !mbar_wait(&k_full[g & 1], (g >> 1) & 1, abort_p))
-          break;
-        tc_fence_after();
-        // S of both tiles for the first block (the previous segment's P V, issued earlier, has
-        // read S by the time the tensor core gets here)
-        for (int x = 0; x < 2; ++x)
-          if (s.blk0 < ends.e[x]) {
-            qk(x, g & 1);
-            umma_commit(&s_full[x]);
+      for (int n = 0; ok; ++n) {
+        const Posted* post = segment(n);
+        if (!post) break;
+        const int blk0 = post->s.blk0, blk1 = post->s.blk1;
+        const int two = post->two, split = post->split, step = post->step;
+        const int first[2] = {post->first[0], post->first[1]}, end[2] = {post->end[0], post->end[1]};
+        mbar_arrive(&post_empty[n % POSTS]);
+        if (blk0 == blk1) continue;
+        const uint32_t q1 = two ? sq + C::TILE_BYTES : sq;  // what tile 1 multiplies
+        // S of tile x for block j, once K_j is there; a block's last reader frees it
+        auto score = [&](int x, int j) -> bool {
+          const int at = g + j - blk0;
+          while (kw <= at) {
+            if (!mbar_wait(&k_full[kw & 1], (kw >> 1) & 1, abort_p)) return false;
+            ++kw;
           }
-        if (s.blk1 - s.blk0 == 1) umma_commit(&q_empty);  // that was the last read of Q
-        for (int j = s.blk0; ok && j < s.blk1; ++j, ++g) {
-          const int st = g & 1;
-          bool v_ready = false, k_ready = false;
-          for (int x = 0; x < 2 && ok; ++x) {
-            if (j >= ends.e[x]) continue;
-            if (!mbar_wait(&p_full[x], cnt[x] & 1, abort_p)) { ok = false; break; }
+          tc_fence_after();
+          qk(x, x ? q1 : sq, at & 1);
+          umma_commit(&s_full[x]);
+          if (!two || x == 1) umma_commit(&k_empty[at & 1]);
+          if ((!two || x == 1) && j == blk1 - 1) umma_commit(&q_empty);  // the last read of Q
+          return true;
+        };
+        if (!mbar_wait(&q_full, nq++ & 1, abort_p)) break;
+        // (the previous segment's P V, issued earlier, have read S by the time the tensor core gets here)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (ok && first[x] < end[x]) ok = score(x, first[x]);
+        for (int j = blk0; ok && j < blk1; ++j) {
+          const int st = (g + j - blk0) & 1;
+          bool v_ready = false;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || j >= end[x] || (split && ((j - blk0) & 1) != x)) continue;
+            if (!mbar_wait(&p_full[x], cnt[x] & 1, abort_p)) { ok = false; continue; }
             // a segment's first P V overwrites O: the tile's last epilogue must have read it
-            if (j == s.blk0 && used[x] > 0 && !mbar_wait(&o_free[x], (used[x] - 1) & 1, abort_p)) {
+            if (j == first[x] && used[x] > 0 && !mbar_wait(&o_free[x], (used[x] - 1) & 1, abort_p)) {
               ok = false;
-              break;
+              continue;
             }
-            if (!v_ready && !mbar_wait(&v_full[st], (g >> 1) & 1, abort_p)) { ok = false; break; }
+            if (!v_ready && !mbar_wait(&v_full[st], ((g + j - blk0) >> 1) & 1, abort_p)) { ok = false; continue; }
             v_ready = true;
             tc_fence_after();
-            pv(x, st, j > s.blk0);
+            pv(x, st, j > first[x]);
             ++cnt[x];
-            if (x == lead) umma_commit(&kv_empty[st]);
-            if (j == ends.e[x] - 1) {
+            if (!two || x == 1) umma_commit(&v_empty[st]);
+            if (j + step >= end[x]) {
               umma_commit(&o_done[x]);
               ++used[x];
             } else {
-              const int ng = g + 1;
-              if (!k_ready && !mbar_wait(&k_full[ng & 1], (ng >> 1) & 1, abort_p)) { ok = false; break; }
-              k_ready = true;
-              tc_fence_after();
-              qk(x, ng & 1);
-              umma_commit(&s_full[x]);
-              if (x == lead && j + 2 == s.blk1) umma_commit(&q_empty);
+              ok = score(x, j + step);
             }
           }
         }
+        g += blk1 - blk0;
       }
     }
   } else {  // ---------------------------------------------------------- softmax / epilogue
@@ -274,21 +357,22 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t t_o = t_s + 128;
     const int cap = capacity(a.l);
     bool ok = true;
-    int cnt = 0, used = 0, g = 0;
-    while (ok && walk.next(s)) {
-      const Ends ends = ends_of(a, p, s);
-      const int tok = s.t_lo + x * p.tt + row / a.G;
-      const bool valid = row < p.tt * a.G && tok < s.t_hi;
-      const int vis = valid ? visible_keys(s.r, tok, a.causal) : 0;
+    int cnt = 0, n_split = 0;
+    int used[2] = {0, 0};  // segments in which each tile had blocks
+    for (int n = 0; ok; ++n) {
+      const Posted* post = segment(n);
+      if (!__all_sync(0xffffffffu, post != nullptr)) break;
+      int vis;  // keys that this thread's row sees; what else is known of the row is looked up again in
+      {         // the epilogue: the loop needs every register
+        const int tok = post->s.t_lo + (post->split ? 0 : x) * p.tt + row / a.G;
+        vis = row < p.tt * a.G && tok < post->s.t_hi ? visible_keys(post->s.r, tok, a.causal) : 0;
+      }
       float m_ref = -INFINITY, l = 0.f;
-      int bad = cap;
-      const int g0 = g;
-      g += s.blk1 - s.blk0;
-      for (int j = s.blk0; j < ends.e[x]; ++j, ++cnt) {
+      const int step = post->step, end = post->end[x];
+      for (int j = post->first[x]; j < end; j += step, ++cnt) {
         const bool w = mbar_wait(&s_full[x], cnt & 1, abort_p);
         if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
         tc_fence_after();
-        bad = min(bad, s_bad[(g0 + j - s.blk0) & 1]);
         const int kmax = vis - j * BKV;  // keys below this are visible to the row
         uint32_t r[128];
 #pragma unroll
@@ -356,52 +440,94 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) mbar_arrive(&p_full[x]);
       }
       if (!ok) break;
-      const bool took = s.blk0 < ends.e[x];  // the tile has an O
-      if (took) {
-        const bool w = mbar_wait(&o_done[x], used & 1, abort_p);
+      const Segment& s = post->s;
+      const bool split = post->split;
+      const int tile = split ? 0 : x;
+      const int tok = s.t_lo + tile * p.tt + row / a.G;
+      const bool valid = row < p.tt * a.G && tok < s.t_hi;
+      // (blocks loaded since then, if any, hold no key that this tile's rows see)
+      if (vis > min(post->bad, cap)) l = __int_as_float(0x7fffffff);  // a key that the row sees has no page
+      const bool took[2] = {post->first[0] < post->end[0], post->first[1] < post->end[1]};
+      bool w = true;
+      if (split && x == 1) {  // its output is joined by tile 0's threads
+        w = n_split == 0 || mbar_wait(&ml_free, (n_split - 1) & 1, abort_p);
         if (!__all_sync(0xffffffffu, w)) break;
-        tc_fence_after();
-        ++used;
+        s_ml[row] = make_float2(m_ref, l);
+        ++n_split;
+        ++used[0];
+        ++used[1];
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&ml_full);
+          mbar_arrive(&post_empty[n % POSTS]);
+        }
+        continue;
       }
-      if (vis > bad) l = __int_as_float(0x7fffffff);  // a key that the row sees has no page
+      if (took[x]) w = mbar_wait(&o_done[x], used[x] & 1, abort_p);
+      float f0 = 1.f, f1 = 0.f;  // weights of the tile's output and of the second one of a split
+      if (split) {
+        w = w && mbar_wait(&o_done[1], used[1] & 1, abort_p) && mbar_wait(&ml_full, n_split & 1, abort_p);
+        const float2 ml = s_ml[row];
+        const float mn = fmaxf(m_ref, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+        f0 = ex2_approx(m_ref - ref);
+        f1 = ex2_approx(ml.x - ref);
+        l = l * f0 + ml.y * f1;
+        m_ref = mn;
+        ++n_split;
+      }
+      if (!__all_sync(0xffffffffu, w)) break;
+      if (split && lane == 0) mbar_arrive(&ml_free);
+      tc_fence_after();
+      used[0] += took[0];
+      used[1] += took[1];
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* orow = reinterpret_cast<T*>(a.o) + (int64_t)(s.r.begin + tok) * a.os[0] +
                 (int64_t)(s.h * a.G + row % a.G) * a.os[1];
-      float* part = p.ws + ((int64_t)blockIdx.x * 2 + s.slot) * C::PART;
+      float* part = p.ws + (int64_t)post->part * C::PART;
       const int prow = x * BQ + row;
-      bool odd = false;  // a result that is not finite
+      float odd = 0.f;  // NaN once a result is not finite
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
         __syncwarp();
-        if (took) {
+        if (took[x]) {
           tmem_ld32(t_o + c * 32, r);
           tmem_wait_ld();
           tmem_regs_ready(r);
+          if (split) {
+            uint32_t r1[32];
+            tmem_ld32(t_o + C::TMEM_TILE + c * 32, r1);
+            tmem_wait_ld();
+            tmem_regs_ready(r1);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              r[i] = __float_as_uint(__uint_as_float(r[i]) * f0 + __uint_as_float(r1[i]) * f1);
+          }
           if (c == D / 32 - 1) {  // O has been read
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&o_free[x]);
+            if (lane == 0) {
+              mbar_arrive(&o_free[x]);
+              if (split) mbar_arrive(&o_free[1]);
+            }
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) r[i] = 0;
         }
-        if (!valid) continue;
         if (s.whole) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            uint4 raw;
-            T* e = reinterpret_cast<T*>(&raw);
+            uint32_t e[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float y = l == 0.f ? 0.f : __uint_as_float(r[q * 8 + i]) * inv;
-              odd |= !(fabsf(y) <= 3.4028235e38f);
-              e[i] = E::from_f(y);
+            for (int i = 0; i < 4; ++i) {
+              const float y0 = __uint_as_float(r[q * 8 + 2 * i]) * inv, y1 = __uint_as_float(r[q * 8 + 2 * i + 1]) * inv;
+              odd = fmaf(y0, 0.f, fmaf(y1, 0.f, odd));
+              e[i] = attn_sm::pack2<DT>(y0, y1);
             }
-            reinterpret_cast<uint4*>(orow + c * 32)[q] = raw;
+            if (valid) reinterpret_cast<uint4*>(orow + c * 32)[q] = make_uint4(e[0], e[1], e[2], e[3]);
           }
-        } else {
+        } else if (valid) {
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             __stcg(reinterpret_cast<uint4*>(part) + (c * 8 + q) * ROWS + prow,
@@ -413,7 +539,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         part[ROWS * D + ROWS + prow] = l;
       }
       // rows whose result is not finite although their weights are, beside keys hidden from them
-      unsigned again = __ballot_sync(0xffffffffu, odd && fabsf(l) <= 3.4028235e38f && vis < s.kv_hi);
+      unsigned again = __ballot_sync(0xffffffffu, odd != 0.f && valid && fabsf(l) <= 3.4028235e38f && vis < s.kv_hi);
       while (again) {
         const int i = __ffs(again) - 1, rr = quarter * 32 + i;
         again &= again - 1;
@@ -423,6 +549,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           row_by_key<DT>(a, s.b, s.r, t, s.h * a.G + rr % a.G);
       }
       __syncwarp();
+      if (lane == 0) mbar_arrive(&post_empty[n % POSTS]);
     }
   }
   __syncthreads();
@@ -446,8 +573,8 @@ __global__ void __launch_bounds__(128)
   __shared__ int s_whole, s_again;
   if (threadIdx.x == 0) s_whole = s_again = 0;
   Line line;
-  const Parts parts = find_parts(a, p.rule, line);
   wait_for_parts();
+  const Parts parts = parts_of(a, p.rule, p.cuts[blockIdx.x], line);
   if (parts.n == 0) return;
   const Segment& s = parts.s;
   const int lane = threadIdx.x & 31, part_d = threadIdx.x >> 5;
@@ -526,11 +653,12 @@ static int launch(const AttnArgs& a, float* ws, cudaStream_t st) {
   Params p{};
   p.tt = BQ / a.G;
   p.box = gcd_int(a.l.page_size, BKV);
-  p.rule = TileRule{0, 2 * p.tt, 7, 128, 512, device_info().sm_count, 1};
+  p.rule = TileRule{0, 2 * p.tt, 7, 128, 320, 512, device_info().sm_count, 1};
   const int fmt = DT == AK_BF16 ? 1 : 0;
   p.idesc_qk = idesc_f16(fmt, BQ, BKV, false, false);
   p.idesc_pv = idesc_f16(fmt, BQ, D, false, true);
   p.ws = ws;
+  p.cuts = reinterpret_cast<Cutting*>(ws + 2 * (size_t)device_info().sm_count * Cfg<D>::PART);
   CUtensorMap tq, tk, tv;
   const uint64_t dims[3] = {(uint64_t)D, (uint64_t)a.H, (uint64_t)a.l.N};
   const uint64_t strides[2] = {(uint64_t)(a.H > 1 ? a.qs[1] : D) * 2,
@@ -552,7 +680,7 @@ static int launch(const AttnArgs& a, float* ws, cudaStream_t st) {
 }  // namespace chunk
 
 size_t chunk_workspace(int D) {
-  return 2 * (size_t)device_info().sm_count * chunk::ROWS * (D + 2) * sizeof(float);
+  return (size_t)device_info().sm_count * (2 * chunk::ROWS * (D + 2) * sizeof(float) + sizeof(Cutting));
 }
 
 int run_chunk(const AttnArgs& a, void* ws, cudaStream_t st) {

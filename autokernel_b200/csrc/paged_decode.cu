@@ -45,7 +45,7 @@ static TileRule decode_rule(const AttnArgs& a) {
   const int ctas = device_info().sm_count;
   const double tiles = (double)a.l.B + (double)a.l.N * a.G / kRows;
   const double keys = tiles * a.Hkv * ((double)a.l.max_pages * a.l.page_size + 64);
-  return TileRule{kRows, 0, 6, 64, 256, ctas, keys / ctas >= 4 * kLongPiece && a.l.B <= 512 ? kRounds : 1};
+  return TileRule{kRows, 0, 6, 64, 0, 256, ctas, keys / ctas >= 4 * kLongPiece && a.l.B <= 512 ? kRounds : 1};
 }
 
 static size_t decode_part_floats(int D) { return (size_t)kRows * (D + 2); }

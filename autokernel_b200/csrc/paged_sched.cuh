@@ -25,6 +25,7 @@ struct TileRule {
   int tokens;  // tokens per tile otherwise
   int shift;   // log2 of the keys per block
   int over;    // cost of a tile beside its keys, in keys
+  int lone;    // more of it for a sequence of at most half a tile's tokens, whose blocks go faster
   int64_t min_piece;  // shortest piece of the line that a CTA gets
   int ctas;           // CTAs that run at once
   int rounds;         // kRounds: a long line may be cut into rounds of pieces; or 1
@@ -61,12 +62,13 @@ AK_D SeqCost seq_cost(const AttnArgs& a, const TileRule& t, const SeqRange& r) {
     c.base = c.last = (int64_t)kv + t.over;
   } else {
     c.tiles = (r.n + t.tokens - 1) / t.tokens;
+    const int over = t.over + (2 * r.n <= t.tokens ? t.lone : 0);
     if (a.causal) {
-      c.base = (int64_t)max(kv - r.n, 0) + t.over;
+      c.base = (int64_t)max(kv - r.n, 0) + over;
       c.slope = t.tokens;
       c.last = c.base + r.n;
     } else {
-      c.base = c.last = (int64_t)kv + t.over;
+      c.base = c.last = (int64_t)kv + over;
     }
   }
   return c;
@@ -250,9 +252,12 @@ struct Walker {
   SeqRange r;
   SeqCost c;
   int64_t head;  // length of one head of sequence b
+  // the last tile that was come to, and where it lies on the line
+  int last_b, last_h, last_tile;
+  int64_t last_at, last_cost;
 
   AK_D Walker(const AttnArgs& a_, const TileRule& t_, const Line& line, int piece)
-      : a(a_), t(t_), head(0) {
+      : a(a_), t(t_), head(0), last_b(-1), last_h(0), last_tile(0), last_at(0), last_cost(0) {
     go(line, piece);
   }
   AK_D void go(const Line& line, int piece) {
@@ -282,6 +287,11 @@ struct Walker {
       s.b = b;
       s.tile = c.find(y);
       const int64_t cost = c.cost(s.tile), z0 = y - c.prefix(s.tile);
+      last_b = b;
+      last_h = s.h;
+      last_tile = s.tile;
+      last_at = x - z0;
+      last_cost = cost;
       const int64_t z1 = min(cost, z0 + (end - x));
       s.slot = x == start ? 0 : 1;
       x += z1 - z0;
@@ -331,6 +341,34 @@ AK_D Parts find_parts(const AttnArgs& a, const TileRule& t, Line& line) {
   set_blocks(a, t, p.cost, 0, p.cost, p.s);
   p.first = c - 1;
   if (p.s.nb) p.n = line.cut.holds(p.at + p.cost - 1) - (c - 1) + 1;
+  return p;
+}
+
+// What the join at boundary c has to know, left by the CTA of piece c - 1 (where join blocks find no
+// room beside the main kernel, looking for it there would come after it).
+struct Cutting {
+  int b, h, tile, valid;
+  int64_t at, cost, unit;
+};
+// of the last tile that a piece [start, end) came to
+AK_D Cutting cutting_of(const Walker& w, const Line& line) {
+  const bool first = w.last_b >= 0 && w.last_at >= w.start && w.last_at + w.last_cost > w.end;
+  return Cutting{w.last_b, w.last_h, w.last_tile, first, w.last_at, w.last_cost, line.cut.unit};
+}
+AK_D Parts parts_of(const AttnArgs& a, const TileRule& t, const Cutting& k, Line& line) {
+  Parts p;
+  p.n = 0;
+  if (!k.valid) return p;
+  line.cut = Cut{k.unit, t.ctas, false};
+  p.s.b = k.b;
+  p.s.h = k.h;
+  p.s.tile = k.tile;
+  p.s.r = seq_range(a.l, k.b);
+  p.at = k.at;
+  p.cost = k.cost;
+  p.first = blockIdx.x;
+  set_blocks(a, t, p.cost, 0, p.cost, p.s);
+  if (p.s.nb) p.n = line.cut.holds(p.at + p.cost - 1) - p.first + 1;
   return p;
 }
 
