@@ -544,3 +544,13 @@ def test_attention_decode_wide_table():
     b.table = wide
     q, o = attend(b, 8)
     check_attention(b, q, o)
+
+
+@pytest.mark.parametrize("D,dt", [(64, "bf16"), (128, "f16")])
+def test_attention_chunks_long_line(D, dt):
+    """Chunks whose line is long enough for a second round of pieces, with ragged neighbours."""
+    b = Batch(dt, [(300, 9000), (1, 12000), (65, 7000), (0, 0), (2, 2), (130, 20000)], 8, D, 64, seed=21)
+    q, o = attend(b, 8)
+    check_attention(b, q, o)
+    for _ in range(5):
+        assert torch.equal(attend(b, 8, q=q)[1], o)
