@@ -47,34 +47,29 @@ AK_D Place place_of(const PagedLists& l, int t) {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(256) append_vec_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 4) append_vec_kernel(const __grid_constant__ AppendArgs a) {
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr int VEC = E::kVec, P = VEC / 2;
-  constexpr int U = 6;  // vectors in flight per thread
-  const int vph = a.D / VEC, hstep = blockDim.x / vph;
-  const int dv = threadIdx.x % vph;
+  constexpr int U = 2;  // vectors of each tensor in flight per thread
+  const int vph = a.D / VEC;
+  const int dv = threadIdx.x % vph, h0 = blockIdx.y * (blockDim.x / vph) + threadIdx.x / vph;
+  const int step = gridDim.y * (blockDim.x / vph);  // this thread's heads: h0, h0 + step, ...
   const int t = blockIdx.x;
-  const int heads = 2 * a.Hkv + (a.q ? a.H : 0);
-  const int per = (heads + gridDim.y - 1) / gridDim.y;  // this CTA's heads [h_lo, h_hi)
-  const int h_lo = blockIdx.y * per, h_hi = min(heads, h_lo + per);
+  const T* kp = reinterpret_cast<const T*>(a.k) + t * a.ks[0] + dv * VEC;
+  const T* vp = reinterpret_cast<const T*>(a.v) + t * a.vs[0] + dv * VEC;
+  const T* qp = reinterpret_cast<const T*>(a.q) + t * a.qs[0] + dv * VEC;
+  auto at = [](const T* p, int64_t off) { return __ldcs(reinterpret_cast<const uint4*>(p + off)); };
+  const int H = a.q ? a.H : 0;
 
-  auto source = [&](int h) -> const uint4* {
-    const T* p;
-    if (h < a.Hkv)
-      p = reinterpret_cast<const T*>(a.k) + t * a.ks[0] + h * a.ks[1];
-    else if (h < 2 * a.Hkv)
-      p = reinterpret_cast<const T*>(a.v) + t * a.vs[0] + (h - a.Hkv) * a.vs[1];
-    else
-      p = reinterpret_cast<const T*>(a.q) + t * a.qs[0] + (h - 2 * a.Hkv) * a.qs[1];
-    return reinterpret_cast<const uint4*>(p + dv * VEC);
-  };
-
-  const int h_first = h_lo + threadIdx.x / vph;
-  uint4 x[U];
+  uint4 k[U], v[U], q[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (h_first + u * hstep < h_hi) x[u] = __ldcs(source(h_first + u * hstep));
+  for (int u = 0; u < U; ++u) {
+    const int h = h0 + u * step;
+    if (h < a.Hkv) k[u] = at(kp, h * a.ks[1]);
+    if (h < a.Hkv) v[u] = at(vp, h * a.vs[1]);
+    if (h < H) q[u] = at(qp, h * a.qs[1]);
+  }
 
   __shared__ Place s_place;
   if (threadIdx.x < 32) {
@@ -98,44 +93,46 @@ __global__ void __launch_bounds__(256) append_vec_kernel(const AppendArgs a) {
       s[i] = in ? reinterpret_cast<const float*>(&sv)[i] : __int_as_float(0x7fffffff);
     }
   }
-
-  for (int h0 = h_first; h0 < h_hi; h0 += U * hstep) {
-    if (h0 != h_first) {
+  auto turned = [&](uint4 x) {
+    if (!a.cos) return x;
+    T* e = reinterpret_cast<T*>(&x);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (h0 + u * hstep < h_hi) x[u] = __ldcs(source(h0 + u * hstep));
+    for (int i = 0; i < P; ++i) {
+      const float x1 = E::to_f(e[2 * i]), x2 = E::to_f(e[2 * i + 1]);
+      e[2 * i] = E::from_f(fmaf(x1, c[i], -x2 * s[i]));
+      e[2 * i + 1] = E::from_f(fmaf(x1, s[i], x2 * c[i]));
     }
+    return x;
+  };
+  if (w.page >= 0) {
+    T* kd = reinterpret_cast<T*>(a.k_cache) + w.page * a.kcs[0] + w.slot * a.kcs[2] + dv * VEC;
+    T* vd = reinterpret_cast<T*>(a.v_cache) + w.page * a.vcs[0] + w.slot * a.vcs[2] + dv * VEC;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * hstep;
-      if (h >= h_hi) continue;
-      T* dst;
-      if (h < 2 * a.Hkv) {
-        if (w.page < 0) continue;
-        dst = h < a.Hkv ? reinterpret_cast<T*>(a.k_cache) + w.page * a.kcs[0] + h * a.kcs[1] +
-                              w.slot * a.kcs[2]
-                        : reinterpret_cast<T*>(a.v_cache) + w.page * a.vcs[0] +
-                              (h - a.Hkv) * a.vcs[1] + w.slot * a.vcs[2];
-      } else {
-        dst = reinterpret_cast<T*>(a.q_out) + t * a.os[0] + (h - 2 * a.Hkv) * a.os[1];
-      }
-      if (a.cos && (h < a.Hkv || h >= 2 * a.Hkv)) {
-        T* e = reinterpret_cast<T*>(&x[u]);
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-          const float x1 = E::to_f(e[2 * i]), x2 = E::to_f(e[2 * i + 1]);
-          e[2 * i] = E::from_f(fmaf(x1, c[i], -x2 * s[i]));
-          e[2 * i + 1] = E::from_f(fmaf(x1, s[i], x2 * c[i]));
-        }
-      }
-      *reinterpret_cast<uint4*>(dst + dv * VEC) = x[u];
+      const int h = h0 + u * step;
+      if (h >= a.Hkv) break;
+      *reinterpret_cast<uint4*>(kd + h * a.kcs[1]) = turned(k[u]);
+      *reinterpret_cast<uint4*>(vd + h * a.vcs[1]) = v[u];
+    }
+    for (int h = h0 + U * step; h < a.Hkv; h += step) {
+      const uint4 x = at(kp, h * a.ks[1]), y = at(vp, h * a.vs[1]);
+      *reinterpret_cast<uint4*>(kd + h * a.kcs[1]) = turned(x);
+      *reinterpret_cast<uint4*>(vd + h * a.vcs[1]) = y;
     }
   }
+  T* qd = reinterpret_cast<T*>(a.q_out) + t * a.os[0] + dv * VEC;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = h0 + u * step;
+    if (h < H) *reinterpret_cast<uint4*>(qd + h * a.os[1]) = turned(q[u]);
+  }
+  for (int h = h0 + U * step; h < H; h += step)
+    *reinterpret_cast<uint4*>(qd + h * a.os[1]) = turned(at(qp, h * a.qs[1]));
 }
 
 // Any even head dimension, stride and alignment: one thread per pair.
 template <int DT>
-__global__ void __launch_bounds__(256) append_scalar_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256) append_scalar_kernel(const __grid_constant__ AppendArgs a) {
   using E = Elem<DT>;
   using T = typename E::T;
   const int t = blockIdx.x;
@@ -204,11 +201,10 @@ int run_append(const AppendArgs& a, cudaStream_t st) {
   }
   const int vph = a.D / VEC;
   const int threads = vph * (256 / vph);
-  const int heads = 2 * a.Hkv + (a.q ? a.H : 0);
-  const int passes = (heads + threads / vph - 1) / (threads / vph);
+  const int most = a.q && a.H > a.Hkv ? a.H : a.Hkv, at_once = threads / vph;
   // few tokens: their heads spread over more CTAs, until every SM has one
   int split = 1;
-  while (split < passes && (int64_t)a.l.N * split < device_info().sm_count) ++split;
+  while (split * at_once < most && (int64_t)a.l.N * split < device_info().sm_count) ++split;
   append_vec_kernel<DT><<<dim3((unsigned)a.l.N, (unsigned)split), threads, 0, st>>>(a);
   return launch_status("paged_append");
 }
