@@ -168,10 +168,10 @@ __global__ void __launch_bounds__(512) sample_kernel(const SampleArgs a) {
 //      sorted and cut, and what is not kept dies.  A crowded bin is divided again by the bits of the
 //      rank.
 //   3  top-p: what top-k left, when it is few, is gathered and sorted at once.  Otherwise
-//      the histogram of counts times a weight per bin tells a small stretch of logits that holds the
-//      cut; one pass sums every weight exactly (64-bit floating point above and below the stretch,
-//      fixed point, 2^-45, in 1536 bins of the stretch, where no order of additions matters), and
-//      the stretch is cut like top-k's bin.
+//      the histogram of counts and mean places tells a small stretch of logits that holds the cut;
+//      one pass sums every weight exactly (64-bit floating point above and below the stretch, fixed
+//      point, 2^-45, in 1536 bins of the stretch, where no order of additions matters), and the
+//      stretch is cut like top-k's bin.  A cut outside of the stretch costs one more pass.
 //   4  kept weights per run of 32 vectors, then the run, the lane and the entry that u falls in
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1536, kList = 128, kNear = 2048;
 constexpr int kMaxSlice = 160 * 1024;                   // bytes of a row per CTA
@@ -384,6 +384,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __gri
       for (int i = tid; i < kBins; i += kThreads)
         s.h.digit[0][i] = s.h.digit[1][i] = s.h.digit[2][i] = s.h.count[i] = 0;
       if (tid == 0 && step == kSums) s.n_near = 0;
+      if (tid == 0 && estimate) {  // all of the row, should no bin of the estimate weigh anything
+        s.f_hi = max_;
+        s.f_lo = -3.4028235e38f;
+      }
       __syncthreads();
       if (step == kSums) {  // every weight: above the stretch, in its bins, below it
         double below = 0.0;
@@ -437,8 +441,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __gri
           float f[VEC];
           load(v, f);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (alive(f[e])) atomicAdd(&s.h.count[(int)units(f[e])], 1u);
+          for (int e = 0; e < VEC; ++e) {
+            if (!alive(f[e])) continue;
+            const float u = units(f[e]);
+            const int b = (int)u;
+            atomicAdd(&s.h.count[b], 1u);
+            if (top_p) atomicAdd(&s.h.digit[0][b], (uint32_t)((u - (float)b) * 256.f));  // where in the bin
+          }
         }
       } else {
         add_all();
@@ -446,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __gri
       // the leader's bins from every CTA's; each CTA adds up its share of them
       sync();
       const int share = kBins / C;
-      const bool counts = step == kCount && by == kUnits;
+      const bool counts = step == kCount && by == kUnits;  // (digit 0 is a sum of places then)
       if (C > 1 || !counts) {
         for (int i = rank * share + tid; i < (rank + 1) * share; i += kThreads) {
           u64 ms = 0;
@@ -455,13 +464,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __gri
           for (int c = 0; c < C; ++c) {
             const Bins& h = peer(c).h;
             cs += h.count[i];
-            if (!counts) ms += h.digit[0][i] + ((u64)h.digit[1][i] << 15) + ((u64)h.digit[2][i] << 30);
+            if (top_p) ms += h.digit[0][i];
+            if (!counts) ms += ((u64)h.digit[1][i] << 15) + ((u64)h.digit[2][i] << 30);
           }
           lead.h.count[i] = cs;
-          if (!counts) {
-            lead.h.digit[0][i] = (uint32_t)ms;
-            lead.h.digit[1][i] = (uint32_t)(ms >> 32);
-          }
+          lead.h.digit[0][i] = (uint32_t)ms;
+          lead.h.digit[1][i] = (uint32_t)(ms >> 32);
         }
       }
       sync();
@@ -470,14 +478,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __gri
       if (rank == 0) {
         constexpr int PER = kBins / kThreads;
         u64 c[PER], mine = 0, inc, above = 0, goal, all = 0;
-        double real = 0.0, square = 0.0;
+        double real = 0.0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int b = tid * PER + i;
           if (estimate) {
-            const double x = exp2(-(b + 0.5) / per_bin * rate) * kFixed;
-            c[i] = (u64)(s.h.count[b] * x);
-            square += s.h.count[b] * x * x;
+            // as if a bin's entries all were at their mean place
+            const double n = s.h.count[b], mean = n > 0.0 ? (s.h.digit[0][b] / n + 0.5) / 256.0 : 0.0;
+            c[i] = (u64)(n * exp2(-(b + mean) / per_bin * rate) * kFixed);
           } else {
             c[i] = !top_p ? s.h.count[b] : s.h.digit[0][b] | (u64)s.h.digit[1][b] << 32;
           }
@@ -489,18 +497,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __gri
           const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
           if (lane >= o) inc += y;
         }
-        square = warp_sum_d(square);
-        if (lane == 31) {
-          s.scan[warp] = inc;
-          s.red[warp] = square;
-        }
+        if (lane == 31) s.scan[warp] = inc;
         __syncthreads();
-        square = 0.0;
         u64 before = inc - mine;
         for (int i = 0; i < kWarps; ++i) {
           if (i < warp) before += s.scan[i];
           all += s.scan[i];
-          square += s.red[i];
         }
         if (by == kRanks) {
           above = s.above;
@@ -520,10 +522,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __gri
         }
         __syncthreads();  // everyone has read s.above and s.goal
         before += above;
-        // A weight per bin is off by up to half a bin, T / 96, either way at each entry, 0.6% on average:
-        // the cut is looked for within 3.5 standard deviations of their sum.
-        const double slack = 0.02 * sqrt(square);
-        const u64 goal0 = (u64)max((double)goal - slack, 1.0), goal1 = min((u64)((double)goal + slack), all);
+        // With bins of w times T, entries about their mean place weigh up to w^2 / 8 more than at it
+        // and the places' rounding moves them by up to w / 512: 1e-4 of all at w = 1 / 48.
+        const double wide = 1.0 / ((double)per_bin * set.t);
+        const double slack = wide * (0.5 * wide + 1.0 / 256.0) * (double)all;
+        const u64 goal0 = (u64)max((double)goal - slack, 1.0);
+        const u64 goal1 = min((u64)min((double)goal + slack, (double)all), all);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int b = tid * PER + i;

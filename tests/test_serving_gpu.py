@@ -449,6 +449,24 @@ def test_sample_settings_per_row(dt):
 
 
 @pytest.mark.parametrize("dt", list(DTS))
+@pytest.mark.parametrize("temperature", [1e-30, 1e-4, 0.01, 0.1, 0.3, 0.49, 5.0, 100.0, float("inf")])
+def test_sample_temperatures(dt, temperature):
+    """Cuts among very uneven and very even weights."""
+    x, u = logits(dt, 8, 40000, 10)
+    for kw in (dict(top_p=0.6), dict(top_p=0.999), dict(top_k=20000, top_p=0.95), dict(min_p=0.5)):
+        check_sample(x, u, temperature=temperature, **kw)
+
+
+@pytest.mark.parametrize("dt", list(DTS))
+@pytest.mark.parametrize("vocab", [262144, 262145, 300001])
+def test_sample_longest_rows(dt, vocab):
+    """Up to and beyond the rows that a cluster holds."""
+    x, u = logits(dt, 3, vocab, vocab)
+    for kw in (dict(), dict(top_k=50), dict(top_p=0.9), dict(temperature=0.0), dict(top_k=900, top_p=0.5, min_p=0.01)):
+        check_sample(x, u, **kw)
+
+
+@pytest.mark.parametrize("dt", list(DTS))
 @pytest.mark.parametrize("levels", [1, 2, 5, 60])
 def test_sample_ties(dt, levels):
     """Few distinct logits: cuts fall inside groups of equal ones, lowest index first."""
