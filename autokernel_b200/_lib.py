@@ -110,7 +110,9 @@ def dtype_code(t: torch.dtype) -> int:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The device's current stream, without the Stream object that torch.cuda.current_stream makes
+    (2.2 us of a call, against 0.07)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def require_cuda(*ts: torch.Tensor) -> torch.device:

@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 
 import torch
 
@@ -599,9 +600,6 @@ def flash_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, causal: b
 # Decoding calls these once per layer and token, so the checks read each property of a tensor once:
 # the call itself takes a few microseconds on the GPU.
 
-_I64x10, _I64x14 = ctypes.c_int64 * 10, ctypes.c_int64 * 14
-
-
 def _same_device(*ts: torch.Tensor) -> torch.device:
     """require_cuda, for tensors that are most often on the current device."""
     i = ts[0].get_device()
@@ -708,8 +706,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
             q_out = torch.empty_like(q)
             os = q_out.stride()
         qp, op = q.data_ptr(), q_out.data_ptr()
-    st = _I64x14(ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os[0], os[1], *kcs[:3], *vcs[:3])
-    at = ctypes.addressof(st)
+    st = array("q", (*ks[:2], *vs[:2], *qs[:2], *os[:2], *kcs[:3], *vcs[:3]))
+    at = st.buffer_info()[0]
     call("ak_paged_append", k.data_ptr(), v.data_ptr(), qp, op, k_cache.data_ptr(), v_cache.data_ptr(),
          page_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), cp, sp, N, B, H, Hkv, D, P, S, width, ld,
          positions, at, at + 16, at + 32, at + 48, at + 64, at + 88, code, stream_ptr(dev))
@@ -726,10 +724,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     token per sequence is decoding.  H is a multiple of the cache's heads: query head h reads
     key/value head h // (H // Hkv).  head_dim up to 256; sm_scale (D ** -0.5 by default) positive.
 
-    Returns [N, H, D] (written to out if given: any strides with a contiguous last dim).  A row that
-    sees no key is 0; one that sees a key without a page is NaN.  Rows behind cu_q[B] are left alone
-    (a fresh result is not initialised there).  Nothing behind a sequence's last key matters,
-    whatever the cache holds there."""
+    Returns [N, H, D] (written to out if given: any strides with a contiguous last dim, and none of
+    the inputs' memory).  A row that sees no key (or only scores of -inf) is 0; one that sees a key
+    without a page is NaN.  Rows behind cu_q[B] are left alone (a fresh result is not initialised
+    there).  Nothing behind a sequence's last key matters, whatever the cache holds there."""
     name = "paged_attention"
     (P, Hkv, S, D), kcs, vcs, dt, B, width, ld = _paged_cache(name, k_cache, v_cache, page_table, cu_q, kv_lens)
     (N, H, _), qs = _tokens(name, "q", q, None, None, D, dt)
@@ -751,8 +749,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         dev = _same_device(q, k_cache, v_cache, page_table, cu_q, kv_lens, out)
     nbytes = _lib.load().ak_paged_attention_workspace_size(N, B, H, Hkv, D, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    st = _I64x10(qs[0], qs[1], os[0], os[1], *kcs[:3], *vcs[:3])
-    at = ctypes.addressof(st)
+    st = array("q", (*qs[:2], *os[:2], *kcs[:3], *vcs[:3]))
+    at = st.buffer_info()[0]
     call("ak_paged_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
          page_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), N, B, H, Hkv, D, P, S, width, ld,
          at, at + 16, at + 32, at + 56, 1 if causal else 0, sm_scale, code,
