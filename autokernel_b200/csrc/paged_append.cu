@@ -236,8 +236,8 @@ extern "C" int ak_paged_append(const void* k, const void* v, const void* q, void
   AK_REQUIRE((cos == nullptr) == (sin == nullptr), AK_ERR_ARG, "cos and sin go together");
   AK_REQUIRE(!cos || positions > 0, AK_ERR_SHAPE, "cos and sin hold no position");
   if (N == 0 || B == 0) return AK_OK;
-  AK_REQUIRE(k && v && k_cache && v_cache && page_table && cu_q && kv_lens && k_strides &&
-                 v_strides && k_cache_strides && v_cache_strides,
+  AK_REQUIRE(k && v && cu_q && kv_lens && k_strides && v_strides && k_cache_strides && v_cache_strides &&
+                 ((k_cache && v_cache) || num_pages == 0) && (page_table || max_pages == 0),
              AK_ERR_ARG, "null pointer");
   AK_REQUIRE(!q || (q_out && q_strides && q_out_strides), AK_ERR_ARG, "q without q_out");
   AppendArgs a{};

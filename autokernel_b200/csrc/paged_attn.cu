@@ -129,8 +129,10 @@ static bool tc_ok(const AttnArgs& a) {
     if (!ok(cache[i], a.kcs[i]) || !ok(cache[i], a.vcs[i])) return false;
   for (int i = 0; i < 2; ++i)
     if (!ok(tokens[i], a.qs[i]) || !ok(tokens[i], a.os[i])) return false;
+  // (the line of lists that give every sequence all tokens fits too)
   const double keys = (double)a.l.max_pages * a.l.page_size;
-  if (((double)a.l.N * a.G + a.l.B) * a.Hkv * ((keys < 2147483647.0 ? keys : 2147483647.0) + 1024) > 4e18)
+  if (((double)a.l.N * a.G + 1) * a.l.B * a.Hkv *
+          ((keys < 2147483647.0 ? keys : 2147483647.0) + a.l.N + 1024) > 4e18)
     return false;
   return device_info().cc_major == 10;
 }
@@ -167,8 +169,8 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
   AK_REQUIRE(sm_scale > 0.f && sm_scale <= 3.0e38f, AK_ERR_ARG,
              "sm_scale must be positive and finite");
   if (N == 0 || B == 0) return AK_OK;
-  AK_REQUIRE(q && k_cache && v_cache && out && page_table && cu_q && kv_lens && q_strides &&
-                 out_strides && k_cache_strides && v_cache_strides,
+  AK_REQUIRE(q && out && cu_q && kv_lens && q_strides && out_strides && k_cache_strides && v_cache_strides &&
+                 ((k_cache && v_cache) || num_pages == 0) && (page_table || max_pages == 0),
              AK_ERR_ARG, "null pointer");
   const size_t need = ak_paged_attention_workspace_size(N, B, H, Hkv, D, dtype);
   AK_REQUIRE(need == 0 || (workspace && aligned16(workspace) && ws_bytes >= need), AK_ERR_ARG,

@@ -94,6 +94,14 @@ AK_D void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
 }
 
 AK_D void group_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
+AK_D bool group_all(bool x) {  // of all consumer warps
+  int y;
+  asm volatile("{.reg .pred p, q;\nsetp.ne.s32 p, %1, 0;\nbar.red.and.pred q, 1, %2, p;\nselp.s32 %0, 1, 0, q;}"
+               : "=r"(y)
+               : "r"((int)x), "n"(32 * kWarps)
+               : "memory");
+  return y;
+}
 
 template <int DT, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -263,9 +271,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 4; ++i)
           q[kk][i] = __ldg(reinterpret_cast<const unsigned int*>(qrow[i & 1] + kk * 16 + cq + (i >> 1) * 8));
     };
-    bool ok = true;
     const Posted* now = segment(0);
-    if (now) load_q(now->s);
+    bool ok = group_all(now != nullptr);  // all of them meet in the loop, or none
+    if (ok) load_q(now->s);
     for (int n_seg = 0; ok && now; ++n_seg) {
       const Segment& s = now->s;
       const int row0 = s.tile * kRows;

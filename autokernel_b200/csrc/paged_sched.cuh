@@ -218,7 +218,7 @@ AK_D Line find_piece(const AttnArgs& a, const TileRule& t, int piece) {
     return line;
   }
   int64_t v = first, run = 0;
-  for (int64_t base = 0;; base += blockDim.x) {
+  for (int64_t base = 0; base < a.l.B; base += blockDim.x) {
     if (base) {
       int64_t all;
       v = cost_of(base + threadIdx.x);
@@ -236,10 +236,13 @@ AK_D Line find_piece(const AttnArgs& a, const TileRule& t, int piece) {
       s_b = (int)(base + threadIdx.x);
       s_at = at;
     }
-    if (__syncthreads_or(mine)) break;
+    if (__syncthreads_or(mine)) {
+      line.b = s_b;
+      line.b_at = s_at;
+      return line;
+    }
   }
-  line.b = s_b;
-  line.b_at = s_at;
+  line.x = -1;  // (not reached while nobody writes the lists)
   return line;
 }
 

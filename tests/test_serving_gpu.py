@@ -572,3 +572,57 @@ def test_attention_chunks_long_line(D, dt):
     check_attention(b, q, o)
     for _ in range(5):
         assert torch.equal(attend(b, 8, q=q)[1], o)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("pages", [0, 4])
+def test_no_pages_at_all(dt, new, pages):
+    """Tables without a column over pools with and without pages: keys are missing, not stored and NaN."""
+    b = Batch(dt, [(new, 0), (new, new)], 2, 64, 16, seed=22, spare=4)
+    b.kc, b.vc = b.kc[:pages], b.vc[:pages]
+    b.table = torch.empty(2, 0, dtype=torch.int32, device=DEV)
+    q, o = attend(b, 4)
+    assert (o[:new] == 0).all() and o[new:].isnan().all()
+    k, v = b.normal(b.N, 2, 64), b.normal(b.N, 2, 64)
+    cos, sin = tables(8, 64)
+    check_append(b, k, v, q, cos, sin, lambda: ops.paged_append(k, v, b.kc, b.vc, *b.lists(), q=q, cos=cos, sin=sin))
+
+
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_over_a_shared_table(dt, new):
+    """Sequences that read the same pages: one row of page numbers for all of them."""
+    b = Batch(dt, [(new, 150), (new, 150), (new, 90)], 2, 64, 16, seed=23)
+    b.table = b.table[:1].expand(3, -1)
+    assert b.table.stride(0) == 0
+    q, o = attend(b, 4)
+    check_attention(b, q, o)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("new", [1, 70])
+def test_attention_rows_before_the_first_sequence_stay(dt, new):
+    b = Batch(dt, [(new, 100), (0, 7), (new, new)], 2, 128, 16, seed=24, rows_behind=5)
+    b.cu += 3
+    out = torch.full((b.N, 4, 128), 3.0, device=DEV, dtype=b.dt)
+    q, o = attend(b, 4, out=out)
+    check_attention(b, q, o)
+    assert (o[:3] == 3).all() and (o[3 + 2 * new:] == 3).all()
+
+
+def test_attention_long_line_in_a_graph():
+    """A captured call follows the lists as they are when it is replayed."""
+    b = Batch("bf16", [(1, 40000), (1, 7), (1, 45000)], 8, 128, 64, seed=25)
+    q = b.normal(b.N, 16, 128)
+    attend(b, 16, q=q)
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(q)
+    with torch.cuda.graph(graph):
+        ops.paged_attention(q, b.kc, b.vc, *b.lists(), out=out)
+    for lens in ([40000, 7, 45000], [3, 5, 1], [39000, 1, 2000]):
+        b.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(b, q, out)
+        assert torch.equal(out, attend(b, 16, q=q)[1])
