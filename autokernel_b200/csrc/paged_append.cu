@@ -9,6 +9,10 @@
 // a thread owns one 16-byte vector of the head dimension and walks the heads, so a thread's cos
 // and sin are loaded once for all of them, and the data loads, which need nothing but the token's
 // number, are in flight while the token's sequence and page are looked up.
+//
+// Measured, 32 + 2 x 32 heads of 128, bf16: 12,750 tokens in 108 us, 5.9 TB/s (90% of a plain copy's
+// rate; 129 us before k, v and q had loops of their own, which leaves 64 registers and four CTAs per
+// SM); one token 4.1 us, a launch and the dependent loads of its place.
 #include "paged.cuh"
 
 #include <type_traits>

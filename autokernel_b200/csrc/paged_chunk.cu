@@ -19,6 +19,13 @@
 // and output of their own, and tile 0's threads join the two in the epilogue (a warp reads the
 // TMEM lanes of its quarter of either tile).
 //
+// Measured: two prompts of 4096 and 3700 tokens, 32 heads of 128, bf16, pages of 64: 370 us, 674 TFLOP/s (the
+// tensor pipe busy 34% of the time: a block's softmax takes longer than its two products, and a
+// segment's start and end, which nothing overlaps, cost about 9 us).  501 tokens on 7600 keys, 32
+// heads over 8: 99 us, 649 TFLOP/s.  24 sequences of up to 96 tokens on up to 1500 keys, 12 heads of
+// 64: 60 us, where reading the keys alone would take 10: 288 tiles of a few blocks each, whose starts
+// and ends bound it.
+//
 // P is rounded to 16 bits once, as the matrix unit takes it; maximum, sum and output are fp32.
 // Slots of the last page behind the last visible key may hold anything, NaN included: the
 // producer zeroes their V rows before the matrix unit sees them (their scores are masked).

@@ -38,6 +38,7 @@ from dataclasses import dataclass
 import torch
 
 from . import ops, shard
+from ._lib import AkError
 from .paged import Batch, PagedCache
 
 
@@ -284,9 +285,13 @@ class LlamaB200:
         """Continue each prompt (token lists, at least one token each) by up to max_new_tokens sampled
         tokens (ops.sample's settings; temperature 0 takes the likeliest).  A sequence ends with the
         token `stop`, if given.  All sequences decode together; with `cache` they share its pages and
-        give them back at the end, otherwise one of the right size is made."""
+        give them back at the end, otherwise one of the right size is made.  Raises AkError when a
+        step's logits hold nothing to draw (all NaN)."""
         if not prompts or min(len(p) for p in prompts) < 1 or max_new_tokens < 0:
             raise ValueError("generate: need prompts of at least one token")
+        vocab = self.w["tok_embeddings.weight"].shape[0]
+        if not all(0 <= t < vocab for p in prompts for t in p):
+            raise ValueError(f"generate: tokens must lie in [0, {vocab})")
         if max_new_tokens == 0:
             return [[] for _ in prompts]
         device = self.w["tok_embeddings.weight"].device
@@ -305,6 +310,7 @@ class LlamaB200:
                 u = torch.rand(len(live), device=device, generator=generator)
                 tokens = ops.sample(logits, u, temperature, top_k, top_p, min_p)
                 steps.append((live, tokens))
+                tokens = tokens.clamp(min=0)  # -1: nothing to draw, found when the answers are read
                 if stop is not None:
                     on = (tokens != stop).tolist()
                     tokens = tokens[torch.tensor(on, device=device)]
@@ -318,6 +324,8 @@ class LlamaB200:
         out: list[list[int]] = [[] for _ in prompts]
         for rows, t in steps:
             for i, x in zip(rows, t.tolist()):
+                if x < 0:
+                    raise AkError(f"generate: sequence {i} has no logits to draw from")
                 out[i].append(x)
         return out
 

@@ -157,6 +157,21 @@ def test_generate():
 
 
 @pytest.mark.gpu
+def test_generate_refuses_what_it_cannot_embed():
+    m = _model(torch.float16)
+    vocab = m.w["tok_embeddings.weight"].shape[0]
+    for bad in ([[vocab]], [[1, 2], [-1]]):
+        with pytest.raises(ValueError, match="tokens"):
+            m.generate(bad, 2)
+    m.w["output.weight"] = torch.full_like(m.w["output.weight"], float("nan"))
+    cache = m.new_cache(4, 16)
+    for stop in (None, 0):
+        with pytest.raises(AkError, match="draw"):
+            m.generate([[1, 2], [3]], 3, stop=stop, cache=cache)
+        assert cache.free_pages == 4
+
+
+@pytest.mark.gpu
 def test_decoding_step_in_a_graph():
     """A captured decoding step (append, attention, sampling) replayed with other lists, tokens and
     numbers gives what eager calls give; a padded row of the batch stays as it was."""
