@@ -494,23 +494,25 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int prow = x * BQ + row;
       float odd = 0.f;  // NaN once a result is not finite
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
+      for (int c = 0; c < D / 8; ++c) {
+        uint32_t r[8];
         __syncwarp();
         if (took[x]) {
-          tmem_ld32(t_o + c * 32, r);
-          tmem_wait_ld();
-          tmem_regs_ready(r);
+          tmem_ld8(t_o + c * 8, r);
           if (split) {
-            uint32_t r1[32];
-            tmem_ld32(t_o + C::TMEM_TILE + c * 32, r1);
+            uint32_t r1[8];
+            tmem_ld8(t_o + C::TMEM_TILE + c * 8, r1);
             tmem_wait_ld();
-            tmem_regs_ready(r1);
+            tmem_regs_ready8(r);
+            tmem_regs_ready8(r1);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
+            for (int i = 0; i < 8; ++i)
               r[i] = __float_as_uint(__uint_as_float(r[i]) * f0 + __uint_as_float(r1[i]) * f1);
+          } else {
+            tmem_wait_ld();
+            tmem_regs_ready8(r);
           }
-          if (c == D / 32 - 1) {  // O has been read
+          if (c == D / 8 - 1) {  // O has been read
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -520,24 +522,21 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0;
+          for (int i = 0; i < 8; ++i) r[i] = 0;
         }
         if (s.whole) {
+          uint32_t e[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t e[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float y0 = __uint_as_float(r[q * 8 + 2 * i]) * inv, y1 = __uint_as_float(r[q * 8 + 2 * i + 1]) * inv;
-              odd = fmaf(y0, 0.f, fmaf(y1, 0.f, odd));
-              e[i] = attn_sm::pack2<DT>(y0, y1);
-            }
-            if (valid) reinterpret_cast<uint4*>(orow + c * 32)[q] = make_uint4(e[0], e[1], e[2], e[3]);
+          for (int i = 0; i < 4; ++i) {
+            const float y0 = __uint_as_float(r[2 * i]) * inv, y1 = __uint_as_float(r[2 * i + 1]) * inv;
+            odd = fmaf(y0, 0.f, fmaf(y1, 0.f, odd));
+            e[i] = attn_sm::pack2<DT>(y0, y1);
           }
+          if (valid) reinterpret_cast<uint4*>(orow)[c] = make_uint4(e[0], e[1], e[2], e[3]);
         } else if (valid) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            __stcg(reinterpret_cast<uint4*>(part) + (c * 8 + q) * ROWS + prow,
+          for (int q = 0; q < 2; ++q)
+            __stcg(reinterpret_cast<uint4*>(part) + (c * 2 + q) * ROWS + prow,
                    make_uint4(r[q * 4], r[q * 4 + 1], r[q * 4 + 2], r[q * 4 + 3]));
         }
       }
