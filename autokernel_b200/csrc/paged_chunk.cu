@@ -19,12 +19,13 @@
 // and output of their own, and tile 0's threads join the two in the epilogue (a warp reads the
 // TMEM lanes of its quarter of either tile).
 //
-// Measured: two prompts of 4096 and 3700 tokens, 32 heads of 128, bf16, pages of 64: 370 us, 674 TFLOP/s (the
-// tensor pipe busy 34% of the time: a block's softmax takes longer than its two products, and a
-// segment's start and end, which nothing overlaps, cost about 9 us).  501 tokens on 7600 keys, 32
-// heads over 8: 99 us, 649 TFLOP/s.  24 sequences of up to 96 tokens on up to 1500 keys, 12 heads of
-// 64: 60 us, where reading the keys alone would take 10: 288 tiles of a few blocks each, whose starts
-// and ends bound it.
+// Measured: two prompts of 4096 and 3700 tokens, 32 heads of 128, bf16, pages of 64: 350 us, 714 TFLOP/s (a
+// block's softmax takes longer than its two products, and a segment's start and end, which nothing
+// overlaps, cost several us).  501 tokens on 7600 keys, 32 heads over 8: 91 us, 705 TFLOP/s.  24
+// sequences of up to 96 tokens on up to 1500 keys, 12 heads of 64: 56 us, where reading the keys
+// alone would take 10: 288 tiles of a few blocks each, whose starts and ends bound it.  What runs once
+// per segment or block row (masks, the epilogue) is kept short: its instructions are not at hand when
+// their turn comes (masks and epilogue unrolled over a row's registers: 380 us, 99 us and 60 us).
 //
 // P is rounded to 16 bits once, as the matrix unit takes it; maximum, sum and output are fp32.
 // Slots of the last page behind the last visible key may hold anything, NaN included: the
@@ -372,7 +373,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       int vis;  // keys that this thread's row sees; what else is known of the row is looked up again in
       {         // the epilogue: the loop needs every register
         const int tok = post->s.t_lo + (post->split ? 0 : x) * p.tt + row / a.G;
-        vis = row < p.tt * a.G && tok < post->s.t_hi ? visible_keys(post->s.r, tok, a.causal) : 0;
+        // (a row of no token sees all: what it computes goes nowhere, and it masks nothing)
+        vis = row < p.tt * a.G && tok < post->s.t_hi ? visible_keys(post->s.r, tok, a.causal) : 0x7fffffff;
       }
       float m_ref = -INFINITY, l = 0.f;
       const int step = post->step, end = post->end[x];
@@ -381,17 +383,27 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
         tc_fence_after();
         const int kmax = vis - j * BKV;  // keys below this are visible to the row
+        if (!__all_sync(0xffffffffu, kmax >= BKV)) {  // few blocks: masked in TMEM, where code is short
+#pragma unroll 1
+          for (int c = 0; c < BKV; c += 8) {
+            if (__all_sync(0xffffffffu, kmax >= c + 8)) continue;
+            uint32_t y[8];
+            tmem_ld8(t_s + c, y);
+            tmem_wait_ld();
+            tmem_regs_ready8(y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c + i >= kmax) y[i] = __float_as_uint(-INFINITY);
+            tmem_st8(t_s + c, y);
+          }
+          tmem_wait_st();
+        }
         uint32_t r[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, r + c * 32);
         tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_regs_ready(r + c * 32);
-        if (!__all_sync(0xffffffffu, kmax >= BKV)) {
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i >= kmax) r[i] = __float_as_uint(-INFINITY);
-        }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 128; i += 8)
