@@ -22,6 +22,36 @@ AK_D int visible_keys(const SeqRange& r, int i, int causal) {
   return causal ? max(r.kv_len - r.n + i + 1, 0) : r.kv_len;
 }
 
+// Weights P = exp2(score scale log2e - r), of which the matrix units take 16 bits, against a reference r of
+// their row that cancels in O / l.  r moves when a block's largest score passes it by more than
+// kShift + kLag, and is then put kShift below that score, so the largest weight so far is at least
+// 2^kShift and at most 2^(kShift + kLag).  bf16 has the exponents of fp32: no shift.  fp16 weights
+// are kept at the top of its range, where 2^15 is the largest power: below 2^-14 they lose bits
+// (2^-25 each), so a weight under 2^-(14 + kShift) of its row's largest is off by up to
+// 2^-(25 + kShift) of that (20,000 keys 26 below a key whose value is 0 lost 1.3% of their output
+// without the shift).  A smaller lag leaves more room and moves r, and with it O, more often: prompts
+// of 4096 + 3700 tokens, 32 heads of 128, take 354 us with a lag of 8 or 4, 373 with 2 and 387
+// with 0; with scores four times as wide 373, 382, 384 and 387.
+template <int DT>
+struct Weight {
+  static constexpr float kShift = DT == AK_F16 ? 11.f : 0.f;
+  static constexpr float kLag = DT == AK_F16 ? 4.f : 8.f;
+  // Scores are fp32, and so is r.  From 2^23 on its steps are 1 and more: fp16 scores are rounded up to
+  // it, so that no weight passes 2^15, and up to kLimit the largest one is at least 1 (in bf16,
+  // between 2^-64 and 2^72).  A row whose largest score lies beyond is NaN: its weights would be
+  // infinite or all 0, and its scores have lost what tells them apart.
+  static constexpr float kLimit = DT == AK_F16 ? 134217728.f : 2147483648.f;  // 2^27, 2^31
+  // the largest score of a block, scaled
+  static AK_D float top(float score, float scale_log2) {
+    return DT == AK_F16 ? __fmul_ru(score, scale_log2) : __fmul_rn(score, scale_log2);
+  }
+  // whether a block with this top moves r, and where to (r = -inf: nothing has been seen yet)
+  static AK_D bool moves(float top, float r) { return top - r > kShift + kLag; }
+  static AK_D float reference(float top) {
+    return fabsf(top) < kLimit ? __fsub_ru(top, kShift) : __int_as_float(0x7fffffff);
+  }
+};
+
 // paged_decode.cu: 16 query rows per tile, all keys read once; paged_chunk.cu: 128-row tensor-core tiles.
 int run_decode(const AttnArgs& a, void* ws, cudaStream_t st);
 size_t decode_workspace(int D);

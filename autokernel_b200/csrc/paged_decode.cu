@@ -11,7 +11,7 @@
 //               that HBM needs, and a table load per block cost it 2000 (the batch below took 309 us
 //               so; 235 with four producers that fetch 32 page numbers at a time)
 //   warps 4..11 two groups of four take alternate blocks, a warp 16 keys of its block, each with
-//               its own running maximum, sum and output, joined through shared memory per segment
+//               its own reference (Weight), sum and output, joined through shared memory per segment
 // One CTA per SM; the line of paged_sched.cuh gives each the same number of keys.
 //
 // Measured: 64 sequences of 300 to 8100 keys, 32 heads over 8 of 128, fp16, pages of 16: 202 us, 5.45 TB/s
@@ -19,8 +19,9 @@
 // alone would take 5: the rest is latency, of the launch, of the lists and page numbers before the
 // first copy can leave (2 us), of one ring fill and two joins per CTA and of the joining kernel (2 us).
 //
-// P = exp2(S scale log2e - m) is split into two 16-bit terms for P V (P = hi + lo, 16 bits of P kept):
-// the matrix units have time to spare here, and it leaves one rounding, that of the result.
+// The weights P (Weight) are split into two 16-bit terms for P V, P = hi + lo: the matrix units have
+// time to spare here.  In bf16 that keeps 16 bits of every P; in fp16 22, or what lies above 2^-25,
+// where P's largest is 2^11 at least.  What is left is the rounding of the result.
 #include "paged_sched.cuh"
 #include "sm100.cuh"
 
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 4; ++j)
               if (key0 + n * 8 + cq + (j & 1) >= vis[j >> 1]) sc[n][j] = -INFINITY;
         }
-        // running maximum, moved only when a block raises it by more than 8 (log2)
+        // m: the reference of the weights (Weight)
         float alpha[2];
         bool move = false;
 #pragma unroll
@@ -333,9 +334,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           float x = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          x *= a.scale_log2;
+          x = Weight<DT>::top(x, a.scale_log2);
           alpha[i] = 1.f;
-          if (x > m[i] + 8.f) {
+          if (Weight<DT>::moves(x, m[i])) {
+            x = Weight<DT>::reference(x);
             alpha[i] = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - x);
             m[i] = x;
             move = true;

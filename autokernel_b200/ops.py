@@ -726,8 +726,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     Returns [N, H, D] (written to out if given: any strides with a contiguous last dim, and none of
     the inputs' memory).  A row that sees no key (or only scores of -inf) is 0; one that sees a key
-    without a page is NaN.  Rows behind cu_q[B] are left alone (a fresh result is not initialised
-    there).  Nothing behind a sequence's last key matters, whatever the cache holds there."""
+    without a page is NaN, and in 16-bit types one whose largest score (scaled) is 9.3e7 (fp16) or 1.5e9
+    (bf16) or more in size may be: no 16-bit weights reach from there.  Rows behind cu_q[B] are left
+    alone (a fresh result is not initialised there).  Nothing behind a sequence's last key matters, whatever the cache holds there."""
     name = "paged_attention"
     (P, Hkv, S, D), kcs, vcs, dt, B, width, ld = _paged_cache(name, k_cache, v_cache, page_table, cu_q, kv_lens)
     (N, H, _), qs = _tokens(name, "q", q, None, None, D, dt)

@@ -290,7 +290,9 @@ AK_API int ak_paged_append(const void* k, const void* v, const void* q, void* q_
 
 /* out[t, h] = softmax(q[t, h] . K^T * sm_scale) V over the keys that token t sees: all up to its
  * position (causal) or all kv_lens[b].  Query head h reads key/value head h / (H / Hkv).  A row
- * that sees no key (or only scores of -inf) is 0; a row that sees a key without a page is NaN.
+ * that sees no key (or only scores of -inf) is 0; a row that sees a key without a page is NaN, and so may
+ * be, in 16-bit types, one whose largest score times sm_scale log2(e) is 2^27 (fp16) or 2^31 (bf16)
+ * or more in size: no 16-bit weights reach from there.
  * What the cache holds behind a sequence's last key never matters.  D <= 256, sm_scale > 0.
  * workspace: ak_paged_attention_workspace_size bytes, used by this call alone until it is done. */
 AK_API size_t ak_paged_attention_workspace_size(int64_t N, int64_t B, int64_t H, int64_t Hkv,

@@ -1,0 +1,96 @@
+"""The serving operators where their arithmetic is at its limits: bounds as in test_serving_gpu.py (h = half
+a step of the output type, relative), with what fp16 cannot hold counted:
+
+  attention  fp16 weights P lie at the top of the type's range, the largest so far at least 2^11: one below
+             2^-14 is off by at most 2^-25, which is 2^-36 of the row's largest weight.  Decoding splits P
+             in two terms, so there only that and 2^-22 (bf16: 2^-17) of the weight itself remain.  fp16
+             results below 2^-14 are off by 2^-25.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from autokernel_b200 import ops
+from autokernel_b200._lib import device_status
+
+pytestmark = pytest.mark.gpu
+
+DTS = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+DEV = "cuda"
+I32 = torch.int32
+
+
+def _half(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def one_sequence(k, v, new, length):
+    """A cache [1, length, D] (keys, values) in pages of 16 in order, and the lists of `new` tokens."""
+    page, D = 16, k.shape[-1]
+    P = -(-length // page)
+    kc, vc = (torch.zeros(P * page, D, device=DEV, dtype=x.dtype) for x in (k, v))
+    kc[:length], vc[:length] = k, v
+    lists = (torch.arange(P, dtype=I32, device=DEV)[None], torch.tensor([0, new], dtype=I32, device=DEV),
+             torch.tensor([length], dtype=I32, device=DEV))
+    return kc.view(P, 1, page, D), vc.view(P, 1, page, D), lists
+
+
+@pytest.mark.parametrize("gap", [8, 20, 24, 26])
+@pytest.mark.parametrize("new", [1, 40, 300])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_weak_keys_beside_leading_ones_without_value(dt, D, new, gap):
+    """Every 16th key leads the others by `gap` (log2) and has the value 0: the output is the others' alone."""
+    dt, L = DTS[dt], 500
+    g = torch.Generator(DEV).manual_seed(gap)
+    k = torch.zeros(L, D, device=DEV)
+    k[:, 0] = torch.rand(L, device=DEV, generator=g)
+    v = 64 + 64 * torch.rand(L, D, device=DEV, generator=g)
+    k[::16, 0], v[::16] = gap + 1, 0
+    k, v = k.to(dt), v.to(dt)
+    q = torch.zeros(new, 2, D, device=DEV, dtype=dt)
+    q[..., 0] = 1
+    kc, vc, lists = one_sequence(k, v, new, L)
+    o = ops.paged_attention(q, kc, vc, *lists, causal=False, sm_scale=math.log(2)).double()
+    w = torch.exp2(k[:, 0].double() - (gap + 1))
+    w = w / w.max()
+    e, A = (w @ v.double()) / w.sum(), (w @ v.double().abs()) / w.sum()
+    floor = (v.double().abs().sum(0) / w.sum()) * (2.0 ** -36 if dt == torch.float16 else 0)
+    h = _half(dt)
+    hp = h if new > 1 else 2.0 ** -22 if dt == torch.float16 else 2.0 ** -17
+    d = (D + 8) * 2.0 ** -24 * (gap + 1) + 2.0 ** -20
+    tol = torch.clamp(h * e, min=2.0 ** -25 if dt == torch.float16 else 0) + (hp + 2 * d + (L + 8) * 2.0 ** -23) * A + floor
+    err = (o - e).abs()
+    assert (err <= tol).all(), (float((err / e).max()), float((tol / e).min()))
+
+
+@pytest.mark.parametrize("dt", list(DTS))
+@pytest.mark.parametrize("mag", [1e3, 5e3, 2e4, 5e4])
+@pytest.mark.parametrize("new", [1, 300])
+def test_scores_whose_steps_are_large(dt, mag, new):
+    """Scores up to 1e10, whose fp32 steps are 1 and more: which key wins is a matter of rounding, but a row stays a
+    mean of the values, or is NaN where its largest score (scaled, log2) is beyond 2^27 (fp16) or 2^31
+    (bf16): no 16-bit weights reach from there.  fp32 has no such border."""
+    dt, L, D = DTS[dt], 310, 64
+    g = torch.Generator(DEV).manual_seed(2)
+    k, q = ((torch.randn(n, D, device=DEV, generator=g) * mag).clamp(-6e4, 6e4).to(dt) for n in (L, new * 2))
+    v = torch.randn(L, D, device=DEV, generator=g).to(dt)
+    kc, vc, lists = one_sequence(k, v, new, L)
+    o = ops.paged_attention(q.view(new, 2, D), kc, vc, *lists).double()
+    score = (q.double() @ k.double().T).view(new, 2, L) * D ** -0.5 / math.log(2)
+    hidden = torch.arange(L, device=DEV) > torch.arange(L - new, L, device=DEV)[:, None, None]
+    top = score.masked_fill(hidden, -math.inf).amax(-1).abs()
+    limit = {torch.float16: 2.0 ** 27, torch.bfloat16: 2.0 ** 31, torch.float32: math.inf}[dt]
+    near = (D + 8) * 2.0 ** -24 * (q.double().abs() @ k.double().abs().T).amax(-1).view(new, 2) * D ** -0.5 / math.log(2)
+    inside, beyond = top + near < limit, top - near > limit
+    assert o[inside].isfinite().all() and o[beyond].isnan().all()
+    if mag == 1e3:
+        assert inside.all()
+    # weights sum to 1 but for their rounding (h) and that of the sums
+    most = v.double().abs().amax(0) * (1 + 2 * _half(dt) + 2 * (L + 8) * 2.0 ** -23)
+    assert ((o.abs() <= most) | o.isnan()).all()
+    assert device_status() == 0
