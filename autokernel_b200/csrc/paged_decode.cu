@@ -425,14 +425,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (row >= nr) continue;
           const float m1 = s_m[w4][row], mn = fmaxf(m[i], m1), ref = mn == -INFINITY ? 0.f : mn;
           const float f0 = ex2_approx(m[i] - ref), f1 = ex2_approx(m1 - ref);
-          l[i] = l[i] * f0 + s_l[w4][row] * f1;
+          // Which group has the even blocks hangs on the pieces its CTA took before, so the two change places
+          // from call to call: products and sum are rounded apart, which gives the same bits either way.
+          l[i] = __fadd_rn(__fmul_rn(l[i], f0), __fmul_rn(s_l[w4][row], f1));
           m[i] = mn;
 #pragma unroll
           for (int n = 0; n < NF; ++n) {
             const float2 x = *reinterpret_cast<const float2*>(s_o + (w4 * kRows + row) * D +
                                                               ((n * 8 + cq) ^ ((row & 7) * 8)));
-            o[n][2 * i] = o[n][2 * i] * f0 + x.x * f1;
-            o[n][2 * i + 1] = o[n][2 * i + 1] * f0 + x.y * f1;
+            o[n][2 * i] = __fadd_rn(__fmul_rn(o[n][2 * i], f0), __fmul_rn(x.x, f1));
+            o[n][2 * i + 1] = __fadd_rn(__fmul_rn(o[n][2 * i + 1], f0), __fmul_rn(x.y, f1));
           }
         }
         __syncwarp();  // a row's four lanes have read its m and l

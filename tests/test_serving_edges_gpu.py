@@ -94,3 +94,24 @@ def test_scores_whose_steps_are_large(dt, mag, new):
     most = v.double().abs().amax(0) * (1 + 2 * _half(dt) + 2 * (L + 8) * 2.0 ** -23)
     assert ((o.abs() <= most) | o.isnan()).all()
     assert device_status() == 0
+
+
+@pytest.mark.parametrize("dt,D", [("f16", 128), ("bf16", 64)])
+@pytest.mark.parametrize("seqs,heads,kv", [([(1, 3000), (3, 900)] + 6 * [(1, 1500)], 600, 300),
+                                           ([(1, 300 + 119 * i) for i in range(64)], 32, 8)])
+def test_decoding_gives_the_same_bits_every_time(seqs, heads, kv, D, dt):
+    """CTAs take pieces of a long line as they become free: which one took which does not show in the result."""
+    seqs = seqs + [(0, 0)] * (sum(s[0] for s in seqs) - len(seqs))
+    g = torch.Generator(DEV).manual_seed(3)
+    page = 16
+    used = [-(-s[1] // page) for s in seqs]
+    table = torch.full((len(seqs), max(used)), -1, dtype=I32)
+    for b, n in enumerate(used):
+        table[b, :n] = torch.arange(sum(used[:b]), sum(used[:b]) + n)
+    cu = torch.tensor([sum(s[0] for s in seqs[:i]) for i in range(len(seqs) + 1)], dtype=I32, device=DEV)
+    lists = (table.to(DEV), cu, torch.tensor([s[1] for s in seqs], dtype=I32, device=DEV))
+    kc, vc = (torch.randn(sum(used), kv, page, D, device=DEV, dtype=DTS[dt], generator=g) for _ in range(2))
+    q = torch.randn(int(cu[-1]), heads, D, device=DEV, dtype=DTS[dt], generator=g)
+    first = ops.paged_attention(q, kc, vc, *lists)
+    for _ in range(20):
+        assert torch.equal(ops.paged_attention(q, kc, vc, *lists), first)
