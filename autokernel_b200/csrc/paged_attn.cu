@@ -4,102 +4,27 @@
 //   o[t, h] = sum_{j < vis(t)} softmax_j(scale q[t, h] . K[j, h / G]) V[j, h / G],  G = H / Hkv,
 //   vis(t) = position(t) + 1 (causal) or kv_lens[b].
 // A row that sees no key is 0.  A row that would see a key without a page (paged.cuh) is NaN.
-#include "paged_attn.cuh"
+#include "paged_row.cuh"
 
 namespace ak {
 namespace paged {
 
-// One CTA per (token, head): 32 groups of eight lanes each take every 32nd key with a running
-// maximum and sum of their own, and are joined through shared memory at the end, so nothing is
-// exchanged while keys are read.  The eight lanes split the head dimension (element
-// lane + 8 i), which coalesces to whole 32-byte sectors in fp32 at any alignment.
+// One CTA per (token, head).
 template <int DT, int NI>
 __global__ void __launch_bounds__(256) simt_kernel(const AttnArgs a) {
-  using E = Elem<DT>;
-  using T = typename E::T;
-  const int t = blockIdx.x, h = blockIdx.y, hk = h / a.G;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int sub = lane & 7, grp = threadIdx.x >> 3;
+  const int t = blockIdx.x;
   __shared__ int s_seq;
-  if (warp == 0) {
+  __shared__ RowScratch<NI, 256> scratch;
+  if (threadIdx.x < 32) {
     const int b = seq_of_token_warp(a.l, t);
-    if (lane == 0) s_seq = b;
+    if (threadIdx.x == 0) s_seq = b;
   }
   __syncthreads();
   const int b = s_seq;
   if (b < 0 || b >= a.l.B) return;
   const SeqRange r = seq_range(a.l, b);
   if (t < r.begin || t >= r.begin + r.n) return;
-  const int vis = visible_keys(r, t - r.begin, a.causal);
-
-  float q[NI], o[NI];
-  const T* qp = reinterpret_cast<const T*>(a.q) + t * a.qs[0] + h * a.qs[1];
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int d = sub + 8 * i;
-    q[i] = d < a.D ? E::to_f(qp[d]) : 0.f;
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, sum = 0.f;
-  bool missing = false;
-  for (int j = grp; j < vis; j += 32) {
-    const int pi = j / a.l.page_size, slot = j - pi * a.l.page_size;
-    const int page = page_of(a.l, b, pi);
-    if (page < 0) {
-      missing = true;
-      break;
-    }
-    const T* kp = reinterpret_cast<const T*>(a.k) + page * a.kcs[0] + hk * a.kcs[1] + slot * a.kcs[2];
-    const T* vp = reinterpret_cast<const T*>(a.v) + page * a.vcs[0] + hk * a.vcs[1] + slot * a.vcs[2];
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int d = sub + 8 * i;
-      if (d < a.D) s = fmaf(q[i], E::to_f(kp[d]), s);
-    }
-    const unsigned mask = 0xffu << (lane & 24);
-#pragma unroll
-    for (int x = 4; x > 0; x >>= 1) s += __shfl_xor_sync(mask, s, x);
-    const float mn = fmaxf(m, s);
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    const float alpha = exp2f((m - ref) * a.scale_log2), p = exp2f((s - ref) * a.scale_log2);
-    m = mn;
-    sum = sum * alpha + p;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int d = sub + 8 * i;
-      if (d < a.D) o[i] = fmaf(p, E::to_f(vp[d]), o[i] * alpha);
-    }
-  }
-  missing = __syncthreads_or(missing);
-
-  // join the 32 groups
-  __shared__ float s_m[32], s_l[32];
-  __shared__ float s_o[8][8 * NI];
-  if (sub == 0) {
-    s_m[grp] = m;
-    s_l[grp] = sum;
-  }
-  __syncthreads();
-  const float top = warp_max(s_m[lane]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  const float total = warp_sum(s_l[lane] * exp2f((s_m[lane] - ref) * a.scale_log2));
-  const float w = exp2f((m - ref) * a.scale_log2);
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    float x = o[i] * w;
-    x += __shfl_xor_sync(0xffffffffu, x, 8);
-    x += __shfl_xor_sync(0xffffffffu, x, 16);
-    if (lane < 8) s_o[warp][sub + 8 * i] = x;
-  }
-  __syncthreads();
-  T* op = reinterpret_cast<T*>(a.o) + t * a.os[0] + h * a.os[1];
-  for (int d = threadIdx.x; d < a.D; d += blockDim.x) {
-    float x = 0.f;
-#pragma unroll
-    for (int y = 0; y < 8; ++y) x += s_o[y][d];
-    op[d] = E::from_f(missing ? __int_as_float(0x7fffffff) : total == 0.f ? 0.f : x / total);
-  }
+  row_by_cta<DT, NI, 256>(a, b, r, t - r.begin, blockIdx.y, scratch);
 }
 
 template <int DT>

@@ -66,6 +66,9 @@ struct Params {
   uint32_t idesc_qk, idesc_pv;
   float* ws;
   Cutting* cuts;  // one per piece, behind the parts
+  // Two per piece: whether rows of its whole items, and of the item that the boundary behind it cuts first, are
+  // to be looked at again.
+  int2* marks;
 };
 
 // A segment and what each tile does in it.  Tile x takes key blocks first[x], first[x] + step, ...
@@ -135,6 +138,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&post_empty[i], 10);  // the V producer, the MMA issuer and eight softmax warps
     }
     abort_flag = 0;
+    p.marks[blockIdx.x] = make_int2(0, 0);
     fence_mbar_init();
     tma_prefetch_desc(&tq);
     tma_prefetch_desc(&tk);
@@ -560,15 +564,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         part[ROWS * D + ROWS + prow] = l;
       }
       // rows whose result is not finite although their weights are, beside keys hidden from them
-      unsigned again = __ballot_sync(0xffffffffu, odd != 0.f && valid && fabsf(l) <= 3.4028235e38f && vis < s.kv_hi);
-      while (again) {
-        const int i = __ffs(again) - 1, rr = quarter * 32 + i;
-        again &= again - 1;
-        const int t = s.t_lo + x * p.tt + rr / a.G;
-        __syncwarp();
-        if (hidden_not_finite<DT>(a, s.b, s.h, visible_keys(s.r, t, a.causal), s.kv_hi))
-          row_by_key<DT>(a, s.b, s.r, t, s.h * a.G + rr % a.G);
-      }
+      if (odd != 0.f && valid && fabsf(l) <= 3.4028235e38f && vis < s.kv_hi) p.marks[blockIdx.x].x = 1;
       __syncwarp();
       if (lane == 0) mbar_arrive(&post_empty[n % POSTS]);
     }
@@ -591,8 +587,9 @@ __global__ void __launch_bounds__(128)
   using T = typename E::T;
   constexpr int V = D / 16;  // float4 of a row per thread
   __shared__ int s_slot[kParts];
-  __shared__ int s_whole, s_again;
-  if (threadIdx.x == 0) s_whole = s_again = 0;
+  __shared__ int s_whole;
+  if (threadIdx.x == 0) s_whole = 0;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Line line;
   wait_for_parts();
   const Parts parts = parts_of(a, p.rule, p.cuts[blockIdx.x], line);
@@ -658,15 +655,25 @@ __global__ void __launch_bounds__(128)
       reinterpret_cast<uint4*>(orow)[i / 2] = raw;
     }
   }
-  odd = odd && fabsf(sum) <= 3.4028235e38f && visible_keys(s.r, tok, a.causal) < s.kv_hi;
-  if (odd) atomicOr(&s_again, 1 << lane);
-  __syncthreads();
-  for (int i = part_d; i < 32 && s_again; i += 4) {
-    if (!(s_again >> i & 1)) continue;
-    const int rr = blockIdx.y * 32 + i - x * BQ, t = s.t_lo + x * p.tt + rr / a.G;
-    if (hidden_not_finite<DT>(a, s.b, s.h, visible_keys(s.r, t, a.causal), s.kv_hi))
-      row_by_key<DT>(a, s.b, s.r, t, s.h * a.G + rr % a.G);
-  }
+  if (odd && fabsf(sum) <= 3.4028235e38f && visible_keys(s.r, tok, a.causal) < s.kv_hi) p.marks[blockIdx.x].y = 1;
+}
+
+// Looks again at rows of the items that are marked, in a launch of its own: within the joining kernel that code,
+// although it hardly ever runs, cost a call 4 to 10 us; here 2, if it is a function that is called (8 inlined).
+template <int DT, int D>
+__device__ __noinline__ void look_again_at_items(const AttnArgs& a, const Params& p, int2 marked, AgainScratch<D>& sh) {
+  Parts parts;
+  Line line;
+  if (marked.y) parts = parts_of(a, p.rule, p.cuts[blockIdx.x], line);
+  look_again<DT, D>(a, p.rule, parts.s, marked.y, marked.x, blockIdx.x, blockIdx.y * 32, blockIdx.y * 32 + 32, sh);
+}
+template <int DT, int D>
+__global__ void __launch_bounds__(128)
+    chunk_again_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Params p) {
+  __shared__ AgainScratch<D> scratch;
+  wait_for_parts();
+  const int2 marked = __ldcg(p.marks + blockIdx.x);
+  if (marked.x || marked.y) look_again_at_items<DT, D>(a, p, marked, scratch);
 }
 
 template <int DT, int D>
@@ -680,6 +687,7 @@ static int launch(const AttnArgs& a, float* ws, cudaStream_t st) {
   p.idesc_pv = idesc_f16(fmt, BQ, D, false, true);
   p.ws = ws;
   p.cuts = reinterpret_cast<Cutting*>(ws + 2 * (size_t)device_info().sm_count * Cfg<D>::PART);
+  p.marks = reinterpret_cast<int2*>(p.cuts + device_info().sm_count);
   CUtensorMap tq, tk, tv;
   const uint64_t dims[3] = {(uint64_t)D, (uint64_t)a.H, (uint64_t)a.l.N};
   const uint64_t strides[2] = {(uint64_t)(a.H > 1 ? a.qs[1] : D) * 2,
@@ -694,14 +702,16 @@ static int launch(const AttnArgs& a, float* ws, cudaStream_t st) {
   const int pieces = p.rule.ctas;
   chunk_kernel<DT, D><<<pieces, THREADS, Cfg<D>::SMEM, st>>>(tq, tk, tv, a, p);
   const int rc = launch_status("paged_attention");
-  if (rc || pieces < 2) return rc;
-  return launch_after(chunk_join_kernel<DT, D>, dim3(pieces - 1, ROWS / 32), 128, st, a, p);
+  if (rc) return rc;
+  const int joined = pieces < 2 ? AK_OK : launch_after(chunk_join_kernel<DT, D>, dim3(pieces - 1, ROWS / 32), 128, st, a, p);
+  if (joined) return joined;
+  return launch_after(chunk_again_kernel<DT, D>, dim3(pieces, ROWS / 32), 128, st, a, p);
 }
 
 }  // namespace chunk
 
 size_t chunk_workspace(int D) {
-  return (size_t)device_info().sm_count * (2 * chunk::ROWS * (D + 2) * sizeof(float) + sizeof(Cutting));
+  return (size_t)device_info().sm_count * (2 * chunk::ROWS * (D + 2) * sizeof(float) + sizeof(Cutting) + sizeof(int2));
 }
 
 int run_chunk(const AttnArgs& a, void* ws, cudaStream_t st) {

@@ -127,7 +127,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int s_bad[C::STAGES];  // first key of the block without a page
   __shared__ float s_m[kWarps / 2][kRows], s_l[kWarps / 2][kRows];
   __shared__ int s_badw[kWarps];
-  __shared__ int s_again;           // rows to look at again (bits)
   __shared__ int abort_flag, s_stop;
   // Segments, from the first producer to all other warps: finding one takes about 1000 cycles, so it is
   // done once and ahead of time.  part < 0: there are no more.
@@ -153,7 +152,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty[i], 4);
     }
     abort_flag = 0;
-    s_again = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
@@ -161,6 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Line line = find_piece(a, rule, blockIdx.x);
   __syncthreads();
   volatile int* abort_p = &abort_flag;
+  int* const marks = reinterpret_cast<int*>(ws + 2 * (int64_t)gridDim.x * (kRows * (D + 2)));  // one per piece
   int g = 0;  // ring slots used so far
   // the n-th segment: null when there is none (or another warp gave up); free it when done with it
   auto segment = [&](int n) -> const Posted* {
@@ -217,6 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       bool ok = true;
       while (ok) {
+        if (lane == 0) marks[piece] = 0;  // (the consumers may set it once a segment is posted)
         while (ok && walk.next(s)) ok = post(2 * piece + s.slot) && load(s);
         if (!ok || rule.rounds == 1) break;
         if (lane == 0) {
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (s.whole) {
           const float y = sum == 0.f ? 0.f : x / sum;
           if (again && !(fabsf(y) <= 3.4028235e38f) && fabsf(sum) <= 3.4028235e38f && v < s.kv_hi)
-            atomicOr(&s_again, 1 << row);
+            marks[now->part >> 1] = 1;
           reinterpret_cast<T*>(a.o)[(int64_t)(s.r.begin + t) * a.os[0] +
                                     (int64_t)(s.h * a.G + hg) * a.os[1] + d] = E::from_f(y);
         } else {
@@ -481,18 +481,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (threadIdx.x == 32 * kProducers) s_stop = *abort_p;  // one reading, so that all warps leave together
       group_sync();
       ok = !s_stop;
-      if (s.whole && again) {
-        const int rows = s_again;
-        group_sync();
-        if (threadIdx.x == 32 * kProducers) s_again = 0;
-        for (int row = cw; row < nr; row += kWarps) {
-          if (!(rows >> row & 1)) continue;
-          const int t = (row0 + row) / a.G, h = s.h * a.G + (row0 + row) % a.G;
-          if (hidden_not_finite<DT>(a, s.b, s.h, visible_keys(s.r, t, a.causal), s.kv_hi))
-            row_by_key<DT>(a, s.b, s.r, t, h);
-        }
-        group_sync();
-      }
       release(n_seg);
       now = next;
     }
@@ -500,15 +488,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the parts of the tile that boundary blockIdx.x + 1 cuts first, every output element from
-// independent loads.
+// independent loads, and looks again at the rows of piece blockIdx.x if it is marked.
 template <int DT, int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, 5)  // (a block per piece of five rounds at once)
     decode_join_kernel(const __grid_constant__ AttnArgs a, const TileRule rule, const float* ws) {
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr int PART = kRows * (D + 2), U = 6;
   __shared__ int s_slot[kParts];
   __shared__ int s_whole, s_again;
+  __shared__ AgainScratch<D> s_look;
   if (threadIdx.x == 0) s_whole = s_again = 0;
   Line line;
   const Parts p = find_parts(a, rule, line);
@@ -523,10 +512,11 @@ __global__ void __launch_bounds__(128)
   };
   if (p.n) slots(0);
   wait_for_parts();
-  if (p.n == 0) return;
+  const int marked = __ldcg(reinterpret_cast<const int*>(ws + 2 * (int64_t)gridDim.x * PART) + blockIdx.x);
   const Segment& s = p.s;
-  const int row0 = s.tile * kRows, nr = min(kRows, s.r.n * a.G - row0);
-  if (s_whole) return;  // written by the CTA that has all of it
+  const int row0 = s.tile * kRows;
+  // (none, or one that a CTA has all of and has written)
+  const int nr = p.n == 0 || s_whole ? 0 : min(kRows, s.r.n * a.G - row0);
 #pragma unroll 1
   for (int at = 0; at < nr * D; at += 128) {
     const int e = at + threadIdx.x, row = e / D, d = e % D;
@@ -564,18 +554,12 @@ __global__ void __launch_bounds__(128)
     const int t = (row0 + row) / a.G, hg = (row0 + row) % a.G;
     if (!(fabsf(out) <= 3.4028235e38f) && fabsf(l) <= 3.4028235e38f &&
         visible_keys(s.r, t, a.causal) < s.kv_hi)
-      atomicOr(&s_again, 1 << row);
+      s_again = 1;
     reinterpret_cast<T*>(a.o)[(int64_t)(s.r.begin + t) * a.os[0] +
                               (int64_t)(s.h * a.G + hg) * a.os[1] + d] = E::from_f(out);
   }
   __syncthreads();
-  const int rows = s_again;
-  for (int row = threadIdx.x >> 5; row < nr && rows; row += 4) {
-    if (!(rows >> row & 1)) continue;
-    const int t = (row0 + row) / a.G, h = s.h * a.G + (row0 + row) % a.G;
-    if (hidden_not_finite<DT>(a, s.b, s.h, visible_keys(s.r, t, a.causal), s.kv_hi))
-      row_by_key<DT>(a, s.b, s.r, t, h);
-  }
+  look_again<DT, D>(a, rule, s, s_again, marked, blockIdx.x, 0, kRows, s_look);
 }
 
 template <int DT, int D>
@@ -591,12 +575,12 @@ static int launch_decode(const AttnArgs& a, float* ws, cudaStream_t st) {
   const int pieces = rule.ctas * rule.rounds;
   decode_kernel<DT, D><<<pieces, kThreads, DecodeCfg<D>::SMEM, st>>>(tk, tv, a, rule, box, ws);
   const int rc = launch_status("paged_attention");
-  if (rc || pieces < 2) return rc;
-  return launch_after(decode_join_kernel<DT, D>, dim3(pieces - 1), 128, st, a, rule, (const float*)ws);
+  if (rc) return rc;
+  return launch_after(decode_join_kernel<DT, D>, dim3(pieces), 128, st, a, rule, (const float*)ws);
 }
 
 size_t decode_workspace(int D) {
-  return 2 * (size_t)device_info().sm_count * kRounds * decode_part_floats(D) * sizeof(float);
+  return (size_t)device_info().sm_count * kRounds * (2 * decode_part_floats(D) * sizeof(float) + sizeof(int));
 }
 
 int run_decode(const AttnArgs& a, void* ws, cudaStream_t st) {

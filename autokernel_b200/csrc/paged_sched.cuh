@@ -14,7 +14,7 @@
 // that is done takes the next piece that has not begun (the hardware's cancellation of a CTA that
 // waits to be launched hands its number over).
 #pragma once
-#include "paged_attn.cuh"
+#include "paged_row.cuh"
 
 namespace ak {
 namespace paged {
@@ -246,7 +246,7 @@ AK_D Line find_piece(const AttnArgs& a, const TileRule& t, int piece) {
   return line;
 }
 
-// Walks the segments of one piece, in order; every role of a CTA walks for itself.
+// Walks the segments of one piece, in order.
 struct Walker {
   const AttnArgs& a;
   const TileRule& t;
@@ -431,65 +431,88 @@ struct PageFeed {
   }
 };
 
-// ------------------------------------------------------------------ rows read key by key
+// ------------------------------------------------------------------ rows that get a second look
 // The matrix instructions multiply a hidden key's value by a weight of 0, which is NaN when the
-// value is not finite.  A row whose result is not finite although its sum of weights is, and
-// that shares its tile with keys hidden from it, is looked at again: if a hidden value is the
-// cause, the row is computed from its visible keys alone.  One warp does a row.
+// value is not finite.  A row whose result is not finite although its sum of weights is, and that
+// shares its tile with keys hidden from it, is looked at again: if a hidden value may be the cause,
+// the row is computed from its visible keys alone.  Going through a long context key by key takes
+// milliseconds, so that never happens in a kernel whose warps wait for one another (they give up after
+// two seconds): the main kernels only mark the piece, and a kernel that comes after them and waits for
+// nothing within does the rows (200 rows of 200,000 keys: 1.4 s).
 
-// Whether V holds a value that is not finite at keys [lo, hi).
-template <int DT>
-AK_D bool hidden_not_finite(const AttnArgs& a, int b, int hk, int lo, int hi) {
-  using E = Elem<DT>;
-  const int lane = threadIdx.x & 31;
-  bool found = false;
-  for (int j = lo; j < hi; ++j) {
-    const int page = page_of(a.l, b, j / a.l.page_size);
-    if (page < 0) continue;
-    const typename E::T* v = reinterpret_cast<const typename E::T*>(a.v) + page * a.vcs[0] +
-                             hk * a.vcs[1] + (j % a.l.page_size) * a.vcs[2];
-    for (int d = lane; d < a.D; d += 32) found |= !(fabsf(E::to_f(v[d])) <= 3.4028235e38f);
-  }
-  return __any_sync(0xffffffffu, found);
-}
+template <int D>
+struct AgainScratch {
+  int last;
+  RowScratch<D / 8, 128> row;
+};
 
-// Row (token t of the sequence, query head h) from its visible keys; D <= 128.
-template <int DT>
-__device__ __noinline__ void row_by_key(const AttnArgs& a, int b, const SeqRange& r, int t, int h) {
+// The last key of [lo, hi) whose value is not finite, or -1; for a whole CTA.  16-bit types.
+template <int DT, int D>
+AK_D int last_not_finite(const AttnArgs& a, int b, int hk, int lo, int hi, int& s_last) {
   using E = Elem<DT>;
   using T = typename E::T;
-  const int lane = threadIdx.x & 31, hk = h / a.G;
-  const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(r.begin + t) * a.qs[0] + h * a.qs[1];
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+  if (threadIdx.x == 0) s_last = -1;
+  __syncthreads();
+  constexpr int VECS = D / 8;
+  int last = -1;
+  for (int i = threadIdx.x; i < (hi - lo) * VECS; i += blockDim.x) {  // (as many keys as a tile has tokens)
+    const int j = lo + i / VECS;
+    const int page = page_of(a.l, b, j / a.l.page_size);
+    if (page < 0) continue;
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(
+        reinterpret_cast<const T*>(a.v) + page * a.vcs[0] + hk * a.vcs[1] + (j % a.l.page_size) * a.vcs[2] + i % VECS * 8));
+    bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = lane + 32 * i < a.D ? E::to_f(qp[lane + 32 * i]) : 0.f;
-  float m = -INFINITY, sum = 0.f;
-  const int vis = visible_keys(r, t, a.causal);
-  for (int j = 0; j < vis; ++j) {
-    const int slot = j % a.l.page_size, page = page_of(a.l, b, j / a.l.page_size);
-    if (page < 0) {
-      sum = __int_as_float(0x7fffffff);
-      break;
-    }
-    const T* kp = reinterpret_cast<const T*>(a.k) + page * a.kcs[0] + hk * a.kcs[1] + slot * a.kcs[2];
-    const T* vp = reinterpret_cast<const T*>(a.v) + page * a.vcs[0] + hk * a.vcs[1] + slot * a.vcs[2];
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 32 * i < a.D) s = fmaf(q[i], E::to_f(kp[lane + 32 * i]), s);
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
-    const float alpha = exp2f((m - ref) * a.scale_log2), p = exp2f((s - ref) * a.scale_log2);
-    m = mn;
-    sum = sum * alpha + p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 32 * i < a.D) o[i] = fmaf(p, E::to_f(vp[lane + 32 * i]), o[i] * alpha);
+    for (int e = 0; e < 8; ++e) bad |= !(fabsf(E::to_f(reinterpret_cast<const T*>(&raw)[e])) <= 3.4028235e38f);
+    if (bad) last = j;
   }
-  T* op = reinterpret_cast<T*>(a.o) + (int64_t)(r.begin + t) * a.os[0] + h * a.os[1];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < a.D) op[lane + 32 * i] = E::from_f(sum == 0.f ? 0.f : o[i] / sum);
+  last = __reduce_max_sync(0xffffffffu, last);
+  if ((threadIdx.x & 31) == 0) atomicMax(&s_last, last);
+  __syncthreads();
+  return s_last;
+}
+
+// Rows [i0, i1) of tile s, by a CTA of 128 threads.
+template <int DT, int D>
+AK_D void look_again_at_tile(const AttnArgs& a, const TileRule& rule, const Segment& s, int i0, int i1,
+                             AgainScratch<D>& sh) {
+  using T = typename Elem<DT>::T;
+  const int last = last_not_finite<DT, D>(a, s.b, s.h, visible_keys(s.r, s.t_lo, a.causal), s.kv_hi, sh.last);
+  __syncthreads();  // (before the next tile's search)
+  for (int i = i0; i < i1 && last >= 0; ++i) {
+    int t, hg;
+    bool valid;
+    if (rule.rows) {  // rows follow one another
+      const int row = s.tile * rule.rows + i;
+      t = row / a.G;
+      hg = row % a.G;
+      valid = t < s.t_hi;
+    } else {  // two tiles of rule.tokens / 2 tokens
+      const int tt = rule.tokens / 2, row = i % 128;
+      t = s.t_lo + i / 128 * tt + row / a.G;
+      hg = row % a.G;
+      valid = row < tt * a.G && t < s.t_hi;
+    }
+    if (!valid || visible_keys(s.r, t, a.causal) > last) continue;
+    const T* o = reinterpret_cast<const T*>(a.o) + (int64_t)(s.r.begin + t) * a.os[0] + (int64_t)(s.h * a.G + hg) * a.os[1];
+    const bool bad = threadIdx.x < D && !(fabsf(Elem<DT>::to_f(o[threadIdx.x])) <= 3.4028235e38f);
+    if (__syncthreads_or(bad)) row_by_cta<DT, D / 8, 128>(a, s.b, s.r, t, s.h * a.G + hg, sh.row);
+  }
+}
+
+// Those rows of tile s (if `again`) and of every tile that piece `piece` has all of (if `marked`).
+template <int DT, int D>
+AK_D void look_again(const AttnArgs& a, const TileRule& rule, Segment s, bool again, bool marked, int piece, int i0,
+                     int i1, AgainScratch<D>& sh) {
+  if (!again && !marked) return;
+  Line line;
+  line.x = -1;
+  if (marked) line = find_piece(a, rule, piece);
+  Walker walk(a, rule, line, piece);
+  while (again || walk.next(s)) {
+    if (again || (s.whole && s.nb && a.causal && s.t_hi - s.t_lo > 1)) look_again_at_tile<DT, D>(a, rule, s, i0, i1, sh);
+    again = false;
+  }
 }
 
 }  // namespace paged

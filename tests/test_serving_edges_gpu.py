@@ -115,3 +115,71 @@ def test_decoding_gives_the_same_bits_every_time(seqs, heads, kv, D, dt):
     first = ops.paged_attention(q, kc, vc, *lists)
     for _ in range(20):
         assert torch.equal(ops.paged_attention(q, kc, vc, *lists), first)
+
+
+def packed(seqs, heads, kv_heads, D, dt, page=16, seed=0):
+    """(q, k_cache, v_cache, lists) of sequences (new tokens, keys) whose pages lie in order, and their keys'
+    places in the caches."""
+    g = torch.Generator(DEV).manual_seed(seed)
+    new, lens = [s[0] for s in seqs], [s[1] for s in seqs]
+    used = [-(-x // page) for x in lens]
+    first = [sum(used[:i]) for i in range(len(used))]
+    table = torch.full((len(seqs), max(used + [1])), -1, dtype=I32)
+    for b, n in enumerate(used):
+        table[b, :n] = torch.arange(first[b], first[b] + n)
+    kc, vc = (torch.randn(sum(used), kv_heads, page, D, device=DEV, dtype=dt, generator=g) for _ in range(2))
+    cu = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=I32, device=DEV)
+    q = torch.randn(sum(new), heads, D, device=DEV, dtype=dt, generator=g)
+    return q, kc, vc, (table.to(DEV), cu, torch.tensor(lens, dtype=I32, device=DEV)), first
+
+
+def near_64_bits(q, kc, vc, lists, seqs, first, o, rows, heads, page=16):
+    """Rows `rows` (sequence, token) of some heads against the formula in 64 bits, within the bound of
+    test_serving_gpu.py."""
+    G, D, h = q.shape[1] // kc.shape[1], q.shape[2], _half(q.dtype)
+    cu = lists[1].tolist()
+    for b, i in rows:
+        new, length = seqs[b]
+        vis = length - new + i + 1
+        for head in heads:
+            at = torch.arange(vis, device=DEV)
+            k, v = (c[first[b] + at // page, head // G, at % page].double() for c in (kc, vc))
+            x = q[cu[b] + i, head].double()
+            w = torch.softmax(k @ x * D ** -0.5, 0)
+            e, A = w @ v, w @ v.abs()
+            d = (D + 8) * 2.0 ** -24 * (k.abs() @ x.abs()).max() * D ** -0.5 + 2.0 ** -20
+            tol = h * e.abs() + (h + 2 * d + (vis + 8) * 2.0 ** -23) * A
+            err = (o[cu[b] + i, head].double() - e).abs()
+            assert (err <= tol).all(), (b, i, head, float((err - tol).max()))
+
+
+HIDDEN = [  # sequences, heads, kv heads, D: chunks cut into parts and whole in a piece, then decoding tiles
+    ([(256, 100000), (1, 50)], 1, 1, 64), ([(200, 200000)], 1, 1, 128), ([(64, 30000), (3, 77)], 4, 1, 128),
+    ([(250, 6000)], 300, 300, 64), ([(40, 3000), (60, 900)], 300, 300, 128),
+    ([(5, 100000), (1, 9)] + 6 * [(0, 0)], 2, 2, 64), ([(3, 3000), (2, 400)] + 6 * [(0, 0)], 600, 300, 128),
+    ([(4, 20000)] + 6 * [(0, 0)], 64, 16, 64)]
+
+
+@pytest.mark.parametrize("dt,value", [("f16", float("inf")), ("bf16", float("nan"))])
+@pytest.mark.parametrize("case", range(len(HIDDEN)))
+def test_hidden_infinities_under_long_contexts(case, dt, value):
+    """The value of a chunk's last token is not finite: the tokens before it, which share its tile and see long
+    contexts, are as without it; so are the other sequences, and no wait runs out."""
+    seqs, heads, kv, D = HIDDEN[case]
+    q, kc, vc, lists, first = packed(seqs, heads, kv, D, DTS[dt], seed=case)
+    clean = ops.paged_attention(q, kc, vc, *lists)
+    new, length = seqs[0]
+    vc[first[0] + (length - 1) // 16, :, (length - 1) % 16] = value
+    o = ops.paged_attention(q, kc, vc, *lists)
+    again = ops.paged_attention(q, kc, vc, *lists)
+    torch.cuda.synchronize()
+    assert device_status() == 0
+    rest = torch.arange(o.shape[0], device=DEV) != new - 1
+    assert o[rest].isfinite().all() and not o[new - 1].isfinite().any()
+    assert torch.equal(o[rest], again[rest])
+    # the clean call rounds its weights to 16 bits, so it differs; rows of other sequences do not
+    assert torch.equal(o[new:], clean[new:])
+    some = [(0, i) for i in sorted({0, new // 2, new - 2})]
+    if len(seqs) > 1 and seqs[1][0]:
+        some.append((1, seqs[1][0] - 1))
+    near_64_bits(q, kc, vc, lists, seqs, first, o, some, sorted({0, heads // 2, heads - 1}))
