@@ -284,8 +284,8 @@ class LlamaB200:
                  cache: PagedCache | None = None) -> list[list[int]]:
         """Continue each prompt (token lists, at least one token each) by up to max_new_tokens sampled
         tokens (ops.sample's settings; temperature 0 takes the likeliest).  A sequence ends with the
-        token `stop`, if given.  All sequences decode together; with `cache` they share its pages and
-        give them back at the end, otherwise one of the right size is made.  Raises AkError when a
+        token `stop`, if given.  All sequences decode together; with `cache` they share its pages, each
+        giving its own back when it ends, otherwise one of the right size is made.  Raises AkError when a
         step's logits hold nothing to draw (all NaN)."""
         if not prompts or min(len(p) for p in prompts) < 1 or max_new_tokens < 0:
             raise ValueError("generate: need prompts of at least one token")
@@ -299,7 +299,7 @@ class LlamaB200:
             size = 64
             cache = self.new_cache(sum(-(-(len(p) + max_new_tokens) // size) for p in prompts), size)
         live = list(range(len(prompts)))
-        seqs = [cache.add() for _ in prompts]
+        seqs = {i: cache.add() for i in live}  # those that hold pages
         tokens = torch.tensor([t for p in prompts for t in p], device=device)
         counts = [len(p) for p in prompts]
         steps: list[tuple[list[int], torch.Tensor]] = []
@@ -314,12 +314,15 @@ class LlamaB200:
                 if stop is not None:
                     on = (tokens != stop).tolist()
                     tokens = tokens[torch.tensor(on, device=device)]
+                    for i, x in zip(live, on):
+                        if not x:
+                            cache.release(seqs.pop(i))
                     live = [i for i, x in zip(live, on) if x]
                     if not live:
                         break
                 counts = [1] * len(live)
         finally:
-            for s in seqs:
+            for s in seqs.values():
                 cache.release(s)
         out: list[list[int]] = [[] for _ in prompts]
         for rows, t in steps:

@@ -1,0 +1,49 @@
+"""LlamaB200.generate's bookkeeping on the CPU: a model whose next token is the last one + 1, and a sampler that
+takes the likeliest, in place of the kernels."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from autokernel_b200 import AkError, ops
+from autokernel_b200.llama import LlamaB200, LlamaConfig
+
+VOCAB = 100
+
+
+class Counting(LlamaB200):
+    """extend() returns logits whose largest is that of the last token + 1, and checks the batch."""
+
+    def __init__(self):
+        cfg = LlamaConfig(vocab_size=VOCAB, dim=8, n_layers=1, n_heads=1, n_kv_heads=1, hidden_dim=8)
+        super().__init__(cfg, {"tok_embeddings.weight": torch.zeros(VOCAB, 8)})
+
+    def extend(self, tokens, batch, cache):
+        assert tokens.shape == (batch.n_tokens,)
+        last = tokens[batch.cu_q[1:].long() - 1]
+        return torch.nn.functional.one_hot((last + 1) % VOCAB, VOCAB).float()
+
+
+@pytest.fixture
+def settings(monkeypatch):
+    """The settings of every ops.sample call, each as one number per row."""
+    seen = []
+
+    def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        n = logits.shape[0]
+        row = [v.tolist() if isinstance(v, torch.Tensor) else [v] * n for v in (temperature, top_k, top_p, min_p)]
+        assert all(len(r) == n for r in row)
+        seen.append([tuple(x) for x in zip(*row)])
+        return logits.argmax(-1)
+
+    monkeypatch.setattr(ops, "sample", sample)
+    return seen
+
+
+def test_a_stopped_sequence_gives_its_pages_back_at_once(settings):
+    """8 pages of 4: the first two answers stop after one token, and the third grows into their pages."""
+    m = Counting()
+    cache = m.new_cache(8, 4)
+    got = m.generate([[41] * 12, [41] * 8, [1, 2, 3]], 20, stop=42, cache=cache)
+    assert got == [[42], [42], list(range(4, 24))]
+    assert cache.free_pages == 8
