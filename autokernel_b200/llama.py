@@ -39,7 +39,7 @@ import torch
 
 from . import ops, shard
 from ._lib import AkError
-from .paged import Batch, PagedCache
+from .paged import Batch, CacheFull, PagedCache
 
 
 @dataclass
@@ -285,8 +285,9 @@ class LlamaB200:
         """Continue each prompt (token lists, at least one token each) by up to max_new_tokens sampled
         tokens (ops.sample's settings; temperature 0 takes the likeliest).  A sequence ends with the
         token `stop`, if given.  All sequences decode together; with `cache` they share its pages, each
-        giving its own back when it ends, otherwise one of the right size is made.  Raises AkError when a
-        step's logits hold nothing to draw (all NaN)."""
+        giving its own back when it ends, otherwise one of the right size is made.  Raises CacheFull when a
+        step finds no pages, with the tokens sampled so far as its `answers`, and AkError when a step's logits
+        held nothing to draw (all NaN)."""
         if not prompts or min(len(p) for p in prompts) < 1 or max_new_tokens < 0:
             raise ValueError("generate: need prompts of at least one token")
         vocab = self.w["tok_embeddings.weight"].shape[0]
@@ -303,8 +304,18 @@ class LlamaB200:
         tokens = torch.tensor([t for p in prompts for t in p], device=device)
         counts = [len(p) for p in prompts]
         steps: list[tuple[list[int], torch.Tensor]] = []
+
+        def answers() -> list[list[int]]:
+            out: list[list[int]] = [[] for _ in prompts]
+            for rows, t in steps:
+                for i, x in zip(rows, t.tolist()):
+                    if x < 0:
+                        raise AkError(f"generate: sequence {i} has no logits to draw from")
+                    out[i].append(x)
+            return out
+
         try:
-            for step in range(max_new_tokens):
+            for _ in range(max_new_tokens):
                 batch = cache.extend([seqs[i] for i in live], counts)
                 logits = self.extend(tokens, batch, cache)
                 u = torch.rand(len(live), device=device, generator=generator)
@@ -321,16 +332,13 @@ class LlamaB200:
                     if not live:
                         break
                 counts = [1] * len(live)
+        except CacheFull as e:
+            e.answers = answers()
+            raise
         finally:
             for s in seqs.values():
                 cache.release(s)
-        out: list[list[int]] = [[] for _ in prompts]
-        for rows, t in steps:
-            for i, x in zip(rows, t.tolist()):
-                if x < 0:
-                    raise AkError(f"generate: sequence {i} has no logits to draw from")
-                out[i].append(x)
-        return out
+        return answers()
 
     @staticmethod
     def next_token_targets(tokens: torch.Tensor) -> torch.Tensor:

@@ -15,6 +15,12 @@ import torch
 from ._lib import AkError
 
 
+class CacheFull(AkError):
+    """A step needs more pages than are free.  `answers`, where LlamaB200.generate met it: the tokens of each
+    prompt that were sampled before."""
+    answers: list[list[int]] | None = None
+
+
 @dataclass
 class Batch:
     """The device lists of one step (arguments of the paged operators) and what the host knows."""
@@ -70,7 +76,7 @@ class PagedCache:
 
     def extend(self, seqs: list[int], counts: list[int]) -> Batch:
         """Room for counts[i] >= 1 new tokens of sequence seqs[i], and the lists of that step.  Raises
-        AkError, with nothing changed, when the pages do not suffice."""
+        CacheFull, with nothing changed, when the pages do not suffice."""
         if len(seqs) != len(counts) or not seqs:
             raise ValueError("PagedCache.extend: need one count per sequence, and a sequence")
         if len(set(seqs)) != len(seqs):
@@ -80,7 +86,7 @@ class PagedCache:
         lens = [self._lens[s] + c for s, c in zip(seqs, counts)]
         more = [-(-n // self.page_size) - len(self._pages[s]) for s, n in zip(seqs, lens)]
         if sum(more) > len(self._free):
-            raise AkError(f"paged cache is full: {sum(more)} pages needed, {len(self._free)} free")
+            raise CacheFull(f"paged cache is full: {sum(more)} pages needed, {len(self._free)} free")
         for s, n, m in zip(seqs, lens, more):
             self._pages[s].extend(self._free.pop() for _ in range(m))
             self._lens[s] = n
@@ -96,4 +102,4 @@ class PagedCache:
         return Batch(t[:n].view(B, width), t[n:n + B + 1], t[n + B + 1:], cu[-1], max(lens))
 
 
-__all__ = ["Batch", "PagedCache"]
+__all__ = ["Batch", "CacheFull", "PagedCache"]

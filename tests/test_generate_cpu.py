@@ -47,3 +47,17 @@ def test_a_stopped_sequence_gives_its_pages_back_at_once(settings):
     got = m.generate([[41] * 12, [41] * 8, [1, 2, 3]], 20, stop=42, cache=cache)
     assert got == [[42], [42], list(range(4, 24))]
     assert cache.free_pages == 8
+
+
+def test_a_full_cache_does_not_lose_the_answers_so_far(settings):
+    """3 pages of 4: the second sequence's fifth key finds no page; what was sampled by then comes with the error."""
+    m = Counting()
+    cache = m.new_cache(3, 4)
+    with pytest.raises(AkError, match="full") as e:
+        m.generate([[10, 11, 12, 13, 14], [30, 31]], 20, cache=cache)
+    assert e.value.answers == [[15, 16, 17], [32, 33, 34]]
+    assert cache.free_pages == 3
+    with pytest.raises(AkError, match="full") as e:
+        m.generate([[1] * 13], 20, cache=cache)
+    assert e.value.answers == [[]]
+    assert cache.free_pages == 3
