@@ -33,6 +33,7 @@ the new tokens attend by ops.paged_attention, and ops.sample draws the next toke
 """
 from __future__ import annotations
 
+from collections.abc import Sequence
 from dataclasses import dataclass
 
 import torch
@@ -278,13 +279,15 @@ class LlamaB200:
         return ops.linear(ops.rmsnorm_fp32(last, w["norm.weight"], c.norm_eps), w["output.weight"])
 
     @torch.no_grad()
-    def generate(self, prompts: list[list[int]], max_new_tokens: int, temperature: float = 1.0,
-                 top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, stop: int | None = None,
+    def generate(self, prompts: list[list[int]], max_new_tokens: int,
+                 temperature: float | Sequence[float] | torch.Tensor = 1.0,
+                 top_k: int | Sequence[int] | torch.Tensor = 0, top_p: float | Sequence[float] | torch.Tensor = 1.0,
+                 min_p: float | Sequence[float] | torch.Tensor = 0.0, stop: int | None = None,
                  generator: torch.Generator | None = None,
                  cache: PagedCache | None = None) -> list[list[int]]:
         """Continue each prompt (token lists, at least one token each) by up to max_new_tokens sampled
-        tokens (ops.sample's settings; temperature 0 takes the likeliest).  A sequence ends with the
-        token `stop`, if given.  All sequences decode together; with `cache` they share its pages, each
+        tokens (ops.sample's settings, each a number or one per prompt; temperature 0 takes the likeliest).
+        A sequence ends with the token `stop`, if given.  All sequences decode together; with `cache` they share its pages, each
         giving its own back when it ends, otherwise one of the right size is made.  Raises CacheFull when a
         step finds no pages, with the tokens sampled so far as its `answers`, and AkError when a step's logits
         held nothing to draw (all NaN)."""
@@ -293,9 +296,11 @@ class LlamaB200:
         vocab = self.w["tok_embeddings.weight"].shape[0]
         if not all(0 <= t < vocab for p in prompts for t in p):
             raise ValueError(f"generate: tokens must lie in [0, {vocab})")
+        device = self.w["tok_embeddings.weight"].device
+        settings = [_setting(n, v, len(prompts), device) for n, v in (
+            ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p))]
         if max_new_tokens == 0:
             return [[] for _ in prompts]
-        device = self.w["tok_embeddings.weight"].device
         if cache is None:
             size = 64
             cache = self.new_cache(sum(-(-(len(p) + max_new_tokens) // size) for p in prompts), size)
@@ -319,12 +324,15 @@ class LlamaB200:
                 batch = cache.extend([seqs[i] for i in live], counts)
                 logits = self.extend(tokens, batch, cache)
                 u = torch.rand(len(live), device=device, generator=generator)
-                tokens = ops.sample(logits, u, temperature, top_k, top_p, min_p)
+                tokens = ops.sample(logits, u, *settings)
                 steps.append((live, tokens))
                 tokens = tokens.clamp(min=0)  # -1: nothing to draw, found when the answers are read
                 if stop is not None:
                     on = (tokens != stop).tolist()
-                    tokens = tokens[torch.tensor(on, device=device)]
+                    if not all(on):
+                        rest = torch.tensor(on, device=device)
+                        tokens = tokens[rest]
+                        settings = [v[rest] if isinstance(v, torch.Tensor) else v for v in settings]
                     for i, x in zip(live, on):
                         if not x:
                             cache.release(seqs.pop(i))
@@ -361,6 +369,25 @@ class LlamaB200:
             h.view(-1, h.shape[-1]), targets.view(-1), group=group,
             partial_fn=lambda x, t: ops.linear_cross_entropy_partial(x, W, t),
             out_dtype=h.dtype)
+
+
+def _setting(name: str, v, n: int, device) -> float | torch.Tensor:
+    """A sampling setting of n prompts as ops.sample takes it: the number, or a tensor [n] of one each."""
+    dtype = torch.int32 if name == "top_k" else torch.float32
+    if isinstance(v, torch.Tensor):
+        if v.shape != (n,) or v.is_floating_point() != dtype.is_floating_point:
+            raise ValueError(f"generate: a tensor of {name} must hold one {dtype} per prompt ({n})")
+        return v.to(device=device, dtype=dtype)
+    numbers = list(v) if isinstance(v, Sequence) else [v]
+    if isinstance(v, Sequence) and len(numbers) != n:
+        raise ValueError(f"generate: {len(numbers)} values of {name} for {n} prompts")
+    if not all(x >= 0 for x in numbers):
+        raise ValueError(f"generate: {name} must not be negative, got {v}")
+    if isinstance(v, Sequence):
+        if name == "top_k":
+            numbers = [min(int(x), 2 ** 31 - 1) for x in numbers]
+        return torch.tensor(numbers, dtype=dtype, device=device)
+    return v
 
 
 def model_flops(cfg: LlamaConfig, batch: int, seq_len: int) -> float:

@@ -61,3 +61,26 @@ def test_a_full_cache_does_not_lose_the_answers_so_far(settings):
         m.generate([[1] * 13], 20, cache=cache)
     assert e.value.answers == [[]]
     assert cache.free_pages == 3
+
+
+@pytest.mark.parametrize("kind", ["list", "tensor"])
+def test_settings_of_each_prompt_follow_their_sequences(settings, kind):
+    """The second and then the first sequence stop: each row keeps the settings of its prompt."""
+    m = Counting()
+    given = dict(temperature=[0.5, 0.25, 2.0], top_k=[1, 0, 7], top_p=[1.0, 0.5, 0.75], min_p=[0.0, 0.125, 0.25])
+    if kind == "tensor":
+        given = {k: torch.tensor(v) for k, v in given.items()}
+    got = m.generate([[38], [40], [1]], 5, stop=41, **given)
+    assert got == [[39, 40, 41], [41], [2, 3, 4, 5, 6]]
+    rows = list(zip([0.5, 0.25, 2.0], [1, 0, 7], [1.0, 0.5, 0.75], [0.0, 0.125, 0.25]))
+    assert settings == [rows, [rows[0], rows[2]], [rows[0], rows[2]], [rows[2]], [rows[2]]]
+
+
+def test_bad_settings_are_refused_before_anything_is_run(settings):
+    m = Counting()
+    cache = m.new_cache(4, 4)
+    for bad in (dict(temperature=[1.0]), dict(top_p=torch.ones(3)), dict(min_p=torch.ones(2, 1)), dict(top_k=[1, -1]),
+                dict(temperature=[0.5, float("nan")]), dict(top_k=torch.ones(2)), dict(top_p=-0.5)):
+        with pytest.raises(ValueError):
+            m.generate([[1], [2]], 3, cache=cache, **bad)
+    assert settings == [] and cache.free_pages == 4
