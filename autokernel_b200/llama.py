@@ -246,16 +246,24 @@ class LlamaB200:
                          cache.k[i], cache.v[i], *batch.lists, q=q, cos=cos, sin=sin, q_out=q)
         return ops.paged_attention(q, cache.k[i], cache.v[i], *batch.lists).view(N, -1)
 
+    def _embed(self, tokens: torch.Tensor) -> torch.Tensor:
+        """The embeddings of tokens [N]; NaN for one that is not in the vocabulary (no host code knows them, and a
+        gather outside of the table would end the CUDA context)."""
+        table = self.w["tok_embeddings.weight"]
+        known = tokens.clamp(0, table.shape[0] - 1)
+        return torch.nn.functional.embedding(known, table).masked_fill_((known != tokens)[:, None], float("nan"))
+
     @torch.no_grad()
     def extend(self, tokens: torch.Tensor, batch: Batch, cache: PagedCache) -> torch.Tensor:
         """Run the packed new tokens [N] of a batch (cache.extend) and return the logits [B, vocab] that
-        follow the last one of each sequence."""
+        follow the last one of each sequence.  A token outside of the vocabulary (ops.sample's -1) makes its
+        sequence's logits NaN from there on, and no other's."""
         c, w = self.cfg, self.w
         if tokens.shape != (batch.n_tokens,):
             raise ValueError(f"extend: the batch holds {batch.n_tokens} tokens, got {tuple(tokens.shape)}")
         # tables to the next power of two, so that decoding does not rebuild them at every step
         cos, sin = self._tables(max(2048, 1 << (batch.max_len - 1).bit_length()), tokens.device)
-        h = torch.nn.functional.embedding(tokens, w["tok_embeddings.weight"])
+        h = self._embed(tokens)
         ss = ops.row_sumsq(h) if self.fuse_norms else None
         for i in range(c.n_layers):
             p = f"layers.{i}."

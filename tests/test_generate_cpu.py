@@ -84,3 +84,13 @@ def test_bad_settings_are_refused_before_anything_is_run(settings):
         with pytest.raises(ValueError):
             m.generate([[1], [2]], 3, cache=cache, **bad)
     assert settings == [] and cache.free_pages == 4
+
+
+def test_tokens_outside_of_the_vocabulary_embed_as_nan():
+    """A gather with such an index ends the CUDA context; extend() has to take whatever a sampler gave (-1 too)."""
+    m = Counting()
+    m.w["tok_embeddings.weight"] = torch.arange(VOCAB * 8).view(VOCAB, 8).half()
+    for dt in (torch.int64, torch.int32):
+        h = m._embed(torch.tensor([3, -1, 99, 100, 2 ** 31 - 1, -2 ** 31, 0], dtype=dt))
+        assert h.dtype == torch.float16 and h.isnan().all(-1).tolist() == [False, True, False, True, True, True, False]
+        assert torch.equal(h[[0, 2, 6]], m.w["tok_embeddings.weight"][[3, 99, 0]])

@@ -183,3 +183,46 @@ def test_hidden_infinities_under_long_contexts(case, dt, value):
     if len(seqs) > 1 and seqs[1][0]:
         some.append((1, seqs[1][0] - 1))
     near_64_bits(q, kc, vc, lists, seqs, first, o, some, sorted({0, heads // 2, heads - 1}))
+
+
+def _model(dtype=torch.float16, heads=4, dim=256):
+    from autokernel_b200.llama import LlamaB200, LlamaConfig
+    c = LlamaConfig(vocab_size=512, dim=dim, n_layers=2, n_heads=heads, n_kv_heads=2, hidden_dim=512)
+    return LlamaB200(c, LlamaB200.random_weights(c, DEV, dtype=dtype, seed=3, std=0.05))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [40, 70, 3]])
+def test_a_token_outside_of_the_vocabulary_stays_in_its_sequence(dtype, counts):
+    m = _model(dtype)
+    cache = m.new_cache(40, 16)
+    seqs = [cache.add() for _ in counts]
+    g = torch.Generator().manual_seed(1)
+
+    def step(counts, bad):
+        batch = cache.extend(seqs, counts)
+        tokens = torch.randint(0, 512, (sum(counts),), generator=g)
+        out = []
+        for at in (None, bad):  # twice over the same keys: they are written again
+            t = tokens.clone()
+            if at is not None:
+                t[at] = [-1, 512, 2 ** 40][at % 3]
+            out.append(m.extend(t.to(DEV), batch, cache))
+        return out
+
+    step([20, 33, 5], None)
+    good, bad = step(counts, counts[0])  # the second sequence's first token
+    assert torch.equal(good[[0, 2]], bad[[0, 2]]) and good.isfinite().all() and bad[1].isnan().all()
+    good, bad = step([1, 1, 1], None)
+    assert good[[0, 2]].isfinite().all() and good[1].isnan().all()
+    assert ops.sample(good, torch.rand(3, device=DEV)).tolist()[1] == -1
+    assert device_status() == 0
+
+
+def test_generate_with_settings_of_each_prompt():
+    m = _model()
+    prompts = [[1, 2, 3], [7] * 70, [5]]
+    greedy = m.generate(prompts, 6, temperature=0.0)
+    got = m.generate(prompts, 6, temperature=[0.0, 1.0, 0.0], top_k=torch.tensor([0, 50, 0]), top_p=[1.0, 0.9, 1.0],
+                     generator=torch.Generator(DEV).manual_seed(1))
+    assert got[0] == greedy[0] and got[2] == greedy[2] and len(got[1]) == 6
