@@ -74,8 +74,19 @@ class PagedCache:
         self._free.extend(reversed(self._pages.pop(seq)))
         del self._lens[seq]
 
+    def truncate(self, seq: int, length: int) -> None:
+        """Forget the keys from position `length` on, and give back the pages that hold none of the rest: for
+        tokens that extend() counted and no step wrote, or that a caller takes back."""
+        if not 0 <= length <= self._lens[seq]:
+            raise ValueError(f"PagedCache.truncate: length must lie in [0, {self._lens[seq]}], got {length}")
+        pages, kept = self._pages[seq], -(-length // self.page_size)
+        self._free.extend(reversed(pages[kept:]))
+        del pages[kept:]
+        self._lens[seq] = length
+
     def extend(self, seqs: list[int], counts: list[int]) -> Batch:
-        """Room for counts[i] >= 1 new tokens of sequence seqs[i], and the lists of that step.  Raises
+        """Room for counts[i] >= 1 new tokens of sequence seqs[i], and the lists of that step.  The tokens
+        count as keys from here on: a step that is not run after all is taken back by truncate().  Raises
         CacheFull, with nothing changed, when the pages do not suffice."""
         if len(seqs) != len(counts) or not seqs:
             raise ValueError("PagedCache.extend: need one count per sequence, and a sequence")

@@ -274,3 +274,28 @@ def test_registered_serving_ops():
     for op, args in ((AK.paged_append, (k, k, kc, vc, *lists, q, cos, sin)),
                      (AK.paged_attention, (q, kc, vc, *lists)), (AK.sample, (x, u))):
         torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+
+
+def test_a_sequence_can_be_shortened():
+    """What extend() counted and nobody ran is taken back, pages included."""
+    c = _cache()
+    a, b = c.add(), c.add()
+    c.extend([a, b], [6, 3])
+    first = c.pages(a)
+    c.extend([a], [11])
+    assert c.free_pages == 4 and len(c.pages(a)) == 5
+    c.truncate(a, 6)
+    assert c.length(a) == 6 and c.pages(a) == first and c.free_pages == 7
+    c.truncate(a, 4)
+    assert c.pages(a) == first[:1] and c.free_pages == 8
+    x = c.extend([a], [1])
+    assert x.kv_lens.tolist() == [5] and x.page_table[0, 0] == first[0]
+    assert not set(c.pages(a)) & set(c.pages(b))
+    c.truncate(a, 5)
+    c.truncate(a, 0)
+    assert c.length(a) == 0 and c.pages(a) == [] and c.free_pages == 9
+    for n in (-1, 1):
+        with pytest.raises(ValueError, match="truncate"):
+            c.truncate(a, n)
+    with pytest.raises(KeyError):
+        c.truncate(77, 0)
