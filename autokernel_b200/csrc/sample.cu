@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __gri
             for (int e = 0; e < VEC; ++e) {  // no branch: the chains of operations overlap
               const double x = w(f[e]);
               if (f[e] > f_hi) above += x;
-              if (f[e] < f_lo) below += x;
+              if (f[e] < f_lo && alive(f[e])) below += x;  // (a dead entry's x is NaN at T = inf)
               some |= (unsigned)(f[e] <= f_hi && f[e] >= f_lo) << e;
             }
             while (some) {  // their bins come later, from all threads at once

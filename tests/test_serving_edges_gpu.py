@@ -226,3 +226,20 @@ def test_generate_with_settings_of_each_prompt():
     got = m.generate(prompts, 6, temperature=[0.0, 1.0, 0.0], top_k=torch.tensor([0, 50, 0]), top_p=[1.0, 0.9, 1.0],
                      generator=torch.Generator(DEV).manual_seed(1))
     assert got[0] == greedy[0] and got[2] == greedy[2] and len(got[1]) == 6
+
+
+@pytest.mark.parametrize("dt", list(DTS))
+@pytest.mark.parametrize("vocab", [700, 40000])
+def test_infinite_temperature_among_dead_logits(dt, vocab):
+    """Every alive entry weighs the same; NaN and -inf, and what top-k left out, weigh nothing."""
+    from oracle import serve_f64
+    g = torch.Generator(DEV).manual_seed(5)
+    x = torch.randn(12, vocab, device=DEV, generator=g).to(DTS[dt])
+    x[::2, ::3] = -math.inf
+    x[::3, 1::4] = math.nan
+    x[4:6] = torch.where(x[4:6].isfinite(), 1.0, x[4:6])
+    u = torch.rand(12, device=DEV, generator=g)
+    for kw in (dict(top_p=0.5), dict(top_p=0.001), dict(top_p=0.999), dict(top_k=vocab // 2, top_p=0.3), dict(min_p=0.5), dict()):
+        got = ops.sample(x, u, temperature=math.inf, **kw).tolist()
+        kw = {k: float(np.float32(v)) if k != "top_k" else v for k, v in kw.items()}
+        assert got == [serve_f64.sample_row(x[r].double().cpu().numpy(), u[r].item(), math.inf, **kw) for r in range(12)]
