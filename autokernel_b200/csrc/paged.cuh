@@ -23,6 +23,24 @@ struct PagedLists {
   int max_pages, num_pages, page_size;
 };
 
+// Whether the rows of `inner` contiguous elements that n <= 3 strided dims name may share elements: an output
+// of such a layout would be written by several threads at once.
+inline bool may_overlap(const int64_t* sizes, const int64_t* strides, int n, int64_t inner) {
+  int order[3], m = 0;
+  for (int i = 0; i < n; ++i) {  // the dims of more than one element, by stride
+    if (sizes[i] <= 1) continue;
+    int at = m++;
+    for (; at > 0 && strides[order[at - 1]] > strides[i]; --at) order[at] = order[at - 1];
+    order[at] = i;
+  }
+  int64_t extent = inner;  // of what the dims so far span
+  for (int k = 0; k < m; ++k) {
+    if (strides[order[k]] < extent) return true;
+    extent += (sizes[order[k]] - 1) * strides[order[k]];
+  }
+  return false;
+}
+
 struct SeqRange {
   int begin, n;    // first packed token, number of new tokens
   int kv_len;      // keys, the new tokens counted (may exceed what the table can name)

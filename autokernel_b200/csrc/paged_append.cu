@@ -244,6 +244,14 @@ extern "C" int ak_paged_append(const void* k, const void* v, const void* q, void
                  ((k_cache && v_cache) || num_pages == 0) && (page_table || max_pages == 0),
              AK_ERR_ARG, "null pointer");
   AK_REQUIRE(!q || (q_out && q_strides && q_out_strides), AK_ERR_ARG, "q without q_out");
+  const int64_t cache[3] = {num_pages, Hkv, page_size}, tokens[2] = {N, H};
+  AK_REQUIRE(num_pages == 0 || (k_cache != v_cache && !may_overlap(cache, k_cache_strides, 3, D) &&
+                                !may_overlap(cache, v_cache_strides, 3, D)),
+             AK_ERR_ARG, "the caches overlap each other or themselves");
+  AK_REQUIRE(!q || !may_overlap(tokens, q_out_strides, 2, D), AK_ERR_ARG, "q_out overlaps itself");
+  AK_REQUIRE(!q || (q_out != k && q_out != v && q_out != k_cache && q_out != v_cache &&
+                    (q_out != q || (q_strides[0] == q_out_strides[0] && q_strides[1] == q_out_strides[1]))),
+             AK_ERR_ARG, "q_out overlaps another tensor (it may only be q itself)");
   AppendArgs a{};
   a.l = PagedLists{page_table, cu_q,           kv_lens,        table_ld,      (int)N,
                    (int)B,     (int)max_pages, (int)num_pages, (int)page_size};

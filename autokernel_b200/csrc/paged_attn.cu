@@ -91,12 +91,15 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
   AK_REQUIRE(N < (1LL << 31) && B < (1LL << 31) - 64 && H <= 65535 && num_pages < (1LL << 31) &&
                  page_size < (1LL << 31) && max_pages < (1LL << 31),
              AK_ERR_SHAPE, "dimension too large");
-  AK_REQUIRE(sm_scale > 0.f && sm_scale <= 3.0e38f, AK_ERR_ARG,
+  AK_REQUIRE(sm_scale > 0.f && sm_scale <= 2.3e38f, AK_ERR_ARG,  // (times log2(e) it must be finite too)
              "sm_scale must be positive and finite");
   if (N == 0 || B == 0) return AK_OK;
   AK_REQUIRE(q && out && cu_q && kv_lens && q_strides && out_strides && k_cache_strides && v_cache_strides &&
                  ((k_cache && v_cache) || num_pages == 0) && (page_table || max_pages == 0),
              AK_ERR_ARG, "null pointer");
+  const int64_t tokens[2] = {N, H};
+  AK_REQUIRE(!may_overlap(tokens, out_strides, 2, D), AK_ERR_ARG, "out overlaps itself");
+  AK_REQUIRE(out != q && out != k_cache && out != v_cache, AK_ERR_ARG, "out overlaps an input");
   const size_t need = ak_paged_attention_workspace_size(N, B, H, Hkv, D, dtype);
   AK_REQUIRE(need == 0 || (workspace && aligned16(workspace) && ws_bytes >= need), AK_ERR_ARG,
              "workspace of %zu bytes (16-byte aligned) needed, %zu given", need, ws_bytes);

@@ -665,7 +665,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     Returns the rotated q (in q_out if given, which may be q itself), or None without q.  Tokens
     behind cu_q[B] are left alone (a fresh result is not initialised there).  A key whose position
     is negative or has no page in the table is not stored; positions outside cos / sin give NaN.
-    Two tokens of a call must not share a slot: what such a slot holds is undefined."""
+    Outputs that overlap one another, themselves or (but for q_out = q) an input are refused where strides
+    or addresses show it.  Two tokens of a call must not share a slot: what such a slot holds is undefined."""
     name = "paged_append"
     (P, Hkv, S, D), kcs, vcs, dt, B, width, ld = _paged_cache(name, k_cache, v_cache, page_table, cu_q, kv_lens)
     (N, _, _), ks = _tokens(name, "k", k, None, Hkv, D, dt)
@@ -738,7 +739,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"{name}: head_dim {D} exceeds 256")
     if sm_scale is None:
         sm_scale = D ** -0.5
-    if not 0 < sm_scale <= 3e38:
+    if not 0 < sm_scale <= 2.3e38:
         raise ValueError(f"{name}: sm_scale must be positive and finite, got {sm_scale}")
     code = dtype_code(dt)
     if out is None:

@@ -277,8 +277,9 @@ AK_API int ak_flash_attention_strided(const void* Q, const void* K, const void* 
 /* k_cache / v_cache at each token's position = rot(k), v; q_out (with q) = rot(q).  rot is the
  * interleaved RoPE of ak_rotary_embedding with fp32 cos / sin [positions, D / 2] (one rounding);
  * without tables it copies.  Positions outside the tables give NaN; keys without a page (or at
- * a negative position) are not stored.  q may be NULL; q_out may be q.  Two tokens of one call
- * must not name the same slot. */
+ * a negative position) are not stored.  q may be NULL; q_out may be q, with the same strides; an
+ * output that overlaps another, itself or an input otherwise is refused where strides or equal
+ * addresses show it.  Two tokens of one call must not name the same slot. */
 AK_API int ak_paged_append(const void* k, const void* v, const void* q, void* q_out, void* k_cache,
                     void* v_cache, const int32_t* page_table, const int32_t* cu_q,
                     const int32_t* kv_lens, const float* cos, const float* sin, int64_t N,
@@ -293,7 +294,8 @@ AK_API int ak_paged_append(const void* k, const void* v, const void* q, void* q_
  * that sees no key (or only scores of -inf) is 0; a row that sees a key without a page is NaN, and so may
  * be, in 16-bit types, one whose largest score times sm_scale log2(e) is 2^27 (fp16) or 2^31 (bf16)
  * or more in size: no 16-bit weights reach from there.
- * What the cache holds behind a sequence's last key never matters.  D <= 256, sm_scale > 0.
+ * What the cache holds behind a sequence's last key never matters.  D <= 256, 0 < sm_scale <= 2.3e38;
+ * out must not overlap itself or an input.
  * workspace: ak_paged_attention_workspace_size bytes, used by this call alone until it is done. */
 AK_API size_t ak_paged_attention_workspace_size(int64_t N, int64_t B, int64_t H, int64_t Hkv,
                                          int64_t D, int dtype);
