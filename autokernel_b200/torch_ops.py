@@ -1,5 +1,6 @@
 """The nine operators, and the three that serve a model (paged_append, paged_attention, sample), as a
-PyTorch dispatcher op set: ``torch.ops.autokernel_b200.<op>``.
+PyTorch dispatcher op set: ``torch.ops.autokernel_b200.<op>``.  A schema has one form, so two of those
+have a second name: paged_append_kv appends without queries, sample_rows takes its settings per row.
 
 AutoKernel exports an optimized kernel to the Hugging Face kernels layout as a TORCH_LIBRARY
 op set (export_hf.py:367-420; examples/hf_kernels_test/torch-ext/torch_binding.cpp:6-9:
@@ -38,10 +39,14 @@ _SCHEMAS = {
                         "float? sm_scale=None) -> Tensor"),
     "paged_append": ("paged_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, "
                      "Tensor page_table, Tensor cu_q, Tensor kv_lens, Tensor q, Tensor cos, Tensor sin) -> Tensor"),
+    "paged_append_kv": ("paged_append_kv(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+                        "Tensor page_table, Tensor cu_q, Tensor kv_lens, Tensor? cos=None, Tensor? sin=None) -> ()"),
     "paged_attention": ("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, "
                         "Tensor cu_q, Tensor kv_lens, bool causal=True, float? sm_scale=None) -> Tensor"),
     "sample": ("sample(Tensor logits, Tensor u, float temperature=1.0, int top_k=0, float top_p=1.0, "
                "float min_p=0.0) -> Tensor"),
+    "sample_rows": ("sample_rows(Tensor logits, Tensor u, Tensor temperature, Tensor top_k, Tensor top_p, "
+                    "Tensor min_p) -> Tensor"),
 }
 
 
@@ -84,11 +89,19 @@ def _fake_paged_append(k, v, k_cache, v_cache, page_table, cu_q, kv_lens, q, cos
     return torch.empty_like(q)
 
 
+def _paged_append_kv(k, v, k_cache, v_cache, page_table, cu_q, kv_lens, cos=None, sin=None):
+    _ops.paged_append(k, v, k_cache, v_cache, page_table, cu_q, kv_lens, cos=cos, sin=sin)
+
+
+def _fake_paged_append_kv(*_):
+    pass
+
+
 def _fake_paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, causal=True, sm_scale=None):
     return torch.empty_like(q)
 
 
-def _fake_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+def _fake_sample(logits, *_):
     return logits.new_empty(logits.shape[0], dtype=torch.int64)
 
 
@@ -103,8 +116,10 @@ _IMPLS = {
     "fused_mlp": (_ops.fused_mlp, _fake_fused_mlp),
     "flash_attention": (_ops.flash_attention, _fake_attention),
     "paged_append": (_ops.paged_append, _fake_paged_append),
+    "paged_append_kv": (_paged_append_kv, _fake_paged_append_kv),
     "paged_attention": (_ops.paged_attention, _fake_paged_attention),
     "sample": (_ops.sample, _fake_sample),
+    "sample_rows": (_ops.sample, _fake_sample),
 }
 
 for _name, _schema in _SCHEMAS.items():

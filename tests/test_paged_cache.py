@@ -299,3 +299,36 @@ def test_a_sequence_can_be_shortened():
             c.truncate(a, n)
     with pytest.raises(KeyError):
         c.truncate(77, 0)
+
+
+def test_fake_shapes_of_the_second_forms():
+    k, cache = torch.zeros(5, 2, 64, dtype=torch.bfloat16), torch.zeros(6, 2, 16, 64, dtype=torch.bfloat16)
+    lists = [torch.zeros(*s, dtype=torch.int32) for s in ((2, 3), (3,), (2,))]
+    with FakeTensorMode() as mode:
+        f = mode.from_tensor
+        assert AK.paged_append_kv(f(k), f(k), f(cache), f(cache), *[f(t) for t in lists]) is None
+        row = f(torch.zeros(7))
+        t = AK.sample_rows(f(torch.zeros(7, 100)), row, row, f(torch.zeros(7, dtype=torch.int32)), row, row)
+        assert t.shape == (7,) and t.dtype == torch.int64
+
+
+@pytest.mark.gpu
+def test_registered_second_forms():
+    from autokernel_b200 import ops
+    g = torch.Generator("cuda").manual_seed(3)
+    k, v = (torch.randn(2, 2, 64, device="cuda", generator=g).half() for _ in range(2))
+    lists = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[0, 1], [2, 4]], [0, 1, 2], [20, 7])]
+    cos, sin = torch.rand(99, 32, device="cuda"), torch.rand(99, 32, device="cuda")
+    for tables in ((), (cos, sin)):
+        kc, vc = (torch.randn(5, 2, 16, 64, device="cuda", generator=g).half() for _ in range(2))
+        kc2, vc2 = kc.clone(), vc.clone()
+        AK.paged_append_kv(k, v, kc, vc, *lists, *tables)
+        ops.paged_append(k, v, kc2, vc2, *lists, **dict(zip(("cos", "sin"), tables)))
+        assert torch.equal(kc, kc2) and torch.equal(vc, vc2)
+        torch.library.opcheck(AK.paged_append_kv, (k, v, kc, vc, *lists, *tables),
+                              test_utils=("test_schema", "test_faketensor"))
+    x, u = torch.randn(6, 300, device="cuda", generator=g), torch.rand(6, device="cuda")
+    t, p, m = torch.rand(6, device="cuda"), torch.rand(6, device="cuda"), torch.rand(6, device="cuda") * 0.1
+    n = torch.tensor([0, 1, 5, 50, 0, 299], dtype=torch.int32, device="cuda")
+    assert torch.equal(AK.sample_rows(x, u, t, n, p, m), ops.sample(x, u, t, n, p, m))
+    torch.library.opcheck(AK.sample_rows, (x, u, t, n, p, m), test_utils=("test_schema", "test_faketensor"))
