@@ -62,6 +62,23 @@ static bool tc_ok(const AttnArgs& a) {
   return device_info().cc_major == 10;
 }
 
+// The decoding kernel for few query rows a sequence and key/value head, on average: its tiles of 16 rows each
+// read all keys and are put together row by row, where the chunk kernel's 256 rows read them once.  Rows
+// are what the host knows (N G / B); how they spread over the sequences it does not.  Measured, us, decoding
+// kernel : chunk kernel, heads of 128, bf16:
+//   rows 1   64 x 300..8100 keys, 32 heads   649 : 1008      1 x 2000, 32 heads          22 : 30
+//   rows 4   the same, 32 over 8 heads       204 : 273       16 x 300..8000, 32 over 8   82 : 80
+//   rows 8   128 x 300..4000, 32 over 8      227 : 311       1 x 4000, 32 over 8         40 : 29
+//   rows 16  64 x 300..8100, 32 over 2       121 : 87        1 x 4000, 32 over 2         61 : 28
+// Between 5 and 9 rows the joins at the ends of pieces decide: the decoding kernel is ahead where an SM has two
+// (sequence, head) pairs or more, whose loads hide them (48 x 300..8000, 32 over 8: 182 : 197), and level with
+// the other for short ones.  One sequence of two tokens among 63 of one (32 over 8) is 204 : 273; 63 and a
+// chunk of 512 299 : 464 there.  A call with room for 64 sequences that holds one chunk of 64 tokens is the
+// worst of it, 72 : 35 (nothing the host sees tells it from 64 of one).
+static bool few_rows(int64_t N, int64_t B, int64_t G, int64_t Hkv) {
+  return N * G <= 5 * B || (N * G <= 9 * B && B * Hkv >= 2 * (int64_t)device_info().sm_count);
+}
+
 }  // namespace paged
 }  // namespace ak
 
@@ -69,8 +86,8 @@ using namespace ak;
 
 extern "C" size_t ak_paged_attention_workspace_size(int64_t N, int64_t B, int64_t H, int64_t Hkv,
                                                     int64_t D, int dtype) {
-  if (dtype == AK_F32 || (D != 64 && D != 128)) return 0;
-  return N <= B ? paged::decode_workspace((int)D) : paged::chunk_workspace((int)D);
+  if (dtype == AK_F32 || (D != 64 && D != 128) || Hkv <= 0) return 0;
+  return paged::few_rows(N, B, H / Hkv, Hkv) ? paged::decode_workspace((int)D) : paged::chunk_workspace((int)D);
 }
 
 extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void* v_cache,
@@ -120,9 +137,8 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
     a.vcs[i] = v_cache_strides[i];
   }
   cudaStream_t st = (cudaStream_t)stream;
-  // No more tokens than sequences is a decoding step (any sequence may still hold several).
   if (paged::tc_ok(a))
-    return N <= B ? paged::run_decode(a, workspace, st) : paged::run_chunk(a, workspace, st);
+    return paged::few_rows(N, B, a.G, Hkv) ? paged::run_decode(a, workspace, st) : paged::run_chunk(a, workspace, st);
   switch (dtype) {
     case AK_F32: return paged::run_simt<AK_F32>(a, st);
     case AK_F16: return paged::run_simt<AK_F16>(a, st);

@@ -52,7 +52,8 @@ struct Weight {
   }
 };
 
-// paged_decode.cu: 16 query rows per tile, all keys read once; paged_chunk.cu: 128-row tensor-core tiles.
+// paged_decode.cu: tiles of 16 query rows, each of which reads all of its keys; paged_chunk.cu: two tensor-core
+// tiles of 128.  Either takes any lists; paged_attn.cu chooses.
 int run_decode(const AttnArgs& a, void* ws, cudaStream_t st);
 size_t decode_workspace(int D);
 int run_chunk(const AttnArgs& a, void* ws, cudaStream_t st);

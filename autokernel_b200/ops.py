@@ -725,6 +725,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     token per sequence is decoding.  H is a multiple of the cache's heads: query head h reads
     key/value head h // (H // Hkv).  head_dim up to 256; sm_scale (D ** -0.5 by default) positive.
 
+    Weights and sums are fp32.  In 16-bit types a call of few query rows per sequence and key/value head (5
+    on average, 9 in large batches) keeps two 16-bit terms of each weight for the product with the values,
+    any other rounds weights once: the last bits of a row depend on which of the two its batch takes.
+
     Returns [N, H, D] (written to out if given: any strides with a contiguous last dim, and none of
     the inputs' memory).  A row that sees no key (or only scores of -inf) is 0; one that sees a key
     without a page is NaN, and in 16-bit types one whose largest score (scaled) is 9.3e7 (fp16) or 1.5e9

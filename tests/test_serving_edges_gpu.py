@@ -243,3 +243,44 @@ def test_infinite_temperature_among_dead_logits(dt, vocab):
         got = ops.sample(x, u, temperature=math.inf, **kw).tolist()
         kw = {k: float(np.float32(v)) if k != "top_k" else v for k, v in kw.items()}
         assert got == [serve_f64.sample_row(x[r].double().cpu().numpy(), u[r].item(), math.inf, **kw) for r in range(12)]
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,D,seqs", [
+    (64, 8, 128, [(1, 20 + 37 * i) for i in range(40)]),                     # 8 rows a sequence, many pairs
+    (64, 8, 64, [(1, 700)] * 3),                                             # 8 rows, few pairs
+    (32, 2, 128, [(1, 333), (1, 64), (1, 1)]),                               # 16
+    (40, 1, 64, [(1, 500), (1, 3)]),                                         # 40
+    (32, 8, 128, [(1, 50 + i) for i in range(50)] + [(2, 99)]),              # one of two tokens
+    (16, 8, 64, [(0, 0)] * 30 + [(61, 400), (1, 77)] + [(0, 0)] * 30),       # slots, one of them a chunk
+    (8, 8, 128, [(5, 90), (9, 9), (4, 250)] + [(1, 30 + i) for i in range(40)])])
+def test_groups_and_batches_of_all_widths(heads, kv, D, seqs, dt):
+    """Calls on both sides of the rule that chooses a kernel, each row against the formula."""
+    q, kc, vc, lists, first = packed(seqs, heads, kv, D, DTS[dt], seed=heads + D)
+    o = ops.paged_attention(q, kc, vc, *lists)
+    rows = [(b, i) for b, (new, _) in enumerate(seqs) for i in sorted({0, new // 2, new - 1}) if new]
+    near_64_bits(q, kc, vc, lists, seqs, first, o, rows, sorted({0, heads // 2, heads - 1}))
+
+
+@pytest.mark.parametrize("heads,kv,n", [(32, 2, 1), (8, 8, 3)])
+def test_a_call_whose_lists_change_under_a_graph(heads, kv, n):
+    """64 slots, captured once: the lists may spread the tokens over the sequences in any way."""
+    B, D, page = 64, 128, 16
+    g = torch.Generator(DEV).manual_seed(9)
+    q = torch.randn(B * n, heads, D, device=DEV, generator=g).half()
+    kc, vc = (torch.randn(B * 4, kv, page, D, device=DEV, generator=g).half() for _ in range(2))
+    table = torch.arange(B * 4, device=DEV, dtype=I32).view(B, 4)
+    cu, lens = torch.zeros(B + 1, dtype=I32, device=DEV), torch.zeros(B, dtype=I32, device=DEV)
+    out = torch.empty_like(q)
+    ops.paged_attention(q, kc, vc, table, cu, lens)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_attention(q, kc, vc, table, cu, lens, out=out)
+    for seqs in ([(n, 20 + b % 40) for b in range(B)], [(0, 0)] * 60 + [(40, 64), (0, 9), (23, 30), (1, 1)], [(0, 64)] * B):
+        cu.copy_(torch.tensor([sum(s[0] for s in seqs[:i]) for i in range(B + 1)], dtype=I32))
+        lens.copy_(torch.tensor([s[1] for s in seqs], dtype=I32))
+        out.fill_(7.0)
+        graph.replay()
+        rows = [(b, s[0] - 1) for b, s in enumerate(seqs) if s[0]]
+        near_64_bits(q, kc, vc, (table, cu, lens), seqs, [4 * b for b in range(B)], out, rows, [0, heads - 1])
+        assert (out[int(cu[-1]):] == 7).all()
