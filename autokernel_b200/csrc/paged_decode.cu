@@ -46,13 +46,17 @@ struct DecodeCfg {
   static constexpr int SMEM = O_OFF + kWarps / 2 * kRows * D * 4 + 1024;
 };
 
-// Rounds of pieces where the tables could name a long line (paged_sched.cuh; a shorter one that turns
-// out is cut into single pieces, whose spare CTAs then only cost their cancellation).
+// Rounds of pieces (paged_sched.cuh) where the tables could name a long line: four times the shortest share,
+// since what they name is twice what is there or more in a batch of mixed lengths, and single pieces are the
+// better ones for even lengths (159 : 170 us at 12,000 keys an SM).  Where the line turns out shorter, it is cut
+// into single pieces, and the spare CTAs only cost their cancellation.  Fewer than 4 (sequence, head) pairs for 3
+// SMs are cut into more parts by rounds than these gain: 160 pairs of 11,000 keys 162 : 183 us, 24 of 74,000 166 : 215.
 static TileRule decode_rule(const AttnArgs& a) {
   const int ctas = device_info().sm_count;
+  const int64_t pairs = (int64_t)a.l.B * a.Hkv;
   const double tiles = (double)a.l.B + (double)a.l.N * a.G / kRows;
   const double keys = tiles * a.Hkv * ((double)a.l.max_pages * a.l.page_size + 64);
-  return TileRule{kRows, 0, 6, 64, 0, 256, ctas, keys / ctas >= 4 * kLongPiece && a.l.B <= 512 ? kRounds : 1};
+  return TileRule{kRows, 0, 6, 64, 0, 256, ctas, keys / ctas >= 4 * kLongPiece && 3 * pairs >= 4 * ctas ? kRounds : 1};
 }
 
 static size_t decode_part_floats(int D) { return (size_t)kRows * (D + 2); }

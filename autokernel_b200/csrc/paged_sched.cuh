@@ -9,10 +9,14 @@
 // not depend on timing.
 //
 // Equal pieces do not take equal time when memory is the bound: decoding 64 sequences of up to 8K
-// keys, the first of 148 CTAs was done after 164 us and the last after 215.  Long lines are
-// therefore cut into five rounds of pieces, 46, 8, 5, 3 and 2 64ths of an equal share, and a CTA
-// that is done takes the next piece that has not begun (the hardware's cancellation of a CTA that
-// waits to be launched hands its number over).
+// keys, the first of 148 CTAs was done after 164 us and the last after 215; many short tiles take longer
+// than their keys say.  Long lines are therefore cut into five rounds of pieces, 32, 16, 8, 5 and 3 64ths
+// of an equal share, and a CTA that is done takes the next piece that has not begun (the hardware's
+// cancellation of a CTA that waits to be launched hands its number over).  Decoding, 32 heads of 128, us, single
+// pieces : rounds (of 46, 8, 5, 3, 2 / 54, 4, 3, 2, 1 64ths):
+//   over 8, 64 x 300..8100 keys  204 : 196 (198 / 213)    over 32, 16 x 300..8000  211 : 184 (184 / 189)
+//   over 8, 512 x 100..2000      590 : 431 (448 / 513)    over 8, 2048 x 50..600  1238 : 924 (946 / 1086)
+//   over 8, 64 x 4000            179 : 187 (188 / 193)    over 8, 3 x 74000        166 : 215 (few tiles, many parts)
 #pragma once
 #include "paged_row.cuh"
 
@@ -108,14 +112,14 @@ AK_D void set_blocks(const AttnArgs& a, const TileRule& t, int64_t cost, int64_t
 
 // How a line is cut into pieces.
 constexpr int kRounds = 5;
-constexpr int64_t kLongPiece = 4096;  // shortest equal share that is worth rounds
+constexpr int64_t kLongPiece = 4096;  // shortest equal share that is worth rounds (3000: 64 : 76, 66 : 77 us)
 struct Cut {
   int64_t unit;  // a piece of round r is size(r) units long
   int ctas;
   bool rounds;
-  // 46, 8, 5, 3, 2 of 64
-  AK_D static int size(int r) { return r == 0 ? 46 : r == 1 ? 8 : r == 2 ? 5 : r == 3 ? 3 : 2; }
-  AK_D static int before(int r) { return r == 0 ? 0 : r == 1 ? 46 : r == 2 ? 54 : r == 3 ? 59 : r == 4 ? 62 : 64; }
+  // 32, 16, 8, 5, 3 of 64
+  AK_D static int size(int r) { return r == 0 ? 32 : r == 1 ? 16 : r == 2 ? 8 : r == 3 ? 5 : 3; }
+  AK_D static int before(int r) { return r == 0 ? 0 : r == 1 ? 32 : r == 2 ? 48 : r == 3 ? 56 : r == 4 ? 61 : 64; }
   AK_D int64_t start(int piece) const {
     if (!rounds) return piece * unit;
     const int r = piece / ctas;

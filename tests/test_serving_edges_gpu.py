@@ -284,3 +284,26 @@ def test_a_call_whose_lists_change_under_a_graph(heads, kv, n):
         rows = [(b, s[0] - 1) for b, s in enumerate(seqs) if s[0]]
         near_64_bits(q, kc, vc, (table, cu, lens), seqs, [4 * b for b in range(B)], out, rows, [0, heads - 1])
         assert (out[int(cu[-1]):] == 7).all()
+
+
+@pytest.mark.parametrize("dt,D", [("f16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("seqs", [
+    [(1, 100 + b) for b in range(20)] + [(1, 26000), (3, 25000), (1, 27000)] + [(1, 1 + b) for b in range(15)] + [(0, 50), (0, 0)],
+    [(1, 90 + b % 40) for b in range(600)] + [(1, 400), (2, 700)]])
+def test_decoding_in_rounds_of_pieces(seqs, D, dt):
+    """Lines long enough for rounds, with tiles that several pieces share and pieces that hold many tiles; then
+    other lists under the same captured call, a short line among them."""
+    q, kc, vc, lists, first = packed(seqs, 16, 8, D, DTS[dt], seed=D)
+    o = ops.paged_attention(q, kc, vc, *lists)
+    live = [b for b, s in enumerate(seqs) if s[0]]
+    some = sorted({*live[:2], *live[len(live) // 2 - 2:len(live) // 2 + 4], *live[-3:]})
+    near_64_bits(q, kc, vc, lists, seqs, first, o, [(b, seqs[b][0] - 1) for b in some], [0, 7, 15])
+    out, graph = torch.empty_like(q), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_attention(q, kc, vc, *lists, out=out)
+    graph.replay()
+    assert torch.equal(out, o)
+    short = [(n, min(x, 40 + b % 30)) for b, (n, x) in enumerate(seqs)]
+    lists[2].copy_(torch.tensor([s[1] for s in short], dtype=I32))
+    graph.replay()
+    near_64_bits(q, kc, vc, lists, short, first, out, [(b, short[b][0] - 1) for b in some], [0, 15])
