@@ -31,6 +31,15 @@ def rotate(x, cos, sin):
     return y
 
 
+def rotate_size(x, cos, sin):
+    """What rotate adds up in each element, |x1 c| + |x2 s| or |x1 s| + |x2 c|: the scale of its fp32 rounding."""
+    a, b = np.abs(x[..., 0::2]), np.abs(x[..., 1::2])
+    y = np.empty_like(x)
+    y[..., 0::2] = a * np.abs(cos) + b * np.abs(sin)
+    y[..., 1::2] = a * np.abs(sin) + b * np.abs(cos)
+    return y
+
+
 def paged_append(k, v, k_cache, v_cache, page_table, cu_q, kv_lens, q=None, cos=None, sin=None):
     """(k_cache, v_cache, q) after the append; q keeps its values outside every sequence."""
     k_cache, v_cache = k_cache.copy(), v_cache.copy()

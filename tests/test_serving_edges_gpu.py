@@ -307,3 +307,30 @@ def test_decoding_in_rounds_of_pieces(seqs, D, dt):
     lists[2].copy_(torch.tensor([s[1] for s in short], dtype=I32))
     graph.replay()
     near_64_bits(q, kc, vc, lists, short, first, out, [(b, short[b][0] - 1) for b in some], [0, 15])
+
+
+@pytest.mark.parametrize("dt", list(DTS))
+@pytest.mark.parametrize("heads,kv,D,page", [(8, 2, 128, 16), (3, 1, 80, 5), (2, 2, 6, 3), (32, 32, 64, 64)])
+def test_append_rotation_element_by_element(dt, heads, kv, D, page):
+    """Each rotated element within h |e| (2^-25 where fp16 is subnormal) + 3 * 2^-24 of what its own sum adds up:
+    two fp32 products, their sum, one rounding.  Sizes from 1e-3 to 1e3 within a vector."""
+    from oracle import serve_f64
+    dt, seqs = DTS[dt], [(7, 23), (1, 90), (40, 64), (0, 3), (130, 131)]
+    g = torch.Generator(DEV).manual_seed(D)
+    q, kc, vc, lists, first = packed(seqs, heads, kv, D, dt, page, seed=D)
+    k = torch.randn(q.shape[0], kv, D, device=DEV, generator=g)
+    spread = 10 ** (6 * torch.rand(D, device=DEV, generator=g) - 3)
+    q, k = (q * spread).to(dt), (k * spread).to(dt)
+    angle = torch.rand(140, D // 2, device=DEV, generator=g, dtype=torch.float64) * 6.3
+    cos, sin = angle.cos().float(), angle.sin().float()
+    out = ops.paged_append(k, k, kc, vc, *lists, q=q, cos=cos, sin=sin)
+    h, floor = _half(dt), 2.0 ** -25 if dt == torch.float16 else 0
+    cu, n64 = lists[1].tolist(), lambda t: t.double().cpu().numpy()  # noqa: E731
+    for b, (new, length) in enumerate(seqs):
+        at = np.arange(length - new, length)
+        c, s = n64(cos)[at][:, None], n64(sin)[at][:, None]
+        stored = kc[first[b] + torch.tensor(at // page, device=DEV), :, torch.tensor(at % page, device=DEV)]
+        for x, y in ((q, out[cu[b]:cu[b + 1]]), (k, stored)):
+            x = n64(x[cu[b]:cu[b + 1]])
+            e, size = serve_f64.rotate(x, c, s), serve_f64.rotate_size(x, c, s)
+            assert (np.abs(n64(y) - e) <= np.maximum(h * np.abs(e), floor) + 3 * 2.0 ** -24 * size).all()
