@@ -19,18 +19,19 @@
 // and output of their own, and tile 0's threads join the two in the epilogue (a warp reads the
 // TMEM lanes of its quarter of either tile).
 //
-// Measured: two prompts of 4096 and 3700 tokens, 32 heads of 128, bf16, pages of 64: 350 us, 714 TFLOP/s (a
-// block's softmax takes longer than its two products, and a segment's start and end, which nothing
-// overlaps, cost several us).  501 tokens on 7600 keys, 32 heads over 8: 91 us, 705 TFLOP/s.  24
-// sequences of up to 96 tokens on up to 1500 keys, 12 heads of 64: 56 us, where reading the keys
-// alone would take 10: 288 tiles of a few blocks each, whose starts and ends bound it.  What runs once
-// per segment or block row (masks, the epilogue) is kept short: its instructions are not at hand when
-// their turn comes (masks and epilogue unrolled over a row's registers: 380 us, 99 us and 60 us).
+// Measured: two prompts of 4096 and 3700 tokens, 32 heads of 128, bf16, pages of 64: 337 us, 741 TFLOP/s
+// (360 us when called without a pause, where the clock gives way; a block's softmax takes longer than its
+// two products, and a segment's start and end, which nothing overlaps, cost several us).  501 tokens on 7600
+// keys, 32 heads over 8: 87 us, 739 TFLOP/s.  24 sequences of up to 96 tokens on up to 1500 keys, 12 heads
+// of 64: 57 us, where reading the keys alone would take 10: 288 tiles of a few blocks each, whose starts and
+// ends bound it.  What runs once per segment or block row (masks, the epilogue) is kept short: its
+// instructions are not at hand when their turn comes (unrolled over a row's registers they took 380, 99 and
+// 60 us, where the loops took 350, 91 and 56).
 //
-// P is rounded to 16 bits once, as the matrix unit takes it (a second term, as the decoding kernel has
-// it, would be half as much matrix work again, and its columns are where S lies); reference, sum and
-// output are fp32.  It costs a third on top of the result's own rounding: the relative error of the
-// chunk below is 2.3e-3 in bf16, where one rounding of exact results has 1.7e-3.
+// P is rounded to 16 bits once, as the matrix unit takes it; reference, sum and output are fp32.  A second
+// term of P, as the decoding kernel has it, would be half as much matrix work again, and as many more
+// conversions and stores for the softmax threads, which bound the kernel.  Without it the relative error of
+// the chunk above is 2.3e-3 in bf16, where exact results rounded once have 1.7e-3.
 // Slots of the last page behind the last visible key may hold anything, NaN included: the
 // producer zeroes their V rows before the matrix unit sees them (their scores are masked).
 #include "attn_softmax.cuh"

@@ -14,8 +14,8 @@
 //               its own reference (Weight), sum and output, joined through shared memory per segment
 // One CTA per SM; the line of paged_sched.cuh gives each the same number of keys.
 //
-// Measured: 64 sequences of 300 to 8100 keys, 32 heads over 8 of 128, fp16, pages of 16: 202 us, 5.45 TB/s
-// (83% of a plain copy's rate).  One sequence of 2011 keys, 32 heads of 128: 22 us, where the rate
+// Measured: 64 sequences of 300 to 8100 keys, 32 heads over 8 of 128, fp16, pages of 16: 194 us, 5.69 TB/s
+// (87% of a plain copy's rate).  One sequence of 2011 keys, 32 heads of 128: 22.5 us, where the rate
 // alone would take 5: the rest is latency, of the launch, of the lists and page numbers before the
 // first copy can leave (2 us), of one ring fill and two joins per CTA and of the joining kernel (2 us).
 //
