@@ -20,7 +20,7 @@
 // TMEM lanes of its quarter of either tile).
 //
 // Measured: two prompts of 4096 and 3700 tokens, 32 heads of 128, bf16, pages of 64: 337 us, 741 TFLOP/s
-// (360 us when called without a pause, where the clock gives way; a block's softmax takes longer than its
+// (360 to 371 us when called without a pause, where the clock gives way; a block's softmax takes longer than its
 // two products, and a segment's start and end, which nothing overlaps, cost several us).  501 tokens on 7600
 // keys, 32 heads over 8: 87 us, 739 TFLOP/s.  24 sequences of up to 96 tokens on up to 1500 keys, 12 heads
 // of 64: 57 us, where reading the keys alone would take 10: 288 tiles of a few blocks each, whose starts and

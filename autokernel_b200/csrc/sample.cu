@@ -175,9 +175,9 @@ __global__ void __launch_bounds__(512) sample_kernel(const SampleArgs a) {
 //   4  kept weights per run of 32 vectors, then the run, the lane and the entry that u falls in
 //
 // Bound by 64-bit exponentials and the passes' synchronisation rather than by memory: 192 rows of 131072
-// fp32 logits, top-p 0.9, take 299 us (337 GB/s of logits; a CTA's sums of 64-bit weights are a quarter of it,
+// fp32 logits, top-p 0.9, take 296 us (341 GB/s of logits; a CTA's sums of 64-bit weights are a quarter of it,
 // the histograms' merges and the leader's searches a third); 256 rows of 32000 in bf16 with settings of
-// their own 79 us; one row with top-k and top-p 20 us, about ten cluster barriers and a launch.  256 rows of
+// their own 78 us; one row with top-k and top-p 20 us, about ten cluster barriers and a launch.  256 rows of
 // 32000: temperature alone 36 us, top-k 50 34 us, greedy 9.
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1536, kList = 128, kNear = 2048;
 constexpr int kMaxSlice = 160 * 1024;                   // bytes of a row per CTA
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __gri
             for (int e = 0; e < VEC; ++e) {  // no branch: the chains of operations overlap
               const double x = w(f[e]);
               if (f[e] > f_hi) above += x;
-              if (f[e] < f_lo && alive(f[e])) below += x;  // (a dead entry's x is NaN at T = inf)
+              if (f[e] < f_lo) below += x;
               some |= (unsigned)(f[e] <= f_hi && f[e] >= f_lo) << e;
             }
             while (some) {  // their bins come later, from all threads at once
@@ -419,6 +419,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const __gri
           }
           above = warp_sum_d(above);
           if (lane == 0) s.run[v * kWarps + warp] = above;
+        }
+        if (!(below >= 0.0)) {  // T = inf: a dead entry's x is NaN, any other's 1 (a test of each x cost 2%)
+          below = 0.0;
+#pragma unroll 1
+          for (int j = tid; j < nv * kThreads; j += kThreads)
+#pragma unroll 1
+            for (int e = 0; e < VEC; ++e) below += alive(entry(j, e)) && entry(j, e) < f_lo;
         }
         below = warp_sum_d(below);
         if (lane == 0) s.red[warp] = below;
