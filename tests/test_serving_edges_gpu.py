@@ -334,3 +334,27 @@ def test_append_rotation_element_by_element(dt, heads, kv, D, page):
             x = n64(x[cu[b]:cu[b + 1]])
             e, size = serve_f64.rotate(x, c, s), serve_f64.rotate_size(x, c, s)
             assert (np.abs(n64(y) - e) <= np.maximum(h * np.abs(e), floor) + 3 * 2.0 ** -24 * size).all()
+
+
+def test_calls_on_several_streams_at_once():
+    """Decoding in rounds, decoding of one, chunks and sampling side by side: each as if it were alone."""
+    def attention(seqs, heads, kv, D):
+        q, kc, vc, lists, _ = packed(seqs, heads, kv, D, torch.float16, seed=len(seqs))
+        return lambda: ops.paged_attention(q, kc, vc, *lists)
+
+    g = torch.Generator(DEV).manual_seed(1)
+    x, u = torch.randn(40, 30000, device=DEV, generator=g), torch.rand(40, device=DEV, generator=g)
+    calls = [attention([(1, 100 + 97 * i) for i in range(48)], 32, 8, 128), attention([(1, 3000)], 8, 8, 64),
+             attention([(130, 2000), (1, 700), (33, 33)], 8, 2, 128), lambda: ops.sample(x, u, 0.9, 0, 0.8)]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for turn in range(20):
+        got = []
+        for i, (f, s) in enumerate(zip(calls, streams)):
+            with torch.cuda.stream(s):
+                got.append([f() for _ in range(1 + (turn + i) % 3)])
+        torch.cuda.synchronize()
+        for w, results in zip(want, got):
+            assert all(torch.equal(w, r) for r in results)
+    assert device_status() == 0
