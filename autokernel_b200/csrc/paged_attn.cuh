@@ -38,9 +38,11 @@ struct Weight {
   static constexpr float kLag = DT == AK_F16 ? 4.f : 8.f;
   // Scores are fp32, and so is r.  From 2^23 on its steps are 1 and more: fp16 scores are rounded up to
   // it, so that no weight passes 2^15, and up to kLimit the largest one is at least 1 (in bf16,
-  // between 2^-64 and 2^72).  A row whose largest score lies beyond is NaN: its weights would be
-  // infinite or all 0, and its scores have lost what tells them apart.
+  // between 2^-64 and 2^72).  A row whose largest score lies beyond, on either side, is NaN: its weights
+  // would be infinite or all 0, and its scores have lost what tells them apart.  Scores below -kLimit
+  // beside larger ones weigh 0.
   static constexpr float kLimit = DT == AK_F16 ? 134217728.f : 2147483648.f;  // 2^27, 2^31
+  static constexpr float kFar = -3.4028235e38f;  // r of a row of which only scores below -kLimit were seen
   // the largest score of a block, scaled
   static AK_D float top(float score, float scale_log2) {
     return DT == AK_F16 ? __fmul_ru(score, scale_log2) : __fmul_rn(score, scale_log2);
@@ -48,8 +50,12 @@ struct Weight {
   // whether a block with this top moves r, and where to (r = -inf: nothing has been seen yet)
   static AK_D bool moves(float top, float r) { return top - r > kShift + kLag; }
   static AK_D float reference(float top) {
-    return fabsf(top) < kLimit ? __fsub_ru(top, kShift) : __int_as_float(0x7fffffff);
+    return fabsf(top) < kLimit ? __fsub_ru(top, kShift) : top < 0.f ? kFar : __int_as_float(0x7fffffff);
   }
+  // what is subtracted from scores: with no r to subtract, the exponential of what was seen is 0
+  static AK_D float base(float r) { return r <= kFar ? 0.f : r; }
+  // a row's sum of weights, from that sum and r over all of its keys
+  static AK_D float total(float sum, float r) { return r == kFar ? __int_as_float(0x7fffffff) : sum; }
 };
 
 // paged_decode.cu: tiles of 16 query rows, each of which reads all of its keys; paged_chunk.cu: two tensor-core

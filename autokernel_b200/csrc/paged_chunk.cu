@@ -19,10 +19,10 @@
 // and output of their own, and tile 0's threads join the two in the epilogue (a warp reads the
 // TMEM lanes of its quarter of either tile).
 //
-// Measured: two prompts of 4096 and 3700 tokens, 32 heads of 128, bf16, pages of 64: 337 us, 741 TFLOP/s
+// Measured: two prompts of 4096 and 3700 tokens, 32 heads of 128, bf16, pages of 64: 339 us, 736 TFLOP/s
 // (360 to 371 us when called without a pause, where the clock gives way; a block's softmax takes longer than its
 // two products, and a segment's start and end, which nothing overlaps, cost several us).  501 tokens on 7600
-// keys, 32 heads over 8: 87 us, 739 TFLOP/s.  24 sequences of up to 96 tokens on up to 1500 keys, 12 heads
+// keys, 32 heads over 8: 89 us, 720 TFLOP/s.  24 sequences of up to 96 tokens on up to 1500 keys, 12 heads
 // of 64: 57 us, where reading the keys alone would take 10: 288 tiles of a few blocks each, whose starts and
 // ends bound it.  What runs once per segment or block row (masks, the epilogue) is kept short: its
 // instructions are not at hand when their turn comes (unrolled over a row's registers they took 380, 99 and
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           tmem_wait_st();
         }
-        const float mr = m_ref == -INFINITY ? 0.f : m_ref;
+        const float mr = Weight<DT>::base(m_ref);
         float2 sum2[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -507,6 +507,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_after();
       used[0] += took[0];
       used[1] += took[1];
+      if (s.whole) l = Weight<DT>::total(l, m_ref);
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* orow = reinterpret_cast<T*>(a.o) + (int64_t)(s.r.begin + tok) * a.os[0] +
                 (int64_t)(s.h * a.G + row % a.G) * a.os[1];
@@ -639,6 +640,7 @@ __global__ void __launch_bounds__(128)
   }
   bool odd = false;
   if (valid) {
+    sum = Weight<DT>::total(sum, top);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T* orow = reinterpret_cast<T*>(a.o) + (int64_t)(s.r.begin + tok) * a.os[0] +
               (int64_t)(s.h * a.G + row % a.G) * a.os[1] + part_d * (D / 4);

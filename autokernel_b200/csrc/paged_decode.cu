@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t ph[4], pl[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float ref = m[i] == -INFINITY ? 0.f : m[i];
+          const float ref = Weight<DT>::base(m[i]);
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
             const float x = ex2_approx(fmaf(sc[n][2 * i], a.scale_log2, -ref));
@@ -469,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int v = visible_keys(s.r, t, a.causal);
         if (v > first_bad) sum = __int_as_float(0x7fffffff);
         if (s.whole) {
+          sum = Weight<DT>::total(sum, top);
           const float y = sum == 0.f ? 0.f : x / sum;
           if (again && !(fabsf(y) <= 3.4028235e38f) && fabsf(sum) <= 3.4028235e38f && v < s.kv_hi)
             marks[now->part >> 1] = 1;
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(128, 5)  // (a block per piece of five rounds 
       }
     }
     if (row >= nr) break;
-    const float l = sum, out = l == 0.f ? 0.f : x / l;
+    const float l = Weight<DT>::total(sum, top), out = l == 0.f ? 0.f : x / l;
     const int t = (row0 + row) / a.G, hg = (row0 + row) % a.G;
     if (!(fabsf(out) <= 3.4028235e38f) && fabsf(l) <= 3.4028235e38f &&
         visible_keys(s.r, t, a.causal) < s.kv_hi)

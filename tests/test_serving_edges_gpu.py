@@ -358,3 +358,38 @@ def test_calls_on_several_streams_at_once():
         for w, results in zip(want, got):
             assert all(torch.equal(w, r) for r in results)
     assert device_status() == 0
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("new", [1, 40, 300])
+@pytest.mark.parametrize("far", ["first", "last", "most", "all but one", "all"])
+def test_scores_far_below_the_others(dt, new, far):
+    """Keys whose scores are -3e8 (fp16) or -1e10: beside others they weigh nothing, wherever they lie; a row that
+    sees no others is NaN in 16 bits (no 16-bit weights reach from there), a mean of their values in fp32."""
+    dt, L, D = DTS[dt], 3000, 64
+    g = torch.Generator(DEV).manual_seed(6)
+    k, v = (torch.randn(L, D, device=DEV, generator=g) for _ in range(2))
+    q = torch.randn(new, 2, D, device=DEV, generator=g)
+    at = torch.zeros(L, dtype=torch.bool, device=DEV)
+    if far == "first":
+        at[:1700] = True
+    elif far == "last":
+        at[1300:] = True
+    else:
+        at[:] = True
+        at[{"most": torch.arange(5, L, 97), "all but one": torch.tensor([1234]), "all": torch.arange(0)}[far]] = False
+    big = 3e4 if dt == torch.float16 else 1e5
+    k[:, 0], q[..., 0] = torch.where(at, -big / 3 if dt == torch.float16 else -big, 0.0), big
+    q, k, v = q.to(dt), k.to(dt), v.to(dt)
+    kc, vc, lists = one_sequence(k, v, new, L)
+    o = ops.paged_attention(q, kc, vc, *lists, causal=False, sm_scale=1.0).double()
+    if far == "all":
+        assert o.isfinite().all() if dt == torch.float32 else o.isnan().all()
+        return
+    s = torch.where(at, -math.inf, q.double() @ k.double().T)
+    w = torch.softmax(s, -1)
+    e, A, h = w @ v.double(), w @ v.double().abs(), _half(dt)
+    d = (D + 8) * 2.0 ** -24 * (q.double().abs() @ torch.where(at[:, None], 0.0, k.double()).abs().T).amax(-1, keepdim=True)
+    floor = (2.0 ** -36 if dt == torch.float16 else 0) * v.double().abs().sum(0)
+    tol = torch.clamp(h * e.abs(), min=2.0 ** -25 if dt == torch.float16 else 0) + (h + 2 * (d + 2.0 ** -20) + (L + 8) * 2.0 ** -23) * A + floor
+    assert ((o - e).abs() <= tol).all()
