@@ -294,11 +294,11 @@ class LlamaB200:
                  generator: torch.Generator | None = None,
                  cache: PagedCache | None = None) -> list[list[int]]:
         """Continue each prompt (token lists, at least one token each) by up to max_new_tokens sampled
-        tokens (ops.sample's settings, each a number or one per prompt; temperature 0 takes the likeliest).
-        A sequence ends with the token `stop`, if given.  All sequences decode together; with `cache` they share its pages, each
-        giving its own back when it ends, otherwise one of the right size is made.  Raises CacheFull when a
-        step finds no pages, with the tokens sampled so far as its `answers`, and AkError when a step's logits
-        held nothing to draw (all NaN)."""
+        tokens (ops.sample's settings, each a number or one per prompt; temperature 0 takes the
+        likeliest).  A sequence ends with the token `stop`, if given.  All sequences decode together; with
+        `cache` they share its pages, each giving its own back when it ends, otherwise one of the right
+        size is made.  Raises CacheFull when a step finds no pages, with the tokens sampled so far as its
+        `answers`, and AkError when a step's logits held nothing to draw (all NaN)."""
         if not prompts or min(len(p) for p in prompts) < 1 or max_new_tokens < 0:
             raise ValueError("generate: need prompts of at least one token")
         vocab = self.w["tok_embeddings.weight"].shape[0]
